@@ -60,6 +60,17 @@ class Conv3dDesc(ctypes.Structure):
         "padding_right", "padding_front", "padding_back", "weight_layout", "bias")]
 
 
+class KVCacheDesc(ctypes.Structure):
+    _fields_ = [("pages", ctypes.c_int64)] + [(n, ctypes.c_int32) for n in (
+        "page_size", "heads_q", "heads_kv", "head_dim", "bits", "causal")] + [("scale", ctypes.c_float)]
+
+
+class KVCacheBatchDesc(ctypes.Structure):
+    """mm4_kv_cache_batch: sizes, and the device addresses of the page table, the lengths and the offsets."""
+    _fields_ = [(n, ctypes.c_int32) for n in ("sequences", "tokens", "max_new", "pages_per_sequence")] + [
+        (n, ctypes.c_void_p) for n in ("page_table", "lengths", "offsets")]
+
+
 class PeerHandle(ctypes.Structure):
     """mm4_peer_handle: a CUDA IPC memory handle as plain bytes."""
     _fields_ = [("bytes", ctypes.c_ubyte * 64)]
@@ -67,6 +78,7 @@ class PeerHandle(ctypes.Structure):
 
 _vp = ctypes.c_void_p
 _i32 = ctypes.c_int32
+_i64 = ctypes.c_int64
 _sz = ctypes.c_size_t
 
 # name -> (restype, argtypes); every symbol include/mm4.h declares.
@@ -114,6 +126,15 @@ SIGNATURES = {
     "mm4_attention_bwd_host": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, ctypes.c_size_t, ctypes.c_int32, _vp]),
     "mm4_attention_bwd_workspace_size": (_sz, [_vp]),
     "mm4_attention_bwd": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "mm4_kv_cache_plan_create": (ctypes.c_int, [ctypes.POINTER(_vp), ctypes.POINTER(KVCacheDesc)]),
+    "mm4_kv_cache_plan_destroy": (None, [_vp]),
+    "mm4_kv_cache_page_bytes": (_sz, [_vp]),
+    "mm4_kv_cache_bytes": (_sz, [_vp]),
+    "mm4_kv_cache_append": (ctypes.c_int, [_vp, _vp, _vp, _i64, _vp, _i64, _vp, _vp]),
+    "mm4_kv_cache_read": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp]),
+    "mm4_kv_cache_attention_workspace_size": (_sz, [_vp, _vp]),
+    "mm4_kv_cache_attention": (ctypes.c_int, [_vp, _vp, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _sz, _vp]),
+    "mm4_kv_cache_attention_kernel_name": (ctypes.c_char_p, [_vp, _vp]),
     "mm4_conv2d_plan_create": (ctypes.c_int, [ctypes.POINTER(_vp), ctypes.POINTER(Conv2dDesc)]),
     "mm4_conv3d_plan_create": (ctypes.c_int, [ctypes.POINTER(_vp), ctypes.POINTER(Conv3dDesc)]),
     "mm4_conv_plan_destroy": (None, [_vp]),

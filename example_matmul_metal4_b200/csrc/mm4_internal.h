@@ -64,6 +64,14 @@ mm4_status launch_debug_wait(int* word, uint64_t timeout_ns, cudaStream_t stream
 // synchronised the stream. Defined in mm4_noalloc.cu.
 mm4_status noalloc_take_status(int dev, int* code);
 
+// Reads and clears the status words of the key / value cache kernels on device
+// `dev` (both 0 when none ever ran there); the caller has synchronised the
+// stream. `wait` is a run-out wait, `data` what the kernels found wrong in a
+// batch's arrays. Defined in mm4_kv_cache.cu.
+mm4_status kv_cache_take_status(int dev, int* wait, int* data);
+// What a data site of the key / value cache kernels stands for.
+const char* kv_cache_site_text(int site);
+
 // cuTensorMapEncodeTiled through the runtime's driver entry point (no link
 // dependency on libcuda, so the library loads on machines without a GPU).
 mm4_status encode_tiled(CUtensorMap* map, CUtensorMapDataType dtype, uint32_t rank, const void* base,

@@ -1,0 +1,268 @@
+// Key / value cache plans and dispatch: argument checks, launches and the
+// status words of the mm4_kv_cache_* entry points.
+#include <algorithm>
+#include <atomic>
+#include <cmath>
+#include <cstdio>
+#include <new>
+
+#include "kv_attention_sm100.cuh"
+#include "kv_cache_sm100.cuh"
+#include "mm4_internal.h"
+
+using namespace mm4;
+
+struct mm4_kv_cache_plan {
+  mm4_kv_cache_desc d;
+  float scale;
+  int page_shift;
+  long long page_bytes;
+};
+
+namespace {
+
+constexpr int kMaxDevices = 64;
+// Set once a kernel that can write the status words was launched on a device;
+// before that mm4_check has nothing to read there.
+std::atomic<bool> g_used[kMaxDevices];
+
+int row_bytes(const mm4_kv_cache_desc& d) { return d.head_dim * d.bits / 8 + d.head_dim / KV_GROUP * 4; }
+
+mm4_status check_batch(const mm4_kv_cache_plan* p, const mm4_kv_cache_batch* b) {
+  if (!p) return fail(MM4_ERR_INVALID, "null plan");
+  if (!b) return fail(MM4_ERR_INVALID, "null batch");
+  if (b->sequences < 0 || b->tokens < 0 || b->max_new < 0 || b->pages_per_sequence < 0)
+    return fail(MM4_ERR_INVALID, "batch sizes must not be negative");
+  if (b->sequences == 0 || b->tokens == 0) return MM4_OK;
+  if (!b->page_table && b->pages_per_sequence > 0) return fail(MM4_ERR_INVALID, "null page table");
+  if (!b->lengths || !b->offsets) return fail(MM4_ERR_INVALID, "null lengths or offsets");
+  const void* ptrs[] = {b->page_table, b->lengths, b->offsets};
+  for (const void* q : ptrs)
+    if ((reinterpret_cast<uintptr_t>(q) & 3u) != 0)
+      return fail(MM4_ERR_INVALID, "page_table, lengths and offsets must be 4-byte aligned");
+  if ((static_cast<long long>(b->pages_per_sequence) << p->page_shift) > (1ll << 30))
+    return fail(MM4_ERR_UNSUPPORTED, "a sequence of more than 2^30 tokens");
+  return MM4_OK;
+}
+
+mm4_status check_rows(const char* name, const void* ptr, int64_t stride, int64_t width) {
+  if (!ptr) return fail(MM4_ERR_INVALID, "null %s pointer", name);
+  if (!aligned16(ptr)) return fail(MM4_ERR_INVALID, "%s must be 16-byte aligned", name);
+  if (stride % 8 != 0 || stride < width)
+    return fail(MM4_ERR_INVALID, "the rows of %s must be a multiple of 8 elements and at least %lld apart", name,
+                static_cast<long long>(width));
+  return MM4_OK;
+}
+
+mm4_status check_cache(const void* cache) {
+  if (!cache) return fail(MM4_ERR_INVALID, "null cache pointer");
+  if (!aligned16(cache)) return fail(MM4_ERR_INVALID, "the cache must be 16-byte aligned");
+  return MM4_OK;
+}
+
+KvBatch batch_args(const mm4_kv_cache_plan* p, const mm4_kv_cache_batch* b) {
+  KvBatch kb{};
+  kb.table = b->page_table;
+  kb.lengths = b->lengths;
+  kb.offsets = b->offsets;
+  kb.sequences = b->sequences;
+  kb.tokens = b->tokens;
+  kb.max_new = b->max_new;
+  kb.pages_per_seq = b->pages_per_sequence;
+  kb.page_shift = p->page_shift;
+  kb.pages = p->d.pages;
+  kb.heads_kv = p->d.heads_kv;
+  kb.page_bytes = p->page_bytes;
+  return kb;
+}
+
+mm4_status use_device(DeviceInfo* info) {
+  mm4_status rc = current_device(info);
+  if (rc != MM4_OK) return rc;
+  if (info->device < 0 || info->device >= kMaxDevices)
+    return fail(MM4_ERR_CUDA, "device id %d out of range", info->device);
+  g_used[info->device].store(true);
+  return MM4_OK;
+}
+
+// Calls f<D, BITS>() for the plan's head_dim and bits.
+template <typename F>
+mm4_status by_row(const mm4_kv_cache_desc& d, F&& f) {
+  if (d.head_dim == 128)
+    return d.bits == 4 ? f(KvRow<128, 4>{}, std::integral_constant<int, 128>{}, std::integral_constant<int, 4>{})
+                       : f(KvRow<128, 8>{}, std::integral_constant<int, 128>{}, std::integral_constant<int, 8>{});
+  return d.bits == 4 ? f(KvRow<64, 4>{}, std::integral_constant<int, 64>{}, std::integral_constant<int, 4>{})
+                     : f(KvRow<64, 8>{}, std::integral_constant<int, 64>{}, std::integral_constant<int, 8>{});
+}
+
+mm4_status launch_io(const mm4_kv_cache_plan* p, KvIoArgs& a, bool write, cudaStream_t st) {
+  DeviceInfo info;
+  mm4_status rc = use_device(&info);
+  if (rc != MM4_OK) return rc;
+  const int vecs = 2 * p->d.heads_kv * p->d.head_dim / 8;
+  a.parts = (vecs + KV_IO_PART - 1) / KV_IO_PART;
+  const long long blocks = (static_cast<long long>(a.kb.tokens) * a.parts + KV_IO_WARPS - 1) / KV_IO_WARPS;
+  if (blocks > 0x7fffffffLL) return fail(MM4_ERR_UNSUPPORTED, "too many tokens for one launch");
+  return by_row(p->d, [&](auto, auto D, auto B) -> mm4_status {
+    if (write)
+      kv_append_kernel<D.value, B.value><<<static_cast<unsigned>(blocks), KV_IO_WARPS * 32, 0, st>>>(a);
+    else
+      kv_read_kernel<D.value, B.value><<<static_cast<unsigned>(blocks), KV_IO_WARPS * 32, 0, st>>>(a);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return cuda_fail(e, write ? "kv_append_kernel launch" : "kv_read_kernel launch");
+    return MM4_OK;
+  });
+}
+
+}  // namespace
+
+namespace mm4 {
+
+mm4_status kv_cache_take_status(int dev, int* wait, int* data) {
+  *wait = *data = 0;
+  if (dev < 0 || dev >= kMaxDevices || !g_used[dev].load()) return MM4_OK;
+  const int zero = 0;
+  MM4_CUDA_TRY(cudaMemcpyFromSymbol(wait, g_kv_wait, sizeof(int)));
+  MM4_CUDA_TRY(cudaMemcpyFromSymbol(data, g_kv_data, sizeof(int)));
+  if (*wait != 0) MM4_CUDA_TRY(cudaMemcpyToSymbol(g_kv_wait, &zero, sizeof(int)));
+  if (*data != 0) MM4_CUDA_TRY(cudaMemcpyToSymbol(g_kv_data, &zero, sizeof(int)));
+  return MM4_OK;
+}
+
+const char* kv_cache_site_text(int site) {
+  switch (site) {
+    case KV_DATA_PAGE: return "a page number lies outside the pool";
+    case KV_DATA_LENGTH: return "a length is negative or beyond the page table";
+    case KV_DATA_OFFSETS: return "offsets are out of order or beyond the rows";
+    case KV_DATA_NEW: return "a sequence has more rows than max_new";
+    default: return "unknown";
+  }
+}
+
+}  // namespace mm4
+
+extern "C" {
+
+mm4_status mm4_kv_cache_plan_create(mm4_kv_cache_plan** out, const mm4_kv_cache_desc* d) {
+  if (!out) return fail(MM4_ERR_INVALID, "null plan pointer");
+  *out = nullptr;
+  if (!d) return fail(MM4_ERR_INVALID, "null key / value cache descriptor");
+  if (d->pages <= 0 || d->heads_q <= 0 || d->heads_kv <= 0 || d->head_dim <= 0)
+    return fail(MM4_ERR_INVALID, "pages, heads and head_dim must be positive");
+  if (d->heads_q % d->heads_kv != 0)
+    return fail(MM4_ERR_INVALID, "heads_kv (%d) must divide heads_q (%d)", d->heads_kv, d->heads_q);
+  if (d->page_size < 16 || d->page_size > 256 || (d->page_size & (d->page_size - 1)) != 0)
+    return fail(MM4_ERR_INVALID, "page_size %d: 16, 32, 64, 128 or 256", d->page_size);
+  if (d->bits != 4 && d->bits != 8) return fail(MM4_ERR_INVALID, "bits %d: 4 or 8", d->bits);
+  if (d->causal != 0 && d->causal != 1) return fail(MM4_ERR_INVALID, "causal must be 0 or 1");
+  if (d->head_dim != 128 && d->head_dim != 64)
+    return fail(MM4_ERR_UNSUPPORTED, "head_dim %d: this build implements head_dim 128 and 64", d->head_dim);
+  if (std::isnan(d->scale) || std::isinf(d->scale)) return fail(MM4_ERR_INVALID, "scale must be finite");
+  if (d->heads_q > 4096) return fail(MM4_ERR_UNSUPPORTED, "heads_q %d: at most 4096", d->heads_q);
+  if (d->pages > 0x7fffffffLL) return fail(MM4_ERR_UNSUPPORTED, "more than 2^31 - 1 pages");
+  mm4_kv_cache_plan* p = new (std::nothrow) mm4_kv_cache_plan();
+  if (!p) return fail(MM4_ERR_INVALID, "out of host memory");
+  p->d = *d;
+  p->scale = d->scale > 0.f ? d->scale : 1.0f / std::sqrt(static_cast<float>(d->head_dim));
+  p->page_shift = 0;
+  while ((1 << p->page_shift) < d->page_size) ++p->page_shift;
+  p->page_bytes = 2ll * d->heads_kv * d->page_size * row_bytes(*d);
+  *out = p;
+  return MM4_OK;
+}
+
+void mm4_kv_cache_plan_destroy(mm4_kv_cache_plan* plan) { delete plan; }
+
+size_t mm4_kv_cache_page_bytes(const mm4_kv_cache_plan* p) { return p ? static_cast<size_t>(p->page_bytes) : 0; }
+
+size_t mm4_kv_cache_bytes(const mm4_kv_cache_plan* p) {
+  return p ? static_cast<size_t>(p->page_bytes) * static_cast<size_t>(p->d.pages) : 0;
+}
+
+mm4_status mm4_kv_cache_append(const mm4_kv_cache_plan* p, const mm4_kv_cache_batch* b, const void* K,
+                               int64_t k_stride, const void* V, int64_t v_stride, void* cache, mm4_stream_t stream) {
+  mm4_status rc = check_batch(p, b);
+  if (rc != MM4_OK) return rc;
+  if (b->sequences == 0 || b->tokens == 0) return MM4_OK;
+  const int64_t width = static_cast<int64_t>(p->d.heads_kv) * p->d.head_dim;
+  if ((rc = check_rows("K", K, k_stride, width)) != MM4_OK) return rc;
+  if ((rc = check_rows("V", V, v_stride, width)) != MM4_OK) return rc;
+  if ((rc = check_cache(cache)) != MM4_OK) return rc;
+  KvIoArgs a{};
+  a.kb = batch_args(p, b);
+  a.in_k = static_cast<const __half*>(K);
+  a.in_v = static_cast<const __half*>(V);
+  a.k_stride = k_stride;
+  a.v_stride = v_stride;
+  a.cache = static_cast<uint8_t*>(cache);
+  return launch_io(p, a, true, static_cast<cudaStream_t>(stream));
+}
+
+mm4_status mm4_kv_cache_read(const mm4_kv_cache_plan* p, const mm4_kv_cache_batch* b, const void* cache, void* K,
+                             int64_t k_stride, void* V, int64_t v_stride, mm4_stream_t stream) {
+  mm4_status rc = check_batch(p, b);
+  if (rc != MM4_OK) return rc;
+  if (b->sequences == 0 || b->tokens == 0) return MM4_OK;
+  const int64_t width = static_cast<int64_t>(p->d.heads_kv) * p->d.head_dim;
+  if ((rc = check_rows("K", K, k_stride, width)) != MM4_OK) return rc;
+  if ((rc = check_rows("V", V, v_stride, width)) != MM4_OK) return rc;
+  if ((rc = check_cache(cache)) != MM4_OK) return rc;
+  KvIoArgs a{};
+  a.kb = batch_args(p, b);
+  a.out_k = static_cast<__half*>(K);
+  a.out_v = static_cast<__half*>(V);
+  a.k_stride = k_stride;
+  a.v_stride = v_stride;
+  a.cache = static_cast<uint8_t*>(const_cast<void*>(cache));
+  return launch_io(p, a, false, static_cast<cudaStream_t>(stream));
+}
+
+size_t mm4_kv_cache_attention_workspace_size(const mm4_kv_cache_plan* p, const mm4_kv_cache_batch* b) {
+  (void)b;
+  return p ? 0 : 0;
+}
+
+const char* mm4_kv_cache_attention_kernel_name(const mm4_kv_cache_plan* p, const mm4_kv_cache_batch* b) {
+  return p && b ? "kv_attention_row" : "";
+}
+
+mm4_status mm4_kv_cache_attention(const mm4_kv_cache_plan* p, const mm4_kv_cache_batch* b, const void* Q,
+                                  int64_t q_stride, const void* cache, void* O, int64_t o_stride, float* lse,
+                                  void* workspace, size_t workspace_bytes, mm4_stream_t stream) {
+  (void)workspace;
+  (void)workspace_bytes;
+  mm4_status rc = check_batch(p, b);
+  if (rc != MM4_OK) return rc;
+  if (b->sequences == 0 || b->tokens == 0) return MM4_OK;
+  if (b->max_new < 1) return fail(MM4_ERR_INVALID, "max_new must be at least 1");
+  const int64_t width = static_cast<int64_t>(p->d.heads_q) * p->d.head_dim;
+  if ((rc = check_rows("Q", Q, q_stride, width)) != MM4_OK) return rc;
+  if ((rc = check_rows("O", O, o_stride, width)) != MM4_OK) return rc;
+  if ((rc = check_cache(cache)) != MM4_OK) return rc;
+  if ((reinterpret_cast<uintptr_t>(lse) & 3u) != 0) return fail(MM4_ERR_INVALID, "lse must be 4-byte aligned");
+  DeviceInfo info;
+  if ((rc = use_device(&info)) != MM4_OK) return rc;
+  KvAttnArgs a{};
+  a.kb = batch_args(p, b);
+  a.Q = static_cast<const __half*>(Q);
+  a.O = static_cast<__half*>(O);
+  a.lse = lse;
+  a.q_stride = q_stride;
+  a.o_stride = o_stride;
+  a.cache = static_cast<const uint8_t*>(cache);
+  a.heads_q = p->d.heads_q;
+  a.group = p->d.heads_q / p->d.heads_kv;
+  a.causal = p->d.causal;
+  a.scale_log2 = p->scale * 1.4426950408889634f;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const long long blocks = (static_cast<long long>(b->tokens) * p->d.heads_q + 3) / 4;
+  if (blocks > 0x7fffffffLL) return fail(MM4_ERR_UNSUPPORTED, "too many rows for one launch");
+  return by_row(p->d, [&](auto, auto D, auto B) -> mm4_status {
+    kv_attention_row_kernel<D.value, B.value><<<static_cast<unsigned>(blocks), 128, 0, st>>>(a);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return cuda_fail(e, "kv_attention_row_kernel launch");
+    return MM4_OK;
+  });
+}
+
+}  // extern "C"

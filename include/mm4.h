@@ -4,7 +4,7 @@
  * This is the drop-in boundary for the tensor-op contraction path of
  * liuliu/example_matmul_metal4: the generated matmul2d GEMM (bias, split-K,
  * dynamic K), the flash-attention forward, and conv2d / conv3d (with and
- * without padding). The reference exposes that path as Swift descriptor
+ * without padding); and attention over a key / value cache held in 4 or 8 bits. The reference exposes that path as Swift descriptor
  * structs + MSL source generators + Metal "sessions"; the entries below take
  * the same descriptors and run hand-written CUDA kernels instead.
  *
@@ -54,9 +54,12 @@ MM4_API const char* mm4_last_error(void);
 MM4_API int mm4_device_supported(void);
 
 /* Synchronises `stream`, then reads and clears the current device's status
- * words: the library's own, and the two of mm4_gemm_splitk_run_noalloc.
+ * words: the library's own, the two of mm4_gemm_splitk_run_noalloc, and the
+ * two of the mm4_kv_cache_* calls.
  * Returns MM4_ERR_TIMEOUT when a kernel recorded a run-out wait (the
- * message names the wait site), MM4_ERR_CUDA on a CUDA error, else MM4_OK.
+ * message names the wait site), MM4_ERR_INVALID when an mm4_kv_cache_* kernel
+ * found a wrong page number, length or offset in its batch, MM4_ERR_CUDA on a
+ * CUDA error, else MM4_OK.
  * It allocates no device memory. */
 MM4_API mm4_status mm4_check(mm4_stream_t stream);
 
@@ -321,6 +324,113 @@ MM4_API mm4_status mm4_attention_bwd_host(const mm4_attention_plan* plan, const 
                                           void* const* host_out, void* const* dev_in, void* const* dev_out,
                                           void* workspace, size_t workspace_bytes, int32_t chunks,
                                           mm4_stream_t stream);
+
+/* ======================================================================== */
+/* Key / value cache in 4 or 8 bits: write, read back, attention             */
+/* ======================================================================== */
+
+/* Attention for callers that keep keys and values between calls (one token at
+ * a time, a few tokens, or a prompt in chunks). No reference counterpart: the
+ * reference's attention reads whole K and V each time (attention.swift:398).
+ *
+ * The cache is one device buffer of `pages` pages, [pages][heads_kv][2: K, V]
+ * [page_size][row], owned by the caller; a page is contiguous, so pages can be
+ * copied, shared between sequences or moved off the device as they are. A row
+ * is one head's vector of one token: head_dim codes of `bits` bits (4: element
+ * d in nibble d % 2 of byte d / 2, the low nibble first; 8: byte d), then for
+ * each group of 32 elements an fp16 scale and an fp16 zero. Per group, with
+ * x the fp16 inputs (NaN counts as 0, infinities as +-65504):
+ *   zero  = min x,  scale = (max x - min x) / (2^bits - 1) rounded towards 0
+ *   code  = min(2^bits - 1, round_half_even((x - zero) / scale)), 0 if scale = 0
+ * (fp32 arithmetic), and a code stands for fp16(code * scale + zero), rounded
+ * once. The values that code stands for never leave fp16's range.
+ *
+ *  pages      pages of the pool, >= 1. page_size: tokens of a page, one of
+ *             16, 32, 64, 128, 256.
+ *  heads_kv   must divide heads_q (grouped-query attention when smaller).
+ *  head_dim   128 or 64. bits: 4 or 8.
+ *  causal     1: a token attends to itself and what lies before it; 0: to
+ *             everything its sequence has in the cache.
+ *  scale      <= 0 selects 1/sqrt(head_dim), as in mm4_attention_desc. */
+typedef struct mm4_kv_cache_desc {
+  int64_t pages;
+  int32_t page_size;
+  int32_t heads_q, heads_kv;
+  int32_t head_dim;
+  int32_t bits;
+  int32_t causal;
+  float scale;
+} mm4_kv_cache_desc;
+
+typedef struct mm4_kv_cache_plan mm4_kv_cache_plan;
+
+/* The sequences of one call; the same batch serves the three calls below, for
+ * every layer. The three arrays are device memory and are read by the kernels
+ * only, so a captured call replays with what they hold then.
+ *  page_table [sequences][pages_per_sequence]: position p of sequence b lies in
+ *             row p % page_size of page page_table[b][p / page_size].
+ *  lengths    [sequences]: tokens that sequence b has in the cache, counting
+ *             those of this call.
+ *  offsets    [sequences + 1], ascending: rows offsets[b] .. offsets[b+1]-1 of
+ *             K, V, Q and O are the LAST tokens of sequence b, so the last of
+ *             them has position lengths[b] - 1. Rows outside every sequence
+ *             (below offsets[0], from offsets[sequences] on) are padding: not
+ *             read, and left as they were in outputs.
+ *  tokens     rows of K, V, Q and O.
+ *  max_new    most rows of one sequence (mm4_kv_cache_attention only).
+ * A sequence may have no rows in a call, length 0, or more rows than its length:
+ * rows that come to lie before position 0 are not written by append or read,
+ * and attend to nothing. Page-table entries behind a sequence's length are not
+ * read. What the kernels find wrong in these arrays - a page number outside the
+ * pool, a length beyond the page table, more rows than max_new, offsets out
+ * of order or beyond tokens - never leads to an access out of bounds: such
+ * tokens are left out by append and read, the outputs of such sequences are
+ * unspecified in attention, and mm4_check() reports MM4_ERR_INVALID. */
+typedef struct mm4_kv_cache_batch {
+  int32_t sequences;
+  int32_t tokens;
+  int32_t max_new;
+  int32_t pages_per_sequence;
+  const int32_t* page_table;
+  const int32_t* lengths;
+  const int32_t* offsets;
+} mm4_kv_cache_batch;
+
+MM4_API mm4_status mm4_kv_cache_plan_create(mm4_kv_cache_plan** plan, const mm4_kv_cache_desc* desc);
+MM4_API void mm4_kv_cache_plan_destroy(mm4_kv_cache_plan* plan);
+/* Bytes of one page, and of the whole cache buffer (0 for a null plan). */
+MM4_API size_t mm4_kv_cache_page_bytes(const mm4_kv_cache_plan* plan);
+MM4_API size_t mm4_kv_cache_bytes(const mm4_kv_cache_plan* plan);
+
+/* Quantises the rows of K and V (fp16 [tokens][heads_kv][head_dim], rows
+ * k_stride / v_stride elements apart) into the cache. One launch. K, V and
+ * the cache are 16-byte aligned; strides are multiples of 8 and at least
+ * heads_kv * head_dim. Two tokens of one call must not share a place in the
+ * cache (two sequences may share pages that neither writes). */
+MM4_API mm4_status mm4_kv_cache_append(const mm4_kv_cache_plan* plan, const mm4_kv_cache_batch* batch, const void* K,
+                                       int64_t k_stride, const void* V, int64_t v_stride, void* cache,
+                                       mm4_stream_t stream);
+
+/* Reads back the rows that an append of the same batch writes, as the fp16
+ * values their codes stand for (a batch whose offsets step by the lengths reads
+ * whole sequences). One launch; alignment and strides as above. */
+MM4_API mm4_status mm4_kv_cache_read(const mm4_kv_cache_plan* plan, const mm4_kv_cache_batch* batch, const void* cache,
+                                     void* K, int64_t k_stride, void* V, int64_t v_stride, mm4_stream_t stream);
+
+/* O = softmax(scale * Q K^T) V over each sequence's cached keys and values (this
+ * call's tokens appended before). Q and O are fp16 [tokens][heads_q][head_dim],
+ * rows q_stride / o_stride elements apart (multiples of 8, at least
+ * heads_q * head_dim; 16-byte aligned bases). lse, if not NULL, receives fp32
+ * [tokens][heads_q] natural-log sums of exp(scale * S). A row that attends to
+ * nothing gets O = 0 and lse = -infinity. fp32 softmax statistics and sums.
+ * workspace: mm4_kv_cache_attention_workspace_size() bytes, 16-byte aligned, any
+ * contents; calls that may overlap on the GPU need one each. */
+MM4_API size_t mm4_kv_cache_attention_workspace_size(const mm4_kv_cache_plan* plan, const mm4_kv_cache_batch* batch);
+MM4_API mm4_status mm4_kv_cache_attention(const mm4_kv_cache_plan* plan, const mm4_kv_cache_batch* batch, const void* Q,
+                                          int64_t q_stride, const void* cache, void* O, int64_t o_stride, float* lse,
+                                          void* workspace, size_t workspace_bytes, mm4_stream_t stream);
+/* Describes the kernel that attention over `batch` runs (static string). */
+MM4_API const char* mm4_kv_cache_attention_kernel_name(const mm4_kv_cache_plan* plan, const mm4_kv_cache_batch* batch);
 
 /* ======================================================================== */
 /* Convolution (implicit GEMM)                                              */

@@ -1,0 +1,133 @@
+"""Key / value cache entry points without a GPU: sizes, refusals (every call below fails before a pointer is
+used or a kernel launched), and the definition's restatement against itself."""
+import ctypes
+
+import numpy as np
+import pytest
+
+import kv_cache_ref as ref
+from example_matmul_metal4_b200 import _lib
+
+FAKE = 1 << 20  # a stand-in address, 16-byte aligned
+INVALID, UNSUPPORTED = _lib.MM4_ERR_INVALID, _lib.MM4_ERR_UNSUPPORTED
+
+
+def _plan(**kw):
+    d = dict(pages=7, page_size=64, heads_q=8, heads_kv=2, head_dim=128, bits=4, causal=1, scale=0.0)
+    d.update(kw)
+    h = ctypes.c_void_p()
+    rc = _lib.lib().mm4_kv_cache_plan_create(ctypes.byref(h), ctypes.byref(_lib.KVCacheDesc(*d.values())))
+    return rc, h
+
+
+def _batch(**kw):
+    d = dict(sequences=3, tokens=5, max_new=2, pages_per_sequence=4, page_table=FAKE, lengths=FAKE, offsets=FAKE)
+    d.update(kw)
+    return _lib.KVCacheBatchDesc(*d.values())
+
+
+@pytest.mark.parametrize("D,bits,row", [(128, 4, 80), (128, 8, 144), (64, 4, 40), (64, 8, 72)])
+def test_sizes(D, bits, row):
+    L = _lib.lib()
+    rc, h = _plan(head_dim=D, bits=bits, page_size=32, heads_kv=4, pages=1 << 20)
+    assert rc == 0 and ref.row_bytes(D, bits) == row
+    assert L.mm4_kv_cache_page_bytes(h) == 4 * 2 * 32 * row
+    assert L.mm4_kv_cache_bytes(h) == (4 * 2 * 32 * row) << 20
+    L.mm4_kv_cache_plan_destroy(h)
+    assert L.mm4_kv_cache_page_bytes(None) == 0 and L.mm4_kv_cache_bytes(None) == 0
+    assert L.mm4_kv_cache_attention_workspace_size(None, None) == 0
+    L.mm4_kv_cache_plan_destroy(None)
+
+
+@pytest.mark.parametrize("kw,rc", [
+    (dict(pages=0), INVALID), (dict(pages=1 << 31), UNSUPPORTED), (dict(page_size=48), INVALID),
+    (dict(page_size=8), INVALID), (dict(page_size=512), INVALID), (dict(heads_q=0), INVALID),
+    (dict(heads_kv=3), INVALID), (dict(heads_kv=-1), INVALID), (dict(head_dim=96), UNSUPPORTED),
+    (dict(head_dim=0), INVALID), (dict(bits=3), INVALID), (dict(causal=2), INVALID),
+    (dict(scale=float("nan")), INVALID), (dict(scale=float("inf")), INVALID),
+    (dict(heads_q=8192, heads_kv=8192), UNSUPPORTED)])
+def test_plan_refusals(kw, rc):
+    got, h = _plan(**kw)
+    assert got == rc and not h
+    assert _lib.lib().mm4_last_error()
+
+
+def test_null_plan_arguments():
+    L = _lib.lib()
+    assert L.mm4_kv_cache_plan_create(None, None) == INVALID
+    h = ctypes.c_void_p()
+    assert L.mm4_kv_cache_plan_create(ctypes.byref(h), None) == INVALID
+
+
+def _calls(L, h):
+    """name -> call(batch reference, pointers, strides): K / V of width 256, Q / O of width 1024."""
+    return {
+        "append": lambda b, p, s: L.mm4_kv_cache_append(h, b, p[0], s[0], p[1], s[1], p[2], None),
+        "read": lambda b, p, s: L.mm4_kv_cache_read(h, b, p[2], p[0], s[0], p[1], s[1], None),
+        "attention": lambda b, p, s: L.mm4_kv_cache_attention(h, b, p[0], s[0], p[2], p[1], s[1], None, FAKE, 1 << 40,
+                                                              None),
+    }
+
+
+@pytest.mark.parametrize("name,width", [("append", 256), ("read", 256), ("attention", 1024)])
+def test_call_refusals(name, width):
+    L = _lib.lib()
+    rc, h = _plan()
+    assert rc == 0
+    call = _calls(L, h)[name]
+    good = ([FAKE] * 3, [width, width])
+    assert _calls(L, None)[name](ctypes.byref(_batch()), *good) == INVALID
+    assert call(None, *good) == INVALID
+    for kw in (dict(sequences=-1), dict(tokens=-1), dict(max_new=-1), dict(pages_per_sequence=-1),
+               dict(page_table=None), dict(lengths=None), dict(offsets=None), dict(lengths=FAKE + 2)):
+        assert call(ctypes.byref(_batch(**kw)), *good) == INVALID, kw
+    assert call(ctypes.byref(_batch(pages_per_sequence=1 << 25)), *good) == UNSUPPORTED
+    for i in range(3):
+        for bad in (None, FAKE + 8):
+            p = [FAKE] * 3
+            p[i] = bad
+            assert call(ctypes.byref(_batch()), p, good[1]) == INVALID, (i, bad)
+    for i in range(2):
+        for bad in (width - 8, width + 4, 0, -width):
+            s = [width, width]
+            s[i] = bad
+            assert call(ctypes.byref(_batch()), good[0], s) == INVALID, (i, bad)
+    # nothing to do: no row, no sequence; no pointer is looked at
+    assert call(ctypes.byref(_batch(tokens=0)), [None] * 3, [0, 0]) == 0
+    assert call(ctypes.byref(_batch(sequences=0)), [None] * 3, [0, 0]) == 0
+    if name == "attention":
+        assert call(ctypes.byref(_batch(max_new=0)), *good) == INVALID
+        assert b"max_new" in L.mm4_last_error()
+        assert L.mm4_kv_cache_attention(h, ctypes.byref(_batch()), FAKE, width, FAKE, FAKE, width, FAKE + 2, FAKE,
+                                        1 << 40, None) == INVALID
+    L.mm4_kv_cache_plan_destroy(h)
+
+
+def test_python_wrapper_refusals():
+    import torch
+
+    from example_matmul_metal4_b200.kv_cache import KVCacheBatch, KVCacheDimensions, KVCachePlan
+    with pytest.raises(_lib.MM4Error):
+        KVCachePlan(KVCacheDimensions(4, 64, 8, 3, 128))
+    plan = KVCachePlan(KVCacheDimensions(4, 64, 8, 2, 128))
+    assert plan.cacheBytes == 4 * plan.pageBytes
+    assert plan.allocate("cpu").shape == (4, plan.pageBytes)
+    i32 = torch.int32
+    with pytest.raises(ValueError, match="CUDA int32"):
+        KVCacheBatch(torch.zeros(1, 1, dtype=i32), torch.zeros(1, dtype=i32), torch.zeros(2, dtype=i32), 1, 1)
+
+
+def test_restatement_rounds_scales_towards_zero_and_inverts():
+    rng = np.random.default_rng(0)
+    x = rng.standard_normal((50, 128)).astype(np.float16)
+    for bits in (4, 8):
+        codes, scale, zero = ref.quantise(x, bits)
+        top = 2 ** bits - 1
+        g = x.astype(np.float64).reshape(50, 4, 32)
+        span = g.max(-1) - g.min(-1)
+        assert (scale.astype(np.float64) * top <= span * (1 + 2.0 ** -23)).all()
+        assert codes.max() <= top
+        back = ref.unpack(ref.pack(x, bits), 128, bits)
+        assert np.array_equal(back, ref.values(codes, scale, zero))
+        err = np.abs(back.astype(np.float64) - x).reshape(50, 4, 32).max(-1)
+        assert (err <= span / top / 2 + span * 2.0 ** -10 + 4 * 2.0 ** -11).all()

@@ -1,0 +1,505 @@
+"""The key / value cache operators on the GPU against their float64 restatement (kv_cache_ref.py): written
+bytes, read-back values and attention, at the lengths, heads, pages and masks where they can go wrong."""
+import numpy as np
+import pytest
+
+import kv_cache_ref as ref
+from example_matmul_metal4_b200 import data, sync_check
+from example_matmul_metal4_b200._lib import MM4_ERR_INVALID, MM4Error
+from example_matmul_metal4_b200.attention import MM4_ATTN_BSHD, AttentionDimensions, AttentionPlan
+from example_matmul_metal4_b200.kv_cache import KVCacheBatch, KVCacheDimensions, KVCachePlan
+
+pytestmark = pytest.mark.gpu
+
+
+def _table(lengths, page, pages, seed, width=None):
+    """A page table whose sequences use distinct pages of the pool in a random order; unused entries point
+    outside the pool (they must not be read)."""
+    rng = np.random.default_rng(seed)
+    order = rng.permutation(pages)
+    width = width or max(1, max((ln + page - 1) // page for ln in lengths))
+    table = np.full((len(lengths), width), 2 ** 30, dtype=np.int32)
+    at = 0
+    for b, ln in enumerate(lengths):
+        n = (ln + page - 1) // page
+        table[b, :n] = order[at:at + n]
+        at += n
+    assert at <= pages
+    return table
+
+
+def _pages_for(lengths, page):
+    return sum((ln + page - 1) // page for ln in lengths) + 2
+
+
+class Setup:
+    """A filled cache and a batch, on the host (bytes) and on the device."""
+
+    def __init__(self, dev, lengths, new, Hq, Hk, D=128, bits=4, page=64, causal=True, seed=1, pad=0, scale=None,
+                 maxNew=None, k_map=lambda k: k):
+        import torch
+        self.lengths, self.new, self.Hq, self.Hk, self.D, self.bits, self.page = lengths, new, Hq, Hk, D, bits, page
+        self.causal, self.pad = causal, pad
+        pages = _pages_for(lengths, page)
+        self.plan = KVCachePlan(KVCacheDimensions(pages, page, Hq, Hk, D, bits), causal=causal, scale=scale)
+        self.table = _table(lengths, page, pages, seed)
+        self.offsets = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+        self.tokens = int(self.offsets[-1]) + pad
+        # unused rows hold bytes whose scales and zeros are NaN: they must not reach any result
+        self.host = np.full((pages, Hk, 2, page, ref.row_bytes(D, bits)), 0xFF, dtype=np.uint8)
+        self.K, self.V = [], []
+        for b, ln in enumerate(lengths):
+            k = k_map(data.normal((ln, Hk, D), 1.0, seed, 10 + 2 * b).astype(np.float32))
+            v = data.normal((ln, Hk, D), 1.0, seed, 11 + 2 * b)
+            rows = [ref.pack(k.astype(np.float16), bits), ref.pack(v, bits)] if ln else None
+            if ln:
+                pos = np.arange(ln)
+                for kv in (0, 1):
+                    self.host[self.table[b, pos // page], :, kv, pos % page] = rows[kv]
+            self.K.append(ref.unpack(rows[0], D, bits) if ln else np.zeros((0, Hk, D), np.float16))
+            self.V.append(ref.unpack(rows[1], D, bits) if ln else np.zeros((0, Hk, D), np.float16))
+        self.Q = data.normal((max(1, self.tokens), Hq, D), 1.0, seed, 5)[:self.tokens]
+        self.dev = dev
+        self.cache = torch.from_numpy(self.host.reshape(pages, -1)).to(dev)
+        self.batch = KVCacheBatch(torch.from_numpy(self.table).to(dev),
+                                  torch.tensor(lengths, dtype=torch.int32, device=dev),
+                                  torch.from_numpy(self.offsets).to(dev), self.tokens,
+                                  max(new) if maxNew is None else maxNew)
+
+    def check(self, O, lse=None, sequences=None):
+        O = O.double().cpu().numpy()
+        lse = None if lse is None else lse.double().cpu().numpy()
+        for b in range(len(self.lengths)) if sequences is None else sequences:
+            r = slice(self.offsets[b], self.offsets[b + 1])
+            eO, eL, tO, tL = ref.attention(self.Q[r], self.K[b], self.V[b], self.new[b], self.causal, self.plan.scale)
+            off = np.abs(O[r] - eO) / np.maximum(tO, 2.0 ** -25)
+            assert off.size == 0 or off.max() <= 1.0, (b, off.max(), np.unravel_index(off.argmax(), off.shape))
+            if lse is not None:
+                empty = np.isneginf(eL)
+                assert np.array_equal(empty, np.isneginf(lse[r])), b
+                d = np.abs(np.where(empty, 0, lse[r]) - np.where(empty, 0, eL))
+                assert (d <= tL).all(), (b, (d - tL).max())
+
+    def attend(self, want_lse=True, **kw):
+        import torch
+        Q = torch.from_numpy(np.ascontiguousarray(self.Q)).to(self.dev)
+        lse = torch.full((self.tokens, self.Hq), 7.0, device=self.dev) if want_lse else None
+        O = self.plan.attention(Q, self.cache, self.batch, lse=lse, **kw)
+        sync_check()
+        return O, lse
+
+
+# ----------------------------------------------------------------------------------------------------------
+# write and read back
+# ----------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("D,Hk,page", [(128, 8, 64), (64, 1, 16), (128, 1, 256), (64, 5, 32), (128, 3, 128)])
+def test_append_writes_the_defined_bytes_and_nothing_else(cuda, D, Hk, page, bits):
+    """Ragged sequences whose new tokens start inside a page, end inside one and cross pages; strided K and V;
+    padding rows behind the last sequence. Every byte of the cache is compared."""
+    import torch
+    lengths, new, pad = [300, 17, 1, 64, 33], [290, 5, 1, 64, 0], 3
+    pages = _pages_for(lengths, page)
+    plan = KVCachePlan(KVCacheDimensions(pages, page, Hk, Hk, D, bits))
+    table = _table(lengths, page, pages, 3)
+    offsets = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+    tokens = int(offsets[-1]) + pad
+    K = data.normal((tokens, Hk, D), 2.0, 4, 0)
+    V = data.normal((tokens, Hk, D), 0.5, 4, 1)
+    host = np.full((pages, Hk, 2, page, ref.row_bytes(D, bits)), 0xA5, dtype=np.uint8)
+    cache = torch.from_numpy(host.reshape(pages, -1).copy()).to(cuda)
+    for b, (ln, n) in enumerate(zip(lengths, new)):
+        pos = np.arange(ln - n, ln)
+        r = slice(offsets[b], offsets[b + 1])
+        host[table[b, pos // page], :, 0, pos % page] = ref.pack(K[r], bits)
+        host[table[b, pos // page], :, 1, pos % page] = ref.pack(V[r], bits)
+    fused = torch.zeros(tokens, 2 * Hk * D + 8, dtype=torch.float16, device=cuda)
+    fused[:, :Hk * D] = torch.from_numpy(K.reshape(tokens, -1)).to(cuda)
+    fused[:, Hk * D:2 * Hk * D] = torch.from_numpy(V.reshape(tokens, -1)).to(cuda)
+    tK, tV = (fused[:, i * Hk * D:(i + 1) * Hk * D].view(tokens, Hk, D) for i in (0, 1))
+    batch = KVCacheBatch(torch.from_numpy(table).to(cuda), torch.tensor(lengths, dtype=torch.int32, device=cuda),
+                         torch.from_numpy(offsets).to(cuda), tokens, max(new))
+    plan.append(tK, tV, cache, batch)
+    sync_check()
+    assert np.array_equal(cache.cpu().numpy().reshape(host.shape), host)
+    # and back, into strided outputs whose padding rows stay as they were
+    out = torch.full((tokens, 2 * Hk * D + 8), -3.0, dtype=torch.float16, device=cuda)
+    oK, oV = (out[:, i * Hk * D:(i + 1) * Hk * D].view(tokens, Hk, D) for i in (0, 1))
+    plan.read(cache, batch, K=oK, V=oV)
+    sync_check()
+    used = int(offsets[-1])
+    assert np.array_equal(oK[:used].cpu().numpy(), ref.unpack(ref.pack(K[:used], bits), D, bits))
+    assert np.array_equal(oV[:used].cpu().numpy(), ref.unpack(ref.pack(V[:used], bits), D, bits))
+    assert (out[used:] == -3.0).all() and (out[:, 2 * Hk * D:] == -3.0).all()
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_groups_at_the_edges_of_fp16(cuda, bits):
+    """Constant groups, zeros of both signs, NaN and infinities, the widest range, subnormals, a range of one
+    smallest step, and values that land half-way between codes."""
+    import torch
+    top = 2 ** bits - 1
+    g = np.zeros((16, 32), dtype=np.float16)
+    g[0] = 1.5
+    g[1, ::2] = -0.0
+    g[2, :3] = [np.nan, np.inf, -np.inf]
+    g[3] = np.where(np.arange(32) % 2, 65504, -65504)
+    g[4] = np.arange(32) * 2.0 ** -24
+    g[5, 7] = 2.0 ** -24
+    g[6] = np.minimum(np.arange(32), top) * 0.5 + 0.25 * (np.arange(32) % 2)   # halves of the step 0.5 * k
+    g[7] = np.nan
+    g[8] = np.inf
+    g[9] = -np.inf
+    g[10] = np.linspace(-65504, 65504, 32)
+    g[11] = 1024 + np.arange(32)
+    g[12] = np.linspace(-1, 1, 32) * 2.0 ** -14
+    g[13, 31] = 65504
+    g[14, 0] = -65504
+    g[15] = np.arange(32) / top
+    x = g.reshape(4, 1, 128)
+    plan = KVCachePlan(KVCacheDimensions(1, 16, 1, 1, 128, bits))
+    cache = plan.allocate(cuda)
+    t = torch.from_numpy(x).to(cuda)
+    batch = KVCacheBatch(torch.zeros(1, 1, dtype=torch.int32, device=cuda),
+                         torch.tensor([4], dtype=torch.int32, device=cuda),
+                         torch.tensor([0, 4], dtype=torch.int32, device=cuda), 4, 4)
+    plan.append(t, t.flip(0), cache, batch)
+    K, V = plan.read(cache, batch)
+    sync_check()
+    want = ref.unpack(ref.pack(x, bits), 128, bits)
+    got = K.cpu().numpy()
+    assert np.isfinite(got).all()
+    assert np.array_equal(got, want)
+    assert np.array_equal(V.cpu().numpy(), want[::-1])
+    # The error itself: half a step, plus what cutting the scale loses at the top code (2^-10 of top * scale, or
+    # top * 2^-24 where scales are subnormal), plus fp16 rounding of the value.
+    clean = np.clip(np.nan_to_num(x.astype(np.float64), nan=0.0), -65504, 65504)
+    v = clean.reshape(16, 32)
+    rng_ = v.max(1) - v.min(1)
+    bound = rng_ / top * 0.5 + rng_ * 2.0 ** -10 + top * 2.0 ** -24
+    err = np.abs(got.reshape(16, 32).astype(np.float64) - v)
+    assert (err <= bound[:, None] + 2.0 ** -11 * np.abs(v) + 2.0 ** -25).all()
+
+
+# ----------------------------------------------------------------------------------------------------------
+# attention
+# ----------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("D", [128, 64])
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("length", [1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 255, 513, 1000])
+def test_single_token_lengths(cuda, length, bits, D):
+    s = Setup(cuda, [length], [1], 8, 2, D=D, bits=bits)
+    s.check(*s.attend())
+
+
+@pytest.mark.parametrize("D,bits", [(128, 4), (64, 8)])
+@pytest.mark.parametrize("Hq,Hk", [(1, 1), (8, 8), (6, 2), (8, 1), (10, 5), (16, 1), (7, 1), (24, 2), (40, 1)])
+def test_head_groups(cuda, Hq, Hk, D, bits):
+    s = Setup(cuda, [333, 40], [1, 1], Hq, Hk, D=D, bits=bits, page=32)
+    s.check(*s.attend())
+
+
+@pytest.mark.parametrize("D,bits,page", [(128, 4, 16), (128, 8, 128), (64, 4, 256), (64, 8, 32)])
+@pytest.mark.parametrize("new", [2, 3, 5, 16, 17, 64, 65, 130, 200])
+@pytest.mark.parametrize("causal", [True, False])
+def test_rows_of_one_sequence(cuda, new, causal, D, bits, page):
+    """From two proposed tokens to prompt chunks, as the last rows of longer sequences and as whole ones."""
+    s = Setup(cuda, [new + 300, new], [new, new], 4, 2, D=D, bits=bits, page=page, causal=causal)
+    s.check(*s.attend())
+
+
+@pytest.mark.parametrize("D,bits", [(128, 4), (64, 4), (128, 8), (64, 8)])
+@pytest.mark.parametrize("new", [1, 4, 150])
+def test_ragged_batches(cuda, new, D, bits):
+    """Many sequences of lengths from one token to over a thousand, some with fewer rows, one with none."""
+    rng = np.random.default_rng(new)
+    lengths = [1, 1031, 2, 500, 64, 65, 127, 700, 33, 8, 1024, 90]
+    n = [int(min(ln, rng.integers(1, new + 1))) for ln in lengths]
+    n[3] = 0
+    n[1] = new
+    s = Setup(cuda, lengths, n, 8, 4, D=D, bits=bits, page=32, maxNew=new)
+    s.check(*s.attend())
+
+
+def test_prompt_over_several_row_blocks(cuda):
+    """A prompt of more rows than one block of the kernel holds, grouped heads, with and without a cached prefix."""
+    s = Setup(cuda, [700, 911], [700, 333], 6, 2, page=64)
+    s.check(*s.attend())
+
+
+@pytest.mark.parametrize("new,maxNew", [(1, 1), (9, 9), (300, 300)])
+def test_rows_that_attend_to_nothing(cuda, new, maxNew):
+    """Length 0, and more rows than the length: O = 0 and lse = -inf for the rows before position 0; padding rows
+    of O and lse are left as they were."""
+    import torch
+    lengths, rows = [0, 5, 40, 3], [1, new, 1, 0]
+    for causal in (True, False):
+        s = Setup(cuda, lengths, rows, 4, 4, page=16, causal=causal, pad=2, maxNew=maxNew)
+        O = torch.full((s.tokens, 4, 128), 9.0, dtype=torch.float16, device=cuda)
+        got, lse = s.attend(O=O)
+        assert got is O
+        s.check(got, lse)
+        assert (got[s.tokens - 2:] == 9.0).all() and (lse[s.tokens - 2:] == 7.0).all()
+        if causal and new > 5:
+            assert (got[1:1 + new - 5] == 0).all()
+
+
+@pytest.mark.parametrize("new", [1, 12, 70])
+def test_large_scores(cuda, new):
+    """Keys that grow along the sequence and a large scale, so the running maximum moves far and often."""
+    s = Setup(cuda, [900], [new], 4, 2, scale=0.5, k_map=lambda k: k * np.linspace(0.25, 3.0, len(k))[:, None, None])
+    s.check(*s.attend())
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_scores_far_below_zero(cuda, new):
+    """Every score of every row lies far below zero: exponentials are taken against the row's own maximum."""
+    s = Setup(cuda, [200], [new], 2, 2, D=64, scale=1.0, k_map=np.abs)
+    s.Q = -np.abs(s.Q)
+    s.check(*s.attend())
+
+
+@pytest.mark.parametrize("new", [1, 100])
+def test_strided_queries_and_outputs(cuda, new):
+    import torch
+    s = Setup(cuda, [400, 222], [new, new], 8, 2, D=64)
+    width = 8 * 64
+    big = torch.zeros(s.tokens, 2 * width + 8, dtype=torch.float16, device=cuda)
+    big[:, 8:8 + width] = torch.from_numpy(s.Q.reshape(s.tokens, -1)).to(cuda)
+    out = torch.full((s.tokens, width + 16), 4.0, dtype=torch.float16, device=cuda)
+    O = out[:, 8:8 + width].view(s.tokens, 8, 64)
+    s.plan.attention(big[:, 8:8 + width].view(s.tokens, 8, 64), s.cache, s.batch, O=O)
+    sync_check()
+    s.check(O)
+    assert (out[:, :8] == 4.0).all() and (out[:, 8 + width:] == 4.0).all()
+
+
+@pytest.mark.parametrize("new,length", [(1, 20000), (6, 9000), (40, 5000)])
+def test_long_axis_is_split_and_joined(cuda, new, length):
+    s = Setup(cuda, [length], [new], 8, 2, page=128)
+    s.check(*s.attend())
+
+
+@pytest.mark.parametrize("new", [1, 5, 200])
+def test_repeated_calls_give_the_same_bits(cuda, new):
+    import torch
+    s = Setup(cuda, [3000, 1200, 77], [new, new, min(new, 77)], 8, 2)
+    first, l0 = s.attend()
+    for _ in range(5):
+        again, l1 = s.attend()
+        assert torch.equal(first, again) and torch.equal(l0, l1)
+
+
+@pytest.mark.parametrize("D", [128, 64])
+def test_agrees_with_the_dense_attention_on_the_values_read_back(cuda, D):
+    """Non-causal attention over the cache against AttentionPlan on what `read` returns: both take the same fp16
+    K and V, so they differ by the kernels' own rounding: twice the tolerance of one."""
+    import torch
+    B, S, H, Hk = 2, 320, 4, 2
+    s = Setup(cuda, [S] * B, [S] * B, H, Hk, D=D, causal=False, page=64)
+    K, V = s.plan.read(s.cache, s.batch)
+    O, _ = s.attend()
+    dense = AttentionPlan(AttentionDimensions(S, S, D, H, Hk), batch=B, layout=MM4_ATTN_BSHD)
+    Q = torch.from_numpy(s.Q).to(cuda).view(B, S, H, D)
+    want = dense.run(Q, K.view(B, S, Hk, D), V.view(B, S, Hk, D)).view(B * S, H, D)
+    sync_check()
+    s.check(O)
+    tol = np.concatenate([ref.attention(s.Q[b * S:(b + 1) * S], s.K[b], s.V[b], S, False, s.plan.scale)[2]
+                          for b in range(B)])
+    assert (np.abs(O.double().cpu().numpy() - want.double().cpu().numpy()) <= 2 * tol).all()
+
+
+# ----------------------------------------------------------------------------------------------------------
+# together, as a program uses them
+# ----------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("bits,D", [(4, 128), (8, 64)])
+def test_prompt_then_tokens_one_by_one(cuda, bits, D):
+    """A prompt is written and attended over, then single tokens, then three at once, on one cache, with the
+    batch's tensors updated in place; every step against the definition on the values written so far."""
+    import torch
+    Hq, Hk, page, pages = 8, 2, 16, 40
+    plan = KVCachePlan(KVCacheDimensions(pages, page, Hq, Hk, D, bits))
+    cache = plan.allocate(cuda)
+    table = np.random.default_rng(0).permutation(pages)[:36].reshape(2, 18).astype(np.int32)
+    tt = torch.from_numpy(table).to(cuda)
+    lengths = torch.zeros(2, dtype=torch.int32, device=cuda)
+    held = [[np.zeros((0, Hk, D), np.float16)] * 2 for _ in range(2)]
+    step = 0
+    for new in ([200, 71], [1, 1], [1, 1], [1, 0], [3, 3], [1, 1]):
+        step += 1
+        offsets = torch.tensor([0, new[0], new[0] + new[1]], dtype=torch.int32, device=cuda)
+        lengths += torch.tensor(new, dtype=torch.int32, device=cuda)
+        tokens = sum(new)
+        batch = KVCacheBatch(tt, lengths, offsets, tokens, max(new))
+        K = data.normal((tokens, Hk, D), 1.0, 50 + step, 0)
+        V = data.normal((tokens, Hk, D), 1.0, 50 + step, 1)
+        Q = data.normal((tokens, Hq, D), 1.0, 50 + step, 2)
+        plan.append(torch.from_numpy(K).to(cuda), torch.from_numpy(V).to(cuda), cache, batch)
+        O = plan.attention(torch.from_numpy(Q).to(cuda), cache, batch)
+        sync_check()
+        got = O.double().cpu().numpy()
+        at = 0
+        for b in range(2):
+            r = slice(at, at + new[b])
+            at += new[b]
+            for kv, x in ((0, K), (1, V)):
+                held[b][kv] = np.concatenate([held[b][kv], ref.unpack(ref.pack(x[r], bits), D, bits)])
+            eO, _, tO, _ = ref.attention(Q[r], held[b][0], held[b][1], new[b], True, plan.scale)
+            assert (np.abs(got[r] - eO) <= tO).all(), (step, b)
+    whole = [len(held[0][0]), len(held[1][0])]
+    batch = KVCacheBatch(tt, lengths, torch.tensor([0, whole[0], sum(whole)], dtype=torch.int32, device=cuda),
+                         sum(whole), max(whole))
+    K, V = plan.read(cache, batch)
+    sync_check()
+    assert np.array_equal(K.cpu().numpy(), np.concatenate([held[0][0], held[1][0]]))
+    assert np.array_equal(V.cpu().numpy(), np.concatenate([held[0][1], held[1][1]]))
+
+
+def test_captured_step_replays_with_new_lengths(cuda):
+    """append + attention of one token, captured once and replayed as the lengths grow; a second captured step
+    of other sequences on the same plan, replayed in turn; both against the definition."""
+    import torch
+    Hq, Hk, D, page, pages = 8, 2, 128, 16, 64
+    plan = KVCachePlan(KVCacheDimensions(pages, page, Hq, Hk, D, 4))
+    states = []
+    for g in range(2):
+        cache = plan.allocate(cuda)
+        table = torch.randperm(pages, device=cuda).to(torch.int32).view(2, 32)
+        lengths = torch.tensor([100, 30 + g], dtype=torch.int32, device=cuda)
+        offsets = torch.tensor([0, 1, 2], dtype=torch.int32, device=cuda)
+        whole = torch.tensor([0, 100, 130 + g], dtype=torch.int32, device=cuda)
+        K0 = torch.from_numpy(data.normal((130 + g, Hk, D), 1.0, 60 + g, 0)).to(cuda)
+        V0 = torch.from_numpy(data.normal((130 + g, Hk, D), 1.0, 60 + g, 1)).to(cuda)
+        plan.append(K0, V0, cache, KVCacheBatch(table, lengths, whole, 130 + g, 100))
+        batch = KVCacheBatch(table, lengths, offsets, 2, 1)
+        K, V = torch.zeros(2, Hk, D, dtype=torch.float16, device=cuda), torch.zeros(2, Hk, D, dtype=torch.float16,
+                                                                                 device=cuda)
+        Q = torch.zeros(2, Hq, D, dtype=torch.float16, device=cuda)
+        O = torch.zeros_like(Q)
+        plan.attention(Q, cache, batch, O=O)  # warm-up
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            plan.append(K, V, cache, batch)
+            plan.attention(Q, cache, batch, O=O)
+        k0, v0 = (ref.unpack(ref.pack(t.cpu().numpy(), 4), D, 4) for t in (K0, V0))
+        held = [[k0[:100], v0[:100]], [k0[100:], v0[100:]]]
+        states.append((graph, cache, lengths, K, V, Q, O, held, batch))  # the batch keeps its tensors alive
+    for step in range(20):
+        for g, (graph, cache, lengths, K, V, Q, O, held, _) in enumerate(states):
+            lengths += 1
+            for i, t in enumerate((K, V, Q)):
+                t.copy_(torch.from_numpy(data.normal(tuple(t.shape), 1.0, 70 + step, 3 * g + i)))
+            graph.replay()
+            got = O.double().cpu().numpy()
+            kn, vn = (ref.unpack(ref.pack(t.cpu().numpy(), 4), D, 4) for t in (K, V))
+            for b in range(2):
+                held[b][0] = np.concatenate([held[b][0], kn[b:b + 1]])
+                held[b][1] = np.concatenate([held[b][1], vn[b:b + 1]])
+                eO, _, tO, _ = ref.attention(Q[b:b + 1].cpu().numpy(), held[b][0], held[b][1], 1, True, plan.scale)
+                assert (np.abs(got[b:b + 1] - eO) <= tO).all(), (step, g, b)
+    sync_check()
+
+
+def test_two_streams_at_once(cuda):
+    """The same plan on two streams with work in flight on both; each call has a workspace of its own."""
+    import torch
+    a = Setup(cuda, [8000, 3001], [1, 1], 8, 2, seed=5)
+    b = Setup(cuda, [5000], [3], 8, 2, seed=6)
+    wa, wb = a.attend()[0], b.attend()[0]
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    Qa, Qb = torch.from_numpy(a.Q).to(cuda), torch.from_numpy(b.Q).to(cuda)
+    torch.cuda.synchronize()
+    out = []
+    for _ in range(20):
+        out.append((a.plan.attention(Qa, a.cache, a.batch, stream=s1), b.plan.attention(Qb, b.cache, b.batch,
+                                                                                        stream=s2)))
+    torch.cuda.synchronize()
+    for x, y in out:
+        assert torch.equal(x, wa) and torch.equal(y, wb)
+
+
+def test_cache_offsets_past_32_bits(cuda):
+    """A pool of over 5 GB whose used pages lie at its end."""
+    import torch
+    page, Hk, D = 256, 16, 128
+    page_bytes = Hk * 2 * page * ref.row_bytes(D, 4)
+    pages = (5 << 30) // page_bytes
+    plan = KVCachePlan(KVCacheDimensions(pages, page, Hk, Hk, D, 4))
+    assert plan.cacheBytes > 1 << 32
+    cache = plan.allocate(cuda)
+    for new in (1, 200):
+        ln = 300
+        table = torch.tensor([[pages - 1, pages - 2]], dtype=torch.int32, device=cuda)
+        lengths = torch.tensor([ln], dtype=torch.int32, device=cuda)
+        K, V = data.normal((ln, Hk, D), 1.0, 80, 0), data.normal((ln, Hk, D), 1.0, 80, 1)
+        Q = data.normal((new, Hk, D), 1.0, 80, 2)
+        plan.append(torch.from_numpy(K).to(cuda), torch.from_numpy(V).to(cuda), cache,
+                    KVCacheBatch(table, lengths, torch.tensor([0, ln], dtype=torch.int32, device=cuda), ln, ln))
+        O = plan.attention(torch.from_numpy(Q).to(cuda), cache,
+                           KVCacheBatch(table, lengths, torch.tensor([0, new], dtype=torch.int32, device=cuda), new,
+                                        new))
+        sync_check()
+        k, v = (ref.unpack(ref.pack(x, 4), D, 4) for x in (K, V))
+        eO, _, tO, _ = ref.attention(Q, k, v, new, True, plan.scale)
+        assert (np.abs(O.double().cpu().numpy() - eO) <= tO).all()
+    assert not cache[:pages - 2].any()
+
+
+# ----------------------------------------------------------------------------------------------------------
+# wrong batches: reported, contained
+# ----------------------------------------------------------------------------------------------------------
+
+def _reported(text):
+    with pytest.raises(MM4Error, match=text) as e:
+        sync_check()
+    assert e.value.status == MM4_ERR_INVALID
+    sync_check()  # reported once
+
+
+@pytest.mark.parametrize("new", [1, 100])
+@pytest.mark.parametrize("entry", [-1, 10 ** 6])
+def test_a_page_outside_the_pool_is_reported_and_touches_no_other_sequence(cuda, entry, new):
+    import torch
+    s = Setup(cuda, [200, 150, 170], [new, new, new], 4, 2, page=32)
+    s.batch.pageTable[1, 2] = entry
+    Q = torch.from_numpy(s.Q).to(cuda)
+    O = s.plan.attention(Q, s.cache, s.batch)
+    _reported("page number")
+    s.check(O, sequences=[0, 2])
+    K, V = s.plan.read(s.cache, s.batch)
+    if new > 1:  # rows 50 .. 149 reach the wrong entry, row 149 alone does not
+        _reported("page number")
+        s.plan.append(K, V, s.cache, s.batch)
+        _reported("page number")
+    sync_check()
+
+
+@pytest.mark.parametrize("new", [1, 100])
+def test_wrong_lengths_offsets_and_row_counts_are_reported(cuda, new):
+    import torch
+    s = Setup(cuda, [200, 150, 170], [new, new, new], 4, 2, page=32)
+    Q = torch.from_numpy(s.Q).to(cuda)
+    for value in (-5, 10 ** 6, 2 ** 31 - 1):
+        s.batch.lengths[1] = value
+        O = s.plan.attention(Q, s.cache, s.batch)
+        with pytest.raises(MM4Error):  # a length too long also reaches the table's entries behind the sequence
+            sync_check()
+        sync_check()
+        s.check(O, sequences=[0, 2])
+    s.batch.lengths[1] = 150
+    keep = s.batch.offsets.clone()
+    for bad in ([0, new, 2 * new, 3 * new + 1], [0, new, 2 * new, -1]):
+        s.batch.offsets.copy_(torch.tensor(bad, dtype=torch.int32))
+        O = s.plan.attention(Q, s.cache, s.batch)
+        _reported("offsets")
+        s.check(O, sequences=[0, 1])
+    s.batch.offsets.copy_(keep)
+    few = KVCacheBatch(s.batch.pageTable, s.batch.lengths, torch.tensor([0, new, 2 * new, 3 * new], dtype=torch.int32,
+                                                                       device=cuda), 3 * new, max(1, new - 1))
+    if new > 1:
+        s.plan.attention(Q, s.cache, few)
+        _reported("max_new")
