@@ -1,5 +1,18 @@
 // Attention over the key / value cache: O = softmax(scale * Q K^T) V with K
-// and V read from the cache's codes.
+// and V read from the cache's codes. This file has what the kernels share (the
+// division of the work, the join of partial results) and the kernel for rows
+// of many tokens; kv_attention_few_sm100.cuh has the one for few rows.
+//
+// The work. A unit is one key / value head of one sequence with up to ROWS rows
+// (a row is one query head of one token; the heads of a group share a unit,
+// so their keys are read once). A unit's keys are walked in tiles, and all
+// tiles of the call, unit after unit, form one line that is cut into equal
+// ranges, one for each worker. The lengths lie on the device and may change
+// between replays of a captured call, so every worker finds its range itself
+// from two scans over the lengths. A unit that spans several workers leaves
+// one partial result (m, l and unscaled O) per worker in the workspace, and a
+// second kernel joins them in worker order, so results do not depend on
+// timing.
 #pragma once
 
 #include "kv_cache_sm100.cuh"
@@ -16,7 +29,96 @@ struct KvAttnArgs {
   int heads_q, group;    // group = heads_q / heads_kv
   int causal;
   float scale_log2;      // scale * log2(e)
+  float* partials;       // workspace
+  int workers;           // of the launch
+  unsigned long long timeout_ns;
 };
+
+// A run of partials is found by arithmetic alone: worker w takes tiles
+// [w T / A, (w + 1) T / A) of the T on the line, A workers being active, so
+// tile x belongs to worker floor(((x + 1) A - 1) / T).
+__device__ __forceinline__ long long kv_range_begin(long long w, long long T, long long A) { return w * T / A; }
+__device__ __forceinline__ long long kv_worker_of(long long x, long long T, long long A) {
+  return ((x + 1) * A - 1) / T;
+}
+
+// Partials of worker w: slot 2 w is a segment that began in another worker's
+// range, slot 2 w + 1 one that begins a unit here and goes on elsewhere.
+// Each holds ROWS x D floats, then (m, l) of ROWS rows; m in the log2 domain.
+template <int D, int ROWS>
+struct KvPartial {
+  static constexpr int FLOATS = ROWS * (D + 2);
+};
+
+constexpr float KV_NO_MAX = -1e30f;  // running maximum of a row that has seen no key
+
+// Tiles of TK keys of sequence b (0 if it has no rows in this call; a row
+// block with no key still takes one tile, which writes its zeros).
+template <int TK>
+__device__ __forceinline__ int kv_tiles(const KvSequence& s) {
+  return s.n == 0 ? 0 : max(1, (s.len + TK - 1) / TK);
+}
+
+// Sum of kv_tiles over all sequences, by one warp.
+template <int TK>
+__device__ __forceinline__ long long kv_total_tiles(const KvBatch& kb, int lane) {
+  long long sum = 0;
+  for (int b = lane; b < kb.sequences; b += 32) sum += kv_tiles<TK>(kv_sequence(kb, b));
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+  return sum;
+}
+
+// Sequence b whose tiles hold x (x < the total), and the tiles before it.
+template <int TK>
+__device__ __forceinline__ int kv_find_tile(const KvBatch& kb, long long x, int lane, long long* before) {
+  long long done = 0;
+  for (int b0 = 0; b0 < kb.sequences; b0 += 32) {
+    const int b = b0 + lane;
+    const int t = b < kb.sequences ? kv_tiles<TK>(kv_sequence(kb, b)) : 0;
+    int inc = t;
+#pragma unroll
+    for (int s = 1; s < 32; s <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, inc, s);
+      if (lane >= s) inc += up;
+    }
+    const unsigned over = __ballot_sync(0xffffffffu, done + inc > x);
+    if (over != 0) {
+      const int k = __ffs(over) - 1;
+      *before = done + __shfl_sync(0xffffffffu, inc - t, k);
+      return b0 + k;
+    }
+    done += __shfl_sync(0xffffffffu, inc, 31);
+  }
+  *before = done;
+  return kb.sequences;  // not reached for x < the total
+}
+
+// Tiles of all sequences before b, by one warp.
+template <int TK>
+__device__ __forceinline__ long long kv_tiles_before(const KvBatch& kb, int b, int lane) {
+  long long sum = 0;
+  for (int i = lane; i < b; i += 32) sum += kv_tiles<TK>(kv_sequence(kb, i));
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+  return sum;
+}
+
+// Keys that row r of a unit sees: those before limit (<= 0: none).
+__device__ __forceinline__ int kv_limit(const KvSequence& s, int token, int causal) {
+  return causal ? s.len - (s.n - 1 - token) : s.len;
+}
+
+__device__ __forceinline__ float kv_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Lets the next kernel of the stream start its blocks, and waits in it until
+// the kernel before it has finished and its writes are visible.
+__device__ __forceinline__ void kv_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void kv_wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 __device__ __forceinline__ float kv_warp_sum(float x) {
 #pragma unroll

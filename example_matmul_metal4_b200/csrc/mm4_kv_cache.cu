@@ -6,6 +6,7 @@
 #include <cstdio>
 #include <new>
 
+#include "kv_attention_few_sm100.cuh"
 #include "kv_attention_sm100.cuh"
 #include "kv_cache_sm100.cuh"
 #include "mm4_internal.h"
@@ -114,6 +115,90 @@ mm4_status launch_io(const mm4_kv_cache_plan* p, KvIoArgs& a, bool write, cudaSt
   });
 }
 
+// Which kernel attention over a batch runs, from its sizes alone (the lengths
+// lie on the device).
+struct Form {
+  enum Kind { FEW8, FEW16, ROWS } kind;
+  bool team;         // FEW: whole units to a CTA, one launch
+  size_t workspace;
+  const char* name;
+};
+
+constexpr int kMaxCtas = 160;  // workspaces are sized for this many SMs
+
+template <int D, int BITS, int NT>
+size_t few_workspace() {
+  using Cfg = KvFew<D, BITS, NT>;
+  return sizeof(float) * 2 * kMaxCtas * Cfg::WARPS * KvPartial<D, Cfg::ROWS>::FLOATS;
+}
+
+Form attention_form(const mm4_kv_cache_plan* p, const mm4_kv_cache_batch* b) {
+  const int group = p->d.heads_q / p->d.heads_kv;
+  const long long rows = static_cast<long long>(b->max_new) * group;
+  Form f{Form::ROWS, false, 0, "kv_attention_row"};
+  if (rows > 16) return f;
+  const long long room = static_cast<long long>(b->pages_per_sequence) << p->page_shift;
+  const bool eight = rows <= 8;
+  f.kind = eight ? Form::FEW8 : Form::FEW16;
+  const int warps = p->d.head_dim == 128 && p->d.bits == 4 ? (eight ? KvFew<128, 4, 1>::WARPS : KvFew<128, 4, 2>::WARPS)
+                    : p->d.head_dim == 128                 ? (eight ? KvFew<128, 8, 1>::WARPS : KvFew<128, 8, 2>::WARPS)
+                    : p->d.bits == 4                       ? (eight ? KvFew<64, 4, 1>::WARPS : KvFew<64, 4, 2>::WARPS)
+                                                           : (eight ? KvFew<64, 8, 1>::WARPS : KvFew<64, 8, 2>::WARPS);
+  f.team = room <= 2 * KVF_TK * warps;
+  f.name = f.team ? (eight ? "kv_attention_few<8 rows, team>" : "kv_attention_few<16 rows, team>")
+                  : (eight ? "kv_attention_few<8 rows, split>" : "kv_attention_few<16 rows, split>");
+  if (!f.team) {
+    if (p->d.head_dim == 128)
+      f.workspace = p->d.bits == 4 ? (eight ? few_workspace<128, 4, 1>() : few_workspace<128, 4, 2>())
+                                   : (eight ? few_workspace<128, 8, 1>() : few_workspace<128, 8, 2>());
+    else
+      f.workspace = p->d.bits == 4 ? (eight ? few_workspace<64, 4, 1>() : few_workspace<64, 4, 2>())
+                                   : (eight ? few_workspace<64, 8, 1>() : few_workspace<64, 8, 2>());
+  }
+  return f;
+}
+
+// The join of partials, allowed to start while the kernel before it ends.
+template <int D, int ROWS, int TK>
+mm4_status launch_join(const KvAttnArgs& a, cudaStream_t st) {
+  const long long units = static_cast<long long>(a.kb.sequences) * a.kb.heads_kv;
+  if (units > 0x7fffffffLL) return fail(MM4_ERR_UNSUPPORTED, "too many sequences for one launch");
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(units), (ROWS + 7) / 8);
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kv_attention_join_kernel<D, ROWS, TK>, a);
+  if (e != cudaSuccess) return cuda_fail(e, "kv_attention_join_kernel launch");
+  return MM4_OK;
+}
+
+template <int D, int BITS, int NT>
+mm4_status launch_few(KvAttnArgs& a, bool team, int sms, cudaStream_t st) {
+  using Cfg = KvFew<D, BITS, NT>;
+  const void* kern = team ? reinterpret_cast<const void*>(kv_attention_few_kernel<D, BITS, NT, true>)
+                          : reinterpret_cast<const void*>(kv_attention_few_kernel<D, BITS, NT, false>);
+  mm4_status rc = ensure_smem_attr(kern, Cfg::SMEM_BYTES);
+  if (rc != MM4_OK) return rc;
+  if (team) {
+    const long long units = static_cast<long long>(a.kb.sequences) * a.kb.heads_kv;
+    const unsigned grid = static_cast<unsigned>(std::min<long long>(units, sms));
+    kv_attention_few_kernel<D, BITS, NT, true><<<grid, Cfg::WARPS * 32, Cfg::SMEM_BYTES, st>>>(a);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return cuda_fail(e, "kv_attention_few_kernel launch");
+    return MM4_OK;
+  }
+  a.workers = sms * Cfg::WARPS;
+  kv_attention_few_kernel<D, BITS, NT, false><<<sms, Cfg::WARPS * 32, Cfg::SMEM_BYTES, st>>>(a);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, "kv_attention_few_kernel launch");
+  return launch_join<D, Cfg::ROWS, KVF_TK>(a, st);
+}
+
 }  // namespace
 
 namespace mm4 {
@@ -218,19 +303,18 @@ mm4_status mm4_kv_cache_read(const mm4_kv_cache_plan* p, const mm4_kv_cache_batc
 }
 
 size_t mm4_kv_cache_attention_workspace_size(const mm4_kv_cache_plan* p, const mm4_kv_cache_batch* b) {
-  (void)b;
-  return p ? 0 : 0;
+  if (!p || !b || b->sequences <= 0 || b->tokens <= 0 || b->max_new <= 0) return 0;
+  return attention_form(p, b).workspace;
 }
 
 const char* mm4_kv_cache_attention_kernel_name(const mm4_kv_cache_plan* p, const mm4_kv_cache_batch* b) {
-  return p && b ? "kv_attention_row" : "";
+  if (!p || !b) return "";
+  return attention_form(p, b).name;
 }
 
 mm4_status mm4_kv_cache_attention(const mm4_kv_cache_plan* p, const mm4_kv_cache_batch* b, const void* Q,
                                   int64_t q_stride, const void* cache, void* O, int64_t o_stride, float* lse,
                                   void* workspace, size_t workspace_bytes, mm4_stream_t stream) {
-  (void)workspace;
-  (void)workspace_bytes;
   mm4_status rc = check_batch(p, b);
   if (rc != MM4_OK) return rc;
   if (b->sequences == 0 || b->tokens == 0) return MM4_OK;
@@ -240,6 +324,12 @@ mm4_status mm4_kv_cache_attention(const mm4_kv_cache_plan* p, const mm4_kv_cache
   if ((rc = check_rows("O", O, o_stride, width)) != MM4_OK) return rc;
   if ((rc = check_cache(cache)) != MM4_OK) return rc;
   if ((reinterpret_cast<uintptr_t>(lse) & 3u) != 0) return fail(MM4_ERR_INVALID, "lse must be 4-byte aligned");
+  const Form form = attention_form(p, b);
+  if (form.workspace > 0) {
+    if (!workspace || workspace_bytes < form.workspace)
+      return fail(MM4_ERR_WORKSPACE, "attention over this batch needs a %zu-byte workspace", form.workspace);
+    if (!aligned16(workspace)) return fail(MM4_ERR_INVALID, "workspace must be 16-byte aligned");
+  }
   DeviceInfo info;
   if ((rc = use_device(&info)) != MM4_OK) return rc;
   KvAttnArgs a{};
@@ -254,14 +344,23 @@ mm4_status mm4_kv_cache_attention(const mm4_kv_cache_plan* p, const mm4_kv_cache
   a.group = p->d.heads_q / p->d.heads_kv;
   a.causal = p->d.causal;
   a.scale_log2 = p->scale * 1.4426950408889634f;
+  a.partials = static_cast<float*>(workspace);
+  a.timeout_ns = wait_timeout_ns();
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const long long blocks = (static_cast<long long>(b->tokens) * p->d.heads_q + 3) / 4;
-  if (blocks > 0x7fffffffLL) return fail(MM4_ERR_UNSUPPORTED, "too many rows for one launch");
+  const int sms = std::min(info.sm_count, kMaxCtas);
+  if (form.kind == Form::ROWS) {
+    const long long blocks = (static_cast<long long>(b->tokens) * p->d.heads_q + 3) / 4;
+    if (blocks > 0x7fffffffLL) return fail(MM4_ERR_UNSUPPORTED, "too many rows for one launch");
+    return by_row(p->d, [&](auto, auto D, auto B) -> mm4_status {
+      kv_attention_row_kernel<D.value, B.value><<<static_cast<unsigned>(blocks), 128, 0, st>>>(a);
+      cudaError_t e = cudaGetLastError();
+      if (e != cudaSuccess) return cuda_fail(e, "kv_attention_row_kernel launch");
+      return MM4_OK;
+    });
+  }
   return by_row(p->d, [&](auto, auto D, auto B) -> mm4_status {
-    kv_attention_row_kernel<D.value, B.value><<<static_cast<unsigned>(blocks), 128, 0, st>>>(a);
-    cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return cuda_fail(e, "kv_attention_row_kernel launch");
-    return MM4_OK;
+    if (form.kind == Form::FEW8) return launch_few<D.value, B.value, 1>(a, form.team, sms, st);
+    return launch_few<D.value, B.value, 2>(a, form.team, sms, st);
   });
 }
 
