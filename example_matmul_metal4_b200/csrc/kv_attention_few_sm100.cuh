@@ -4,9 +4,11 @@
 // Bound by the cache's bytes: each is read once, 160 a token and head at
 // D = 128 in 4 bits, and the arithmetic has to hide behind them: at 6.4 TB/s
 // an SM has about 40 elements of K or V a clock to unpack, scale and multiply.
-//  - Every warp works alone: it copies its tiles of 32 keys into its own ring in
-//    shared memory (untiled bulk copies, a page is contiguous) and needs no
-//    barrier with other warps.
+//  - Every warp works alone on tiles of 32 keys that land in its own ring in
+//    shared memory (untiled bulk copies, a page is contiguous), without a barrier
+//    with other warps. One more warp does all the copying: lane i walks the
+//    range of warp i, so finding places and page numbers costs one instruction
+//    stream for all of them.
 //  - S^T = K Q^T and O^T += V^T P^T on m16n8k16 tensor instructions, with the
 //    cache as the 16-row operand and the rows of Q as the 8 columns: half
 //    the tensor work of a form with 16 padded rows of Q.
@@ -31,20 +33,34 @@ struct KvFew {
   static constexpr int ROWS = 8 * NT;
   static constexpr int ROW_BYTES = KvRow<D, BITS>::BYTES;
   static constexpr int STAGE_BYTES = 2 * KVF_TK * ROW_BYTES;  // K rows, then V rows
-  // Warps a CTA and tiles in flight a warp: up to 164 KB of copies in flight.
-  static constexpr int WARPS = NT == 1 && STAGE_BYTES <= 5120 ? 16 : 8;
+  // Warps that compute, and tiles in flight for each: up to 164 KB of copies in
+  // flight. 16 warps in all with 128 registers a thread, or 8 with more.
+  static constexpr int WARPS = NT == 1 && STAGE_BYTES <= 5120 ? 15 : 7;
+  static constexpr int THREADS = 32 * (WARPS + 1);
   static constexpr int STAGES = STAGE_BYTES * WARPS * 4 <= 168 * 1024 ? 4 : 2;
-  static constexpr int SLOTS = WARPS / 2;                     // of the join inside a CTA
+  static constexpr int SLOTS = (WARPS + 1) / 2;               // of the join inside a CTA
   static constexpr int RING_BYTES = WARPS * STAGES * STAGE_BYTES;
-  static constexpr int SMEM_BYTES = RING_BYTES + SLOTS * KvPartial<D, ROWS>::FLOATS * 4 + WARPS * STAGES * 8;
+  static constexpr int JOIN_BYTES = SLOTS * KvPartial<D, ROWS>::FLOATS * 4;
+  static constexpr int BAR_BYTES = 2 * WARPS * STAGES * 8;
+  static constexpr int SMEM_BYTES = RING_BYTES + JOIN_BYTES + BAR_BYTES + WARPS * 32;
 };
 
+// Where a warp's range begins: unit (sequence b, head h), tile n, and how much
+// there is (tiles, or units where a CTA takes whole units).
+struct alignas(16) KvStart {
+  int b, h, n, pad;
+  long long todo;
+};
+
+// d = a b + (FIRST ? 0 : d).
+template <bool FIRST>
 __device__ __forceinline__ void kv_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                        uint32_t b1) {
+  const float c0 = FIRST ? 0.f : d[0], c1 = FIRST ? 0.f : d[1], c2 = FIRST ? 0.f : d[2], c3 = FIRST ? 0.f : d[3];
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-      "{%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+      "{%10, %11, %12, %13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
 
 __device__ __forceinline__ uint32_t kv_transpose(uint32_t x) {
@@ -82,10 +98,11 @@ __device__ __forceinline__ void kv_load_words(const uint8_t* p, uint32_t (&w)[N]
 // Pairs of K's operand from one word of codes, in the order of kv_query_pairs:
 // 4 bits (0,4) (1,5) (2,6) (3,7); 8 bits (0,1) (2,3).
 template <int BITS>
-__device__ __forceinline__ void kv_key_pairs(uint32_t w, __half2 s2, __half2 z2, uint32_t (&out)[16 / BITS]) {
+__device__ __forceinline__ void kv_key_pairs(uint32_t w, __half2 s2, __half2 z2, uint32_t (&out)[16 / BITS],
+                                             uint32_t k1024) {
   if constexpr (BITS == 4) {
     __half2 c[4];
-    kv_codes4(w, c);
+    kv_codes4(w, c, k1024);
 #pragma unroll
     for (int j = 0; j < 4; ++j) out[j] = as_u32(__hfma2(c[j], s2, z2));
   } else {
@@ -97,36 +114,36 @@ __device__ __forceinline__ void kv_key_pairs(uint32_t w, __half2 s2, __half2 z2,
 // V's operand for one word of two keys: out[e] = (element e of key a, of key b).
 template <int BITS>
 __device__ __forceinline__ void kv_value_pairs(uint32_t wa, uint32_t wb, __half2 s2, __half2 z2,
-                                               uint32_t (&out)[32 / BITS]) {
+                                               uint32_t (&out)[32 / BITS], uint32_t k1024) {
   const uint32_t lo = __byte_perm(wa, wb, 0x5410), hi = __byte_perm(wa, wb, 0x7632);
   if constexpr (BITS == 4) {
     __half2 c[4];
-    kv_codes4(lo, c);
+    kv_codes4(lo, c, k1024);
 #pragma unroll
     for (int j = 0; j < 4; ++j) out[j] = as_u32(__hfma2(c[j], s2, z2));
-    kv_codes4(hi, c);
+    kv_codes4(hi, c, k1024);
 #pragma unroll
     for (int j = 0; j < 4; ++j) out[4 + j] = as_u32(__hfma2(c[j], s2, z2));
   } else {
     const __half2 m1024 = __float2half2_rn(-1024.0f);
-    out[0] = as_u32(__hfma2(__hadd2(kv_bits_1024(lo, 0x00FF00FFu), m1024), s2, z2));
-    out[1] = as_u32(__hfma2(__hadd2(kv_bits_1024(lo >> 8, 0x00FF00FFu), m1024), s2, z2));
-    out[2] = as_u32(__hfma2(__hadd2(kv_bits_1024(hi, 0x00FF00FFu), m1024), s2, z2));
-    out[3] = as_u32(__hfma2(__hadd2(kv_bits_1024(hi >> 8, 0x00FF00FFu), m1024), s2, z2));
+    out[0] = as_u32(__hfma2(__hadd2(kv_bits_1024(lo, 0x00FF00FFu, k1024), m1024), s2, z2));
+    out[1] = as_u32(__hfma2(__hadd2(kv_bits_1024(lo >> 8, 0x00FF00FFu, k1024), m1024), s2, z2));
+    out[2] = as_u32(__hfma2(__hadd2(kv_bits_1024(hi, 0x00FF00FFu, k1024), m1024), s2, z2));
+    out[3] = as_u32(__hfma2(__hadd2(kv_bits_1024(hi >> 8, 0x00FF00FFu, k1024), m1024), s2, z2));
   }
 }
 
-// One warp walks its range. Lane = 4 g + c: in K Q^T it has keys g and g + 8 of
-// each 16, the c-th quarter of the head dimension, and rows 2 c and 2 c + 1
-// of the result; in V^T P^T the g-th eighth of the head dimension and keys 2 c,
-// 2 c + 1, 2 c + 8, 2 c + 9.
+// A computing warp walks its range. Lane = 4 g + c: in K Q^T it has keys g and
+// g + 8 of each 16, the c-th quarter of the head dimension, and rows 2 c and
+// 2 c + 1 of the result; in V^T P^T the g-th eighth of the head dimension and
+// keys 2 c, 2 c + 1, 2 c + 8, 2 c + 9.
 //
 // TEAM: a CTA takes whole units, its warps every WARPS-th tile of each, and
 // joins them in shared memory: one launch and no workspace, for caches that
 // hold few keys a sequence. Otherwise a worker is a warp (worker index =
 // warp * CTAs + CTA, so few workers spread over the SMs).
 template <int D, int BITS, int NT, bool TEAM>
-__global__ void __launch_bounds__(KvFew<D, BITS, NT>::WARPS * 32, 1) kv_attention_few_kernel(const KvAttnArgs a) {
+__global__ void __launch_bounds__(KvFew<D, BITS, NT>::THREADS, 1) kv_attention_few_kernel(const KvAttnArgs a) {
   using Cfg = KvFew<D, BITS, NT>;
   using Row = KvRow<D, BITS>;
   constexpr int W = Cfg::WARPS, ST = Cfg::STAGES, RB = Cfg::ROW_BYTES;
@@ -139,56 +156,70 @@ __global__ void __launch_bounds__(KvFew<D, BITS, NT>::WARPS * 32, 1) kv_attentio
   extern __shared__ __align__(128) uint8_t kvf_smem[];
   const KvBatch& kb = a.kb;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int g = lane >> 2, c = lane & 3;
-  uint8_t* ring = kvf_smem + warp * ST * Cfg::STAGE_BYTES;
   float* join = reinterpret_cast<float*>(kvf_smem + Cfg::RING_BYTES);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(kvf_smem + Cfg::SMEM_BYTES) - W * ST + warp * ST;
+  uint64_t* full = reinterpret_cast<uint64_t*>(kvf_smem + Cfg::RING_BYTES + Cfg::JOIN_BYTES);  // [W][ST] landed
+  uint64_t* empty = full + W * ST;                                                              // [W][ST] read
+  KvStart* starts = reinterpret_cast<KvStart*>(kvf_smem + Cfg::RING_BYTES + Cfg::JOIN_BYTES + Cfg::BAR_BYTES);
   const Watchdog wd{&g_kv_wait, a.timeout_ns};
-  if (lane == 0) {
-    for (int i = 0; i < ST; ++i) mbar_init(&bars[i], 1);
-    fence_mbar_init();
-  }
-  __syncwarp();
   if (!TEAM) kv_launch_dependents();
 
-  // The range: tiles left of the loader and of the consumer, and their places.
+  if (warp < W) {
+    KvStart s{};
+    if constexpr (TEAM) {
+      const long long units = static_cast<long long>(kb.sequences) * kb.heads_kv;
+      s.todo = (units - blockIdx.x + gridDim.x - 1) / gridDim.x;
+      s.b = static_cast<int>(blockIdx.x / kb.heads_kv);
+      s.h = static_cast<int>(blockIdx.x % kb.heads_kv);
+      s.n = warp;
+    } else {
+      const long long total = kv_total_tiles<KVF_TK>(kb, lane) * kb.heads_kv;
+      const long long active = min(static_cast<long long>(a.workers), total);
+      const long long w = static_cast<long long>(warp) * gridDim.x + blockIdx.x;
+      if (w < active) {
+        const long long x = kv_range_begin(w, total, active);
+        s.todo = kv_range_begin(w + 1, total, active) - x;
+        long long before;
+        // Sequence b has heads * tiles(b) places on the line, from heads * before.
+        s.b = kv_find_tile<KVF_TK>(kb, x / kb.heads_kv, lane, &before);
+        const int tiles = s.b < kb.sequences ? max(1, kv_tiles<KVF_TK>(kv_sequence(kb, s.b))) : 1;
+        const long long in = x - before * kb.heads_kv;
+        s.h = static_cast<int>(in / tiles);
+        s.n = static_cast<int>(in % tiles);
+      }
+    }
+    if (lane == 0) {
+      starts[warp] = s;
+      for (int i = 0; i < ST; ++i) {
+        mbar_init(&full[warp * ST + i], 1);
+        mbar_init(&empty[warp * ST + i], 1);
+      }
+      fence_mbar_init();
+    }
+  }
+  __syncthreads();
+
+  // A place on the line, and the walk over units.
   struct Place {
     int b, h, n, tiles;
     KvSequence s;
+    long long todo;  // tiles left (TEAM: units)
   };
-  long long todo = 0;  // tiles of this warp (TEAM: units of this CTA)
-  Place at{};
-  if constexpr (TEAM) {
-    const long long units = static_cast<long long>(kb.sequences) * kb.heads_kv;
-    todo = (units - blockIdx.x + gridDim.x - 1) / gridDim.x;
-    if (todo <= 0) return;
-    at.b = static_cast<int>(blockIdx.x / kb.heads_kv);
-    at.h = static_cast<int>(blockIdx.x % kb.heads_kv);
-    at.n = warp;
-  } else {
-    const long long total = kv_total_tiles<KVF_TK>(kb, lane) * kb.heads_kv;
-    const long long active = min(static_cast<long long>(a.workers), total);
-    const long long w = static_cast<long long>(warp) * gridDim.x + blockIdx.x;
-    if (w >= active) return;
-    const long long x = kv_range_begin(w, total, active);
-    todo = kv_range_begin(w + 1, total, active) - x;
-    long long before;
-    at.b = kv_find_tile<KVF_TK>(kb, x / kb.heads_kv, lane, &before);
-    // x / heads lies in this sequence: its tiles start at heads * before.
-    at.s = kv_sequence(kb, at.b);
-    at.tiles = kv_tiles<KVF_TK>(at.s);
-    const long long in = x - before * kb.heads_kv;
-    at.h = static_cast<int>(in / at.tiles);
-    at.n = static_cast<int>(in % at.tiles);
-  }
-
-  // Moves to the next unit.
-  auto next_unit = [&](Place& p) {
+  auto place_of = [&](int w) {
+    const KvStart s = starts[w];
+    Place p{};
+    p.b = s.b;
+    p.h = s.h;
+    p.n = s.n;
+    p.todo = s.todo;
+    return p;
+  };
+  auto next_unit = [&](Place& p, int w) {
     if constexpr (TEAM) {
       const long long u = static_cast<long long>(p.b) * kb.heads_kv + p.h + gridDim.x;
       p.b = static_cast<int>(u / kb.heads_kv);
       p.h = static_cast<int>(u % kb.heads_kv);
-      p.n = warp;
+      p.n = w;
+      --p.todo;
     } else {
       p.n = 0;
       if (++p.h == kb.heads_kv) {
@@ -197,97 +228,120 @@ __global__ void __launch_bounds__(KvFew<D, BITS, NT>::WARPS * 32, 1) kv_attentio
       }
     }
   };
-  auto read_sequence = [&](Place& p) {
-    p.s = kv_sequence(kb, p.b);
-    p.tiles = kv_tiles<KVF_TK>(p.s);
-  };
-
-  // ------------------------------------------------------------ loader
-  Place ld = at;
-  long long ld_todo = todo;   // TEAM: units, else tiles
-  int ids_b = -1, ids_base = 0, ids = 0;  // 32 page numbers of sequence ids_b from ids_base, one a lane
-  int loaded = 0;             // tiles issued
-  // Skips sequences without rows (and, in TEAM, units whose tiles end before
-  // this warp's first); false when the range is done.
-  auto settle = [&](Place& p, long long& left) -> bool {
-    while (left > 0 && p.b < kb.sequences) {
-      read_sequence(p);
+  // Goes on to the next tile there is (sequences without rows have none, and in
+  // TEAM a unit may end before this warp's first); false at the range's end.
+  auto settle = [&](Place& p, int w) -> bool {
+    while (p.todo > 0 && p.b < kb.sequences) {
+      p.s = kv_sequence(kb, p.b);
+      p.tiles = kv_tiles<KVF_TK>(p.s);
       if (p.n < p.tiles) return true;
-      next_unit(p);
-      if (TEAM) --left;
+      next_unit(p, w);
     }
     return false;
   };
-  bool ld_have = settle(ld, ld_todo);
-  auto load_next = [&]() {
-    if (!ld_have) return;
-    const int st = loaded % ST;
-    uint8_t* dst = ring + st * Cfg::STAGE_BYTES;
-    const int key0 = ld.n * KVF_TK;
-    const int valid = ld.s.len - key0;  // <= 0 only for a sequence of length 0
+
+  if (warp == W) {
+    // ------------------------------------------------------------ copies
+    const int w = min(lane, W - 1);
+    uint8_t* ring = kvf_smem + w * ST * Cfg::STAGE_BYTES;
+    uint64_t* my_full = full + w * ST;
+    uint64_t* my_empty = empty + w * ST;
     const int ps = 1 << kb.page_shift;
-    const int chunk = min(KVF_TK, ps);  // keys of a copy
-    const int copies = valid <= 0 ? 0 : (valid > chunk && chunk < KVF_TK) ? 2 : 1;
-    if (copies > 0) {
-      const int first = key0 >> kb.page_shift;
-      if (ids_b != ld.b || first < ids_base || first + copies > ids_base + 32) {
-        ids_b = ld.b;
-        ids_base = first;
-        const int i = first + lane;
-        ids = 0;
-        if (i < kb.pages_per_seq && (i << kb.page_shift) < ld.s.len) {
-          ids = __ldg(kb.table + static_cast<long long>(ld.b) * kb.pages_per_seq + i);
-          if (ids < 0 || ids >= kb.pages) {
-            kv_note(KV_DATA_PAGE);
-            ids = 0;  // read in place of the page outside the pool
+    const int chunk = min(KVF_TK, ps);  // keys of a copy: a tile lies in one page, or in two of 16
+    Place p = place_of(w);
+    if (lane >= W) p.todo = 0;
+    bool have = settle(p, w);
+    int page[2] = {0, 0};               // of the next tile
+    int copies = 0;
+    // Reads the page numbers of the next tile; they are looked at when it is
+    // copied, so their latency is not waited for here.
+    auto look_up = [&]() {
+      const int key0 = p.n * KVF_TK;
+      const int valid = p.s.len - key0;  // <= 0 only for a sequence of length 0
+      copies = valid <= 0 ? 0 : (valid > chunk && chunk < KVF_TK) ? 2 : 1;
+      const int* t = kb.table + static_cast<long long>(p.b) * kb.pages_per_seq + (key0 >> kb.page_shift);
+      if (copies > 0) page[0] = __ldg(t);
+      if (copies > 1) page[1] = __ldg(t + 1);
+    };
+    if (have) look_up();
+    int issued = 0;
+    uint64_t since = globaltimer_ns();
+    while (__any_sync(0xffffffffu, have)) {
+      const int st = issued % ST;
+      const bool go = have && (issued < ST || mbar_test_wait(&my_empty[st], (issued / ST - 1) & 1));
+      if (go) {
+        uint8_t* dst = ring + st * Cfg::STAGE_BYTES;
+        const uint32_t bytes = static_cast<uint32_t>(chunk * RB);
+        if (copies == 0) {
+          mbar_arrive(&my_full[st]);
+        } else {
+          mbar_arrive_expect_tx(&my_full[st], bytes * 2 * copies);
+          for (int i = 0; i < copies; ++i) {
+            int id = page[i];
+            if (id < 0 || id >= kb.pages) {
+              kv_note(KV_DATA_PAGE);
+              id = 0;  // read in place of the page outside the pool
+            }
+            const uint8_t* src = a.cache + id * kb.page_bytes +
+                                 (static_cast<long long>(p.h * 2 << kb.page_shift) + (p.n * KVF_TK & (ps - 1))) * RB;
+            bulk_load(dst + i * chunk * RB, src, bytes, &my_full[st]);
+            bulk_load(dst + (KVF_TK + i * chunk) * RB, src + (static_cast<long long>(RB) << kb.page_shift), bytes,
+                      &my_full[st]);
           }
         }
+        ++issued;
+        if constexpr (TEAM) {
+          p.n += W;
+          if (p.n >= p.tiles) {
+            next_unit(p, w);
+            have = settle(p, w);
+          }
+        } else {
+          --p.todo;
+          if (++p.n == p.tiles) {
+            next_unit(p, w);
+            have = settle(p, w);
+          } else {
+            have = p.todo > 0;
+          }
+        }
+        if (have) look_up();
       }
-      const int mine = lane >> 1, kv = lane & 1;  // lanes 0 .. 2 copies - 1 issue one copy each
-      const int page = __shfl_sync(0xffffffffu, ids, min(31, first - ids_base + min(mine, copies - 1)));
-      const uint32_t bytes = static_cast<uint32_t>(chunk * RB);
-      if (lane == 0) mbar_arrive_expect_tx(&bars[st], bytes * 2 * copies);
-      __syncwarp();
-      if (mine < copies) {
-        const uint8_t* src = a.cache + page * kb.page_bytes +
-                             (static_cast<long long>((ld.h * 2 + kv) << kb.page_shift) + (key0 & (ps - 1))) * RB;
-        bulk_load(dst + (kv * KVF_TK + mine * chunk) * RB, src, bytes, &bars[st]);
-      }
-    } else if (lane == 0) {
-      mbar_arrive(&bars[st]);
-    }
-    ++loaded;
-    if constexpr (TEAM) {
-      ld.n += W;
-      if (ld.n >= ld.tiles) {
-        next_unit(ld);
-        --ld_todo;
-        ld_have = settle(ld, ld_todo);
-      }
-    } else {
-      --ld_todo;
-      if (++ld.n == ld.tiles) {
-        next_unit(ld);
-        ld_have = settle(ld, ld_todo);
+      if (__any_sync(0xffffffffu, go)) {
+        since = globaltimer_ns();
       } else {
-        ld_have = ld_todo > 0;
+        __nanosleep(40);
+        const bool late = globaltimer_ns() - since > wd.limit_ns;
+        if (late) record_error(wd.status, MM4_ERR_TIMEOUT, 113);
+        if (__any_sync(0xffffffffu, late || aborted(wd.status))) break;
       }
     }
-  };
-  for (int i = 0; i < ST; ++i) load_next();
+    // Copies still in flight after a run-out wait land before the CTA ends.
+    for (int i = max(0, issued - ST); i < issued; ++i) mbar_wait(&my_full[i % ST], (i / ST) & 1, wd, 112);
+    return;
+  }
 
-  // ------------------------------------------------------------ consumer
+  // ------------------------------------------------------------ computation
+  const int g = lane >> 2, c = lane & 3;
+  const uint8_t* ring = kvf_smem + warp * ST * Cfg::STAGE_BYTES;
+  uint64_t* my_full = full + warp * ST;
+  uint64_t* my_empty = empty + warp * ST;
+  Place at = place_of(warp);
   uint32_t q[NT][D / 16][2];
   float acc[NT][MT][4];
-  float m[NT][2], l[NT][2];
+  float m[NT][2], l[NT][2];  // running maximum (log2 domain) and sum of rows 2 c, 2 c + 1
+  float raise[NT][2];        // the score above which the maximum is raised
   int limit[NT][2];
-  int used = 0;  // tiles consumed
+  int clear = 0;             // keys before this one are masked in no row
+  int used = 0;              // tiles consumed
   bool ok = true;
-  const float sl2 = a.scale_log2;
+  const float sl2 = a.scale_log2, inv_sl2 = 1.0f / sl2;
+  const uint32_t k1024 = __shfl_sync(0xffffffffu, a.k1024, 0);
 
   auto start_unit = [&](const Place& p) {
     const int rows = min(p.s.n * a.group, Cfg::ROWS);
     if (static_cast<long long>(p.s.n) * a.group > Cfg::ROWS || p.s.n > kb.max_new) kv_note(KV_DATA_NEW);
+    clear = p.s.len;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int r = nt * 8 + g;
@@ -316,7 +370,9 @@ __global__ void __launch_bounds__(KvFew<D, BITS, NT>::WARPS * 32, 1) kv_attentio
       for (int e = 0; e < 2; ++e) {
         const int row = nt * 8 + 2 * c + e;
         limit[nt][e] = row < rows ? kv_limit(p.s, row / a.group, a.causal) : p.s.len;
+        clear = min(clear, limit[nt][e]);
         m[nt][e] = KV_NO_MAX;
+        raise[nt][e] = -INFINITY;
         l[nt][e] = 0.f;
       }
 #pragma unroll
@@ -324,12 +380,23 @@ __global__ void __launch_bounds__(KvFew<D, BITS, NT>::WARPS * 32, 1) kv_attentio
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[nt][t][e] = 0.f;
     }
+    clear = min(clear, __shfl_xor_sync(0xffffffffu, clear, 1));
+    clear = min(clear, __shfl_xor_sync(0xffffffffu, clear, 2));
   };
 
   auto tile = [&](const Place& p) {
     const uint8_t* sk = ring + (used % ST) * Cfg::STAGE_BYTES;
     const uint8_t* sv = sk + KVF_TK * RB;
     const int key0 = p.n * KVF_TK;
+    const bool masked = key0 + KVF_TK > clear;
+    if (masked && key0 + lane >= p.s.len) {
+      // Rows behind the sequence hold anything: with a scale and zero of 0 their
+      // values are 0, and so is their product with P = 0.
+      for (int i = 0; i < D / KV_GROUP; ++i)
+        *reinterpret_cast<uint32_t*>(const_cast<uint8_t*>(sv) + lane * RB + Row::CODES + 4 * i) = 0u;
+      fence_proxy_async_smem();  // before the next copy into this stage
+    }
+    __syncwarp();
     // S^T for 2 x 16 keys.
     float s[2][NT][4];
 #pragma unroll
@@ -343,29 +410,25 @@ __global__ void __launch_bounds__(KvFew<D, BITS, NT>::WARPS * 32, 1) kv_attentio
       const __half2 pb = *reinterpret_cast<const __half2*>(kb8 + Row::CODES + (c * KC / KV_GROUP) * 4);
       const __half2 sa = __low2half2(pa), za = __high2half2(pa), sb = __low2half2(pb), zb = __high2half2(pb);
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[hf][nt][e] = 0.f;
-#pragma unroll
       for (int i = 0; i < KW; ++i) {
         uint32_t xa[16 / BITS], xb[16 / BITS];
-        kv_key_pairs<BITS>(wa[i], sa, za, xa);
-        kv_key_pairs<BITS>(wb[i], sb, zb, xb);
+        kv_key_pairs<BITS>(wa[i], sa, za, xa, k1024);
+        kv_key_pairs<BITS>(wb[i], sb, zb, xb, k1024);
 #pragma unroll
         for (int j = 0; j < 8 / BITS; ++j) {
           const int step = i * (8 / BITS) + j;
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-            kv_mma(s[hf][nt], xa[2 * j], xb[2 * j], xa[2 * j + 1], xb[2 * j + 1], q[nt][step][0], q[nt][step][1]);
+          for (int nt = 0; nt < NT; ++nt) {
+            if (step == 0)
+              kv_mma<true>(s[hf][nt], xa[0], xb[0], xa[1], xb[1], q[nt][0][0], q[nt][0][1]);
+            else
+              kv_mma<false>(s[hf][nt], xa[2 * j], xb[2 * j], xa[2 * j + 1], xb[2 * j + 1], q[nt][step][0],
+                            q[nt][step][1]);
+          }
         }
       }
     }
-    // Masks: keys at and behind a row's limit.
-    bool inside = true;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) inside = inside && key0 + KVF_TK <= limit[nt][0] && key0 + KVF_TK <= limit[nt][1];
-    inside = __all_sync(0xffffffffu, inside);
-    if (!inside) {
+    if (masked) {
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
@@ -381,8 +444,8 @@ __global__ void __launch_bounds__(KvFew<D, BITS, NT>::WARPS * 32, 1) kv_attentio
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        mx[nt][e] = fmaxf(fmaxf(s[0][nt][e], s[0][nt][e + 2]), fmaxf(s[1][nt][e], s[1][nt][e + 2])) * sl2;
-        grow = grow || mx[nt][e] > m[nt][e] + 8.0f;
+        mx[nt][e] = fmaxf(fmax3(s[0][nt][e], s[0][nt][e + 2], s[1][nt][e]), s[1][nt][e + 2]);
+        grow = grow || mx[nt][e] > raise[nt][e];
       }
     if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
@@ -393,9 +456,10 @@ __global__ void __launch_bounds__(KvFew<D, BITS, NT>::WARPS * 32, 1) kv_attentio
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-          const float m_new = fmaxf(m[nt][e], x);
+          const float m_new = fmaxf(m[nt][e], x * sl2);
           const float f = kv_ex2(m[nt][e] - m_new);
           m[nt][e] = m_new;
+          raise[nt][e] = (m_new + 8.0f) * inv_sl2;
           l[nt][e] *= f;
 #pragma unroll
           for (int t = 0; t < MT; ++t) {
@@ -419,37 +483,46 @@ __global__ void __launch_bounds__(KvFew<D, BITS, NT>::WARPS * 32, 1) kv_attentio
         pt[hf][nt][0] = kv_transpose(pack_half2(p4[0], p4[1]));
         pt[hf][nt][1] = kv_transpose(pack_half2(p4[2], p4[3]));
       }
-    // O^T += V^T P^T. Rows behind the sequence hold anything: their scale and
-    // zero count as 0, so the product with P = 0 is 0.
-    const int valid = p.s.len - key0;
+    // O^T += V^T P^T.
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
       uint32_t w4[4][VW];
       __half2 par[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int key = hf * 16 + 2 * c + (i & 1) + (i >> 1) * 8;
-        const uint8_t* row = sv + key * RB;
+        const uint8_t* row = sv + (hf * 16 + 2 * c + (i & 1) + (i >> 1) * 8) * RB;
         kv_load_words<VW, RB % 16 == 0>(row + g * (VC * BITS / 8), w4[i]);
         par[i] = *reinterpret_cast<const __half2*>(row + Row::CODES + (g * VC / KV_GROUP) * 4);
-        if (key >= valid) par[i] = __float2half2_rn(0.f);
       }
       const __half2 s01 = __lows2half2(par[0], par[1]), z01 = __highs2half2(par[0], par[1]);
       const __half2 s23 = __lows2half2(par[2], par[3]), z23 = __highs2half2(par[2], par[3]);
 #pragma unroll
       for (int i = 0; i < VW; ++i) {
         uint32_t x[32 / BITS], y[32 / BITS];
-        kv_value_pairs<BITS>(w4[0][i], w4[1][i], s01, z01, x);
-        kv_value_pairs<BITS>(w4[2][i], w4[3][i], s23, z23, y);
+        kv_value_pairs<BITS>(w4[0][i], w4[1][i], s01, z01, x, k1024);
+        kv_value_pairs<BITS>(w4[2][i], w4[3][i], s23, z23, y, k1024);
 #pragma unroll
         for (int j = 0; j < 16 / BITS; ++j) {
           const int t = i * (16 / BITS) + j;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
-            kv_mma(acc[nt][t], x[2 * j], x[2 * j + 1], y[2 * j], y[2 * j + 1], pt[hf][nt][0], pt[hf][nt][1]);
+            kv_mma<false>(acc[nt][t], x[2 * j], x[2 * j + 1], y[2 * j], y[2 * j + 1], pt[hf][nt][0], pt[hf][nt][1]);
         }
       }
     }
+  };
+  // Waits for the next tile, computes it and gives its stage back.
+  auto take = [&](const Place& p) -> bool {
+    if (!mbar_try_wait(&my_full[used % ST], (used / ST) & 1) &&
+        !mbar_wait(&my_full[used % ST], (used / ST) & 1, wd, 110))
+      ok = false;
+    ok = __all_sync(0xffffffffu, ok);
+    if (!ok) return false;
+    tile(p);
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&my_empty[used % ST]);
+    ++used;
+    return true;
   };
 
   // Sums l over the lanes that share a row.
@@ -490,20 +563,13 @@ __global__ void __launch_bounds__(KvFew<D, BITS, NT>::WARPS * 32, 1) kv_attentio
 
   if constexpr (!TEAM) {
     float* slots = a.partials + 2 * (static_cast<long long>(warp) * gridDim.x + blockIdx.x) * KvPartial<D, Cfg::ROWS>::FLOATS;
-    while (todo > 0 && ok) {
-      if (!settle(at, todo)) break;
+    while (ok && settle(at, warp)) {
       start_unit(at);
       const int n0 = at.n;
-      const int n1 = static_cast<int>(min(static_cast<long long>(at.tiles), at.n + todo));
-      for (; at.n < n1; ++at.n) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&bars[used % ST], (used / ST) & 1, wd, 110));
-        if (!ok) break;
-        tile(at);
-        __syncwarp();
-        ++used;
-        load_next();
-      }
-      todo -= n1 - n0;
+      const int n1 = static_cast<int>(min(static_cast<long long>(at.tiles), at.n + at.todo));
+      for (; at.n < n1; ++at.n)
+        if (!take(at)) break;
+      at.todo -= n1 - n0;
       sum_l();
       const int rows = min(at.s.n * a.group, Cfg::ROWS);
       if (n0 == 0 && n1 == at.tiles) {
@@ -529,29 +595,24 @@ __global__ void __launch_bounds__(KvFew<D, BITS, NT>::WARPS * 32, 1) kv_attentio
       } else {
         store_partial(slots + (n0 == 0 ? KvPartial<D, Cfg::ROWS>::FLOATS : 0), rows);
       }
-      if (n1 == at.tiles) next_unit(at);
+      if (n1 == at.tiles) next_unit(at, warp);
     }
   } else {
-    while (todo > 0) {  // every warp of the CTA walks the same units
-      read_sequence(at);
+    while (at.todo > 0) {  // every computing warp of the CTA walks the same units
+      at.s = kv_sequence(kb, at.b);
+      at.tiles = kv_tiles<KVF_TK>(at.s);
       if (at.tiles > 0) {
-        start_unit(at);
         const int rows = min(at.s.n * a.group, Cfg::ROWS);
-        for (; at.n < at.tiles && ok; at.n += W) {
-          ok = __all_sync(0xffffffffu, mbar_wait(&bars[used % ST], (used / ST) & 1, wd, 111));
-          if (!ok) break;
-          tile(at);
-          __syncwarp();
-          ++used;
-          load_next();
-        }
+        start_unit(at);
+        for (; ok && at.n < at.tiles; at.n += W)
+          if (!take(at)) break;
         sum_l();
         // Two rounds: the upper half of the warps hands over to the lower, then
         // all threads sum the lower half's slots.
         constexpr int F = KvPartial<D, Cfg::ROWS>::FLOATS;
         if (warp >= Cfg::SLOTS) store_partial(join + (warp - Cfg::SLOTS) * F, rows);
-        __syncthreads();
-        if (warp < Cfg::SLOTS) {
+        named_barrier(1, W * 32);
+        if (warp + Cfg::SLOTS < W) {
           const float* other = join + warp * F;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
@@ -572,7 +633,7 @@ __global__ void __launch_bounds__(KvFew<D, BITS, NT>::WARPS * 32, 1) kv_attentio
         }
         __syncwarp();
         if (warp < Cfg::SLOTS) store_partial(join + warp * F, rows);
-        __syncthreads();
+        named_barrier(1, W * 32);
         for (int i = threadIdx.x; i < rows * (D / 2); i += W * 32) {
           const int row = i / (D / 2), d = (i % (D / 2)) * 2;
           float mm = KV_NO_MAX;
@@ -593,14 +654,11 @@ __global__ void __launch_bounds__(KvFew<D, BITS, NT>::WARPS * 32, 1) kv_attentio
           *reinterpret_cast<__half2*>(o + d) = __floats2half2_rn(x * inv, y * inv);
           if (lse != nullptr && d == 0) *lse = (mm + log2f(ls)) * 0.6931471805599453f;
         }
-        __syncthreads();  // the slots are free for the next unit
+        named_barrier(1, W * 32);  // the slots are free for the next unit
       }
-      next_unit(at);
-      --todo;
+      next_unit(at, warp);
     }
   }
-  // Copies still in flight after a run-out wait land before the CTA ends.
-  for (; used < loaded; ++used) mbar_wait(&bars[used % ST], (used / ST) & 1, wd, 112);
 }
 
 // Joins the partials of the units that several workers share: a block of 8

@@ -121,23 +121,28 @@ __device__ __forceinline__ uint8_t* kv_place(const KvBatch& kb, uint8_t* cache, 
 __device__ __forceinline__ __half2 as_half2(uint32_t x) { return *reinterpret_cast<__half2*>(&x); }
 __device__ __forceinline__ uint32_t as_u32(__half2 x) { return *reinterpret_cast<uint32_t*>(&x); }
 
-// (x & mask) | 0x6400 in both halves: fp16 1024 + the masked bits, exactly.
-__device__ __forceinline__ __half2 kv_bits_1024(uint32_t x, uint32_t mask) {
+constexpr uint32_t KV_1024 = 0x64006400u;  // fp16 1024 in both halves
+
+// (x & mask) | KV_1024: fp16 1024 + the masked bits, exactly. The kernels that
+// unpack in their inner loops get KV_1024 as an argument: as a literal it would be
+// moved into a register again for each use, since the mask takes the one
+// immediate operand of the instruction.
+__device__ __forceinline__ __half2 kv_bits_1024(uint32_t x, uint32_t mask, uint32_t k1024) {
   uint32_t r;
-  asm("lop3.b32 %0, %1, %2, 0x64006400, 0xEA;" : "=r"(r) : "r"(x), "r"(mask));
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(x), "r"(mask), "r"(k1024));
   return as_half2(r);
 }
 
 // The codes of a word whose 16-bit halves hold four 4-bit codes each: out[j] =
 // (code j of the low half, code j of the high half) as exact integers.
-__device__ __forceinline__ void kv_codes4(uint32_t w, __half2 (&out)[4]) {
+__device__ __forceinline__ void kv_codes4(uint32_t w, __half2 (&out)[4], uint32_t k1024) {
   const __half2 m1024 = __float2half2_rn(-1024.0f), m64 = __float2half2_rn(-64.0f),
                 sixteenth = __float2half2_rn(0.0625f);
   const uint32_t v = w >> 8;
-  out[0] = __hadd2(kv_bits_1024(w, 0x000F000Fu), m1024);
-  out[1] = __hfma2(kv_bits_1024(w, 0x00F000F0u), sixteenth, m64);  // (1024 + 16 c) / 16 - 64
-  out[2] = __hadd2(kv_bits_1024(v, 0x000F000Fu), m1024);
-  out[3] = __hfma2(kv_bits_1024(v, 0x00F000F0u), sixteenth, m64);
+  out[0] = __hadd2(kv_bits_1024(w, 0x000F000Fu, k1024), m1024);
+  out[1] = __hfma2(kv_bits_1024(w, 0x00F000F0u, k1024), sixteenth, m64);  // (1024 + 16 c) / 16 - 64
+  out[2] = __hadd2(kv_bits_1024(v, 0x000F000Fu, k1024), m1024);
+  out[3] = __hfma2(kv_bits_1024(v, 0x00F000F0u, k1024), sixteenth, m64);
 }
 
 // Two of a word's four 8-bit codes, picked by a byte-permute selector whose
@@ -286,7 +291,7 @@ __global__ void __launch_bounds__(KV_IO_WARPS * 32) kv_read_kernel(const KvIoArg
     uint4 out;
     if constexpr (BITS == 4) {
       __half2 c[4];
-      kv_codes4(codes[i].x, c);  // pairs (0,4) (1,5) (2,6) (3,7)
+      kv_codes4(codes[i].x, c, KV_1024);  // pairs (0,4) (1,5) (2,6) (3,7)
       const uint32_t p0 = as_u32(__hfma2(c[0], s2, z2)), p1 = as_u32(__hfma2(c[1], s2, z2)),
                      p2 = as_u32(__hfma2(c[2], s2, z2)), p3 = as_u32(__hfma2(c[3], s2, z2));
       out = make_uint4(__byte_perm(p0, p1, 0x5410), __byte_perm(p2, p3, 0x5410), __byte_perm(p0, p1, 0x7632),

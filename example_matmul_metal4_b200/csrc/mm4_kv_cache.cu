@@ -187,13 +187,13 @@ mm4_status launch_few(KvAttnArgs& a, bool team, int sms, cudaStream_t st) {
   if (team) {
     const long long units = static_cast<long long>(a.kb.sequences) * a.kb.heads_kv;
     const unsigned grid = static_cast<unsigned>(std::min<long long>(units, sms));
-    kv_attention_few_kernel<D, BITS, NT, true><<<grid, Cfg::WARPS * 32, Cfg::SMEM_BYTES, st>>>(a);
+    kv_attention_few_kernel<D, BITS, NT, true><<<grid, Cfg::THREADS, Cfg::SMEM_BYTES, st>>>(a);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return cuda_fail(e, "kv_attention_few_kernel launch");
     return MM4_OK;
   }
   a.workers = sms * Cfg::WARPS;
-  kv_attention_few_kernel<D, BITS, NT, false><<<sms, Cfg::WARPS * 32, Cfg::SMEM_BYTES, st>>>(a);
+  kv_attention_few_kernel<D, BITS, NT, false><<<sms, Cfg::THREADS, Cfg::SMEM_BYTES, st>>>(a);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "kv_attention_few_kernel launch");
   return launch_join<D, Cfg::ROWS, KVF_TK>(a, st);
@@ -345,6 +345,7 @@ mm4_status mm4_kv_cache_attention(const mm4_kv_cache_plan* p, const mm4_kv_cache
   a.causal = p->d.causal;
   a.scale_log2 = p->scale * 1.4426950408889634f;
   a.partials = static_cast<float*>(workspace);
+  a.k1024 = KV_1024;
   a.timeout_ns = wait_timeout_ns();
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int sms = std::min(info.sm_count, kMaxCtas);
