@@ -1,0 +1,704 @@
+// Attention over the key / value cache for many rows (prompts, chunks of them,
+// and tokens times query heads beyond 16 rows).
+//
+// Bound by the tensor cores and the exponentials, as attention over fp16 K and
+// V is (4 D FLOP and one exponential per row and key); what the cache adds is
+// turning its codes into fp16 operands. That is done once per 64 keys for all
+// 128 x QT rows of a CTA by warps of its own, into the 128-byte-swizzled layout
+// that tcgen05.mma reads, and overlaps the products of earlier keys.
+//
+// A row is one query head of one token, rows of a unit ordered by token and
+// then head, so grouped heads fill the 128-row tiles and share the unpacked
+// keys. A unit is one key / value head of one sequence and 128 QT rows. 16 warps:
+//   warp 0        copies pages as they lie in the cache into a ring (untiled bulk
+//                 copies).
+//   warp 1        TMEM allocation; one lane issues S_i(g) = Q_i K(g)^T (M = 128,
+//                 N = 64) into slot g % 2 of row tile i.
+//   warp 2        one lane issues O_i += P_i(g) V(g) (P from TMEM).
+//   warp 3        copies the next unit's rows of Q when the last S has read them.
+//   QT x 4 warps  softmax, one row a thread: P = 2^(S scale log2 e - m), rescaling
+//                 O only when the maximum grew by more than 2^8; results out.
+//   the others    codes to fp16: a lane takes 32 elements (one scale and zero).
+// TMEM: two 64-column S slots for each row tile, then O_i (D columns each). Steps
+// of 64 keys are counted across a CTA's units (g), which fixes slots and
+// mbarrier phases; S runs two steps ahead of the softmax.
+#pragma once
+
+#include "attention_sm100.cuh"
+#include "kv_attention_sm100.cuh"
+
+namespace mm4 {
+
+constexpr int KVM_TK = 64;        // keys of a step
+constexpr int KVM_THREADS = 512;
+
+template <int D, int BITS, int QT>
+struct KvMany {
+  static constexpr int ROWS = 128 * QT;
+  static constexpr int Q_BYTES = 128 * D * 2;          // a row tile of Q
+  static constexpr int TILE_BYTES = KVM_TK * D * 2;    // unpacked K or V of a step
+  static constexpr int RAW_BYTES = 2 * KVM_TK * KvRow<D, BITS>::BYTES;
+  static constexpr int KS = 3, VS = 3;
+  static constexpr int RS = RAW_BYTES <= 10240 ? 3 : 2;
+  static constexpr int BAR_OFFSET = QT * Q_BYTES + (KS + VS) * TILE_BYTES + RS * RAW_BYTES;
+  static constexpr int SMEM_BYTES = BAR_OFFSET + 512 + 1024;
+  // Four warps unpack K and V in turn; with one row tile, four each.
+  static constexpr int UNPACK_WARPS = 12 - 4 * QT;
+  // Registers: 128 threads each of warps 0-3, the softmax warps and the
+  // unpacking warps; the sum must not exceed what the block is launched with.
+  static constexpr int REGS_LOW = 64;
+  static constexpr int REGS_SOFTMAX = QT == 2 ? 176 : 192;
+  static constexpr int REGS_UNPACK = QT == 2 ? 96 : 128;
+  static constexpr int REGS_NEEDED = (REGS_LOW + QT * REGS_SOFTMAX + (3 - QT) * REGS_UNPACK) / 4;
+  static_assert(REGS_NEEDED <= 128, "register split");
+  static_assert(SMEM_BYTES <= 232448, "shared memory");
+};
+
+enum : int {
+  SITE_KVM_RAW = 120,
+  SITE_KVM_Q = 121,
+  SITE_KVM_S = 122,
+  SITE_KVM_PV = 123,
+  SITE_KVM_SOFTMAX = 124,
+  SITE_KVM_UNPACK = 125,
+  SITE_KVM_DRAIN = 126,
+};
+
+// Row blocks of a sequence, and the steps of one: the keys its last row sees.
+__device__ __forceinline__ int kvm_blocks(const KvSequence& s, int group, int rows) {
+  return (s.n * group + rows - 1) / rows;
+}
+__device__ __forceinline__ int kvm_steps(const KvSequence& s, int rb, const KvAttnArgs& a, int rows) {
+  int limit = s.len;
+  if (a.causal) {
+    const int last = min((rb + 1) * rows - 1, s.n * a.group - 1) / a.group;
+    limit = min(s.len, kv_limit(s, last, 1));
+  }
+  return max(1, (limit + KVM_TK - 1) / KVM_TK);
+}
+// A sequence with more rows than max_new is left out (and reported).
+__device__ __forceinline__ KvSequence kvm_sequence(const KvAttnArgs& a, int b) {
+  KvSequence s = kv_sequence(a.kb, b);
+  if (s.n > a.kb.max_new) {
+    kv_note(KV_DATA_NEW);
+    s.n = 0;
+  }
+  return s;
+}
+__device__ __forceinline__ int kvm_sequence_steps(const KvAttnArgs& a, int b, int rows) {
+  if (b >= a.kb.sequences) return 0;
+  const KvSequence s = kvm_sequence(a, b);
+  const int blocks = kvm_blocks(s, a.group, rows);
+  int sum = 0;
+  for (int rb = 0; rb < blocks; ++rb) sum += kvm_steps(s, rb, a, rows);
+  return sum;
+}
+
+// A place on the line of all steps: sequences, their row blocks, heads, steps.
+struct KvmPlace {
+  int b, rb, h, n;
+};
+__device__ __forceinline__ long long kvm_total(const KvAttnArgs& a, int rows, int lane) {
+  long long sum = 0;
+  for (int b = lane; b < a.kb.sequences; b += 32) sum += kvm_sequence_steps(a, b, rows);
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+  return sum * a.kb.heads_kv;
+}
+// Place x (by one warp); also where its unit begins.
+__device__ __forceinline__ KvmPlace kvm_find(const KvAttnArgs& a, int rows, long long x, int lane,
+                                             long long* unit_begin, int* unit_steps) {
+  const int heads = a.kb.heads_kv;
+  long long done = 0;  // of whole sequences, for one head
+  for (int b0 = 0; b0 < a.kb.sequences; b0 += 32) {
+    const int t = kvm_sequence_steps(a, b0 + lane, rows);
+    long long inc = t;
+#pragma unroll
+    for (int s = 1; s < 32; s <<= 1) {
+      const long long up = __shfl_up_sync(0xffffffffu, inc, s);
+      if (lane >= s) inc += up;
+    }
+    const unsigned over = __ballot_sync(0xffffffffu, (done + inc) * heads > x);
+    if (over != 0) {
+      const int k = __ffs(over) - 1;
+      long long at = (done + __shfl_sync(0xffffffffu, inc - t, k)) * heads;
+      KvmPlace p{b0 + k, 0, 0, 0};
+      const KvSequence s = kvm_sequence(a, p.b);
+      const int blocks = kvm_blocks(s, a.group, rows);
+      for (; p.rb < blocks; ++p.rb) {
+        const long long all = static_cast<long long>(kvm_steps(s, p.rb, a, rows)) * heads;
+        if (at + all > x) break;
+        at += all;
+      }
+      const int steps = kvm_steps(s, p.rb, a, rows);
+      p.h = static_cast<int>((x - at) / steps);
+      p.n = static_cast<int>((x - at) % steps);
+      *unit_begin = x - p.n;
+      *unit_steps = steps;
+      return p;
+    }
+    done += __shfl_sync(0xffffffffu, inc, 31);
+  }
+  *unit_begin = x;
+  *unit_steps = 1;
+  return KvmPlace{a.kb.sequences, 0, 0, 0};
+}
+
+// Segments of a CTA's range: steps [n0, n1) of one unit.
+struct KvmSegment {
+  KvSequence s;
+  int b, rb, h, n0, n1, steps;
+};
+struct KvmWalk {
+  KvmPlace p;
+  long long left;
+};
+__device__ __forceinline__ bool kvm_next(const KvAttnArgs& a, int rows, KvmWalk& w, KvmSegment& g) {
+  while (w.left > 0 && w.p.b < a.kb.sequences) {
+    g.s = kvm_sequence(a, w.p.b);
+    const int blocks = kvm_blocks(g.s, a.group, rows);
+    if (w.p.rb >= blocks) {
+      w.p = KvmPlace{w.p.b + 1, 0, 0, 0};
+      continue;
+    }
+    g.b = w.p.b;
+    g.rb = w.p.rb;
+    g.h = w.p.h;
+    g.n0 = w.p.n;
+    g.steps = kvm_steps(g.s, g.rb, a, rows);
+    g.n1 = static_cast<int>(min(static_cast<long long>(g.steps), g.n0 + w.left));
+    w.left -= g.n1 - g.n0;
+    w.p.n = g.n1;
+    if (g.n1 == g.steps) {
+      w.p.n = 0;
+      if (++w.p.h == a.kb.heads_kv) {
+        w.p.h = 0;
+        ++w.p.rb;
+      }
+    }
+    return true;
+  }
+  return false;
+}
+
+// A partial of ROWS rows: O in groups of 4 elements, [D / 4][ROWS][4] floats, so
+// that a warp of rows writes and reads whole lines; then m [ROWS], l [ROWS].
+template <int D, int ROWS>
+__device__ __forceinline__ long long kvm_slot(long long slot) {
+  return slot * KvPartial<D, ROWS>::FLOATS;
+}
+
+template <int D, int BITS, int QT>
+__global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const __grid_constant__ KvAttnArgs a) {
+  using Cfg = KvMany<D, BITS, QT>;
+  using Row = KvRow<D, BITS>;
+  constexpr int ROWS = Cfg::ROWS, KS = Cfg::KS, VS = Cfg::VS, RS = Cfg::RS, RB = Row::BYTES;
+  constexpr int TB = Cfg::TILE_BYTES, QB = Cfg::Q_BYTES;
+  constexpr uint32_t IDESC_S = idesc_f16_f32(128, KVM_TK, false, false);
+  constexpr uint32_t IDESC_O = idesc_f16_f32(128, D, false, true);
+  constexpr int EMU = AttFwdCfg<D>::EMU_PER8;
+
+  extern __shared__ uint8_t kvm_smem_raw[];
+  const uint32_t raw_addr = smem_u32(kvm_smem_raw);
+  uint8_t* smem = kvm_smem_raw + ((1024u - (raw_addr & 1023u)) & 1023u);
+  uint8_t* sQ = smem;                       // [QT]
+  uint8_t* sK = smem + QT * QB;             // [KS]
+  uint8_t* sV = sK + KS * TB;               // [VS]
+  uint8_t* sR = sV + VS * TB;               // [RS] pages as they lie in the cache: K rows, V rows
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::BAR_OFFSET);
+  uint64_t* q_full = bars;                  // [tile] the unit's Q_i in place
+  uint64_t* q_empty = bars + 2;             // [tile] its last S_i complete
+  uint64_t* s_full = bars + 4;              // [tile][slot] S_i(g) in TMEM
+  uint64_t* p_full = bars + 8;              // [tile][slot] P_i(g) in TMEM, O_i rescaled
+  uint64_t* pv_done = bars + 12;            // [tile][slot] O_i += P_i(g) V(g) complete
+  uint64_t* o_full = bars + 16;             // [tile] the segment's last P V complete
+  uint64_t* o_empty = bars + 18;            // [tile] O_i read from TMEM
+  uint64_t* drain = bars + 20;
+  uint64_t* k_full = bars + 21;             // [KS] unpacked
+  uint64_t* k_empty = k_full + KS;          // [KS] read by the last S
+  uint64_t* v_full = k_empty + KS;          // [VS]
+  uint64_t* v_empty = v_full + VS;          // [VS]
+  uint64_t* r_full = v_empty + VS;          // [RS] copied
+  uint64_t* r_empty = r_full + RS;          // [RS] unpacked
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(r_empty + RS);
+  KvmWalk* start = reinterpret_cast<KvmWalk*>(smem + Cfg::BAR_OFFSET + 384);
+
+  const KvBatch& kb = a.kb;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Watchdog wd{&g_kv_wait, a.timeout_ns};
+  kv_launch_dependents();
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 32);
+      mbar_init(&q_empty[i], 1);
+      mbar_init(&o_full[i], 1);
+      mbar_init(&o_empty[i], 128);
+      for (int sl = 0; sl < 2; ++sl) {
+        mbar_init(&s_full[2 * i + sl], 1);
+        mbar_init(&p_full[2 * i + sl], 128);
+        mbar_init(&pv_done[2 * i + sl], 1);
+      }
+    }
+    mbar_init(drain, 2);
+    for (int i = 0; i < KS; ++i) {
+      mbar_init(&k_full[i], 4);
+      mbar_init(&k_empty[i], 1);
+    }
+    for (int i = 0; i < VS; ++i) {
+      mbar_init(&v_full[i], 4);
+      mbar_init(&v_empty[i], 1);
+    }
+    for (int i = 0; i < RS; ++i) {
+      mbar_init(&r_full[i], 1);
+      mbar_init(&r_empty[i], Cfg::UNPACK_WARPS);
+    }
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  if (warp == 2) {
+    const long long total = kvm_total(a, ROWS, lane);
+    const long long active = min(static_cast<long long>(a.workers), total);
+    KvmWalk w{KvmPlace{0, 0, 0, 0}, 0};
+    if (blockIdx.x < active) {
+      const long long x = kv_range_begin(blockIdx.x, total, active);
+      long long begin;
+      int steps;
+      w.p = kvm_find(a, ROWS, x, lane, &begin, &steps);
+      w.left = kv_range_begin(blockIdx.x + 1, total, active) - x;
+    }
+    if (lane == 0) *start = w;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  KvmWalk walk = *start;
+  KvmSegment sg;
+
+  if (warp < 4) {
+    regs_dec<Cfg::REGS_LOW>();
+    if (warp == 0) {
+      // ---------------------------------------------------------- pages
+      const int ps = 1 << kb.page_shift;
+      const int chunk = min(KVM_TK, ps);  // keys of a copy
+      const uint32_t bytes = static_cast<uint32_t>(chunk * RB);
+      int cnt = 0, ids = 0, ids_base = 0;
+      bool ok = true;
+      while (ok && kvm_next(a, ROWS, walk, sg)) {
+        ids_base = -64;  // page numbers of another sequence
+        for (int n = sg.n0; n < sg.n1; ++n, ++cnt) {
+          const int rs = cnt % RS;
+          const int key0 = n * KVM_TK;
+          const int valid = min(KVM_TK, sg.s.len - key0);
+          const int copies = valid <= 0 ? 0 : (valid + chunk - 1) / chunk;
+          const int first = key0 >> kb.page_shift;
+          if (copies > 0 && first + copies > ids_base + 32) {
+            ids_base = first;
+            const int i = first + lane;
+            ids = 0;
+            if (i < kb.pages_per_seq && (i << kb.page_shift) < sg.s.len) {
+              ids = __ldg(kb.table + static_cast<long long>(sg.b) * kb.pages_per_seq + i);
+              if (ids < 0 || ids >= kb.pages) {
+                kv_note(KV_DATA_PAGE);
+                ids = 0;  // read in place of the page outside the pool
+              }
+            }
+          }
+          const int mine = lane >> 1, kv = lane & 1;  // lanes 0 .. 2 copies - 1 issue one copy each
+          const int page = __shfl_sync(0xffffffffu, ids, (first - ids_base + min(mine, max(0, copies - 1))) & 31);
+          ok = cnt < RS || mbar_wait(&r_empty[rs], (cnt / RS - 1) & 1, wd, SITE_KVM_RAW);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          if (lane == 0) {
+            if (copies > 0)
+              mbar_arrive_expect_tx(&r_full[rs], bytes * 2 * copies);
+            else
+              mbar_arrive(&r_full[rs]);
+          }
+          __syncwarp();
+          if (mine < copies) {
+            const uint8_t* src = a.cache + page * kb.page_bytes +
+                                 (static_cast<long long>((sg.h * 2 + kv) << kb.page_shift) + (key0 & (ps - 1))) * RB;
+            bulk_load(sR + rs * Cfg::RAW_BYTES + (kv * KVM_TK + mine * chunk) * RB, src, bytes, &r_full[rs]);
+          }
+        }
+      }
+      // The last copies land before the CTA ends.
+      for (int t = max(0, cnt - RS); t < cnt; ++t) mbar_wait(&r_full[t % RS], (t / RS) & 1, wd, SITE_KVM_DRAIN);
+    } else if (warp == 3) {
+      // ---------------------------------------------------------- rows of Q
+      int ul = 0;
+      bool ok = true;
+      while (ok && kvm_next(a, ROWS, walk, sg)) {
+        for (int i = 0; i < QT && ok; ++i) {
+          ok = ul == 0 || mbar_wait(&q_empty[i], (ul - 1) & 1, wd, SITE_KVM_Q);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          const int rows = sg.s.n * a.group;
+          constexpr int CH = D / 8;  // 16-byte chunks of a row
+          for (int j = lane; j < 128 * CH; j += 32) {
+            const int r = j / CH, ch = j % CH;
+            const int row = (sg.rb * QT + i) * 128 + r;
+            const uint32_t dst = smem_u32(sQ + i * QB + (ch >> 3) * 16384 + r * 128 + (((ch & 7) ^ (r & 7)) * 16));
+            const bool have = row < rows;
+            const int tok = have ? row / a.group : 0, hd = have ? row % a.group : 0;
+            const __half* src = a.Q + (sg.s.first + tok) * a.q_stride +
+                                static_cast<long long>(sg.h * a.group + hd) * D + ch * 8;
+            const uint32_t n = have ? 16u : 0u;  // 0: filled with zeros
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+          }
+          asm volatile("cp.async.wait_all;" ::: "memory");
+          fence_proxy_async_smem();
+          mbar_arrive(&q_full[i]);
+        }
+        ++ul;
+      }
+    } else if (elect_one()) {
+      // ---------------------------------------------------------- MMA issuers
+      const uint64_t q_desc0 = sw128_desc(smem_u32(sQ), 16, 1024);
+      const uint64_t k_desc0 = sw128_desc(smem_u32(sK), 16, 1024);
+      const uint64_t v_desc0 = sw128_desc(smem_u32(sV), KVM_TK * 128, 1024);
+      bool ok = true;
+      int g = 0;  // steps across segments
+      for (int ul = 0; ok && kvm_next(a, ROWS, walk, sg); ++ul) {
+        for (int n = sg.n0; n < sg.n1 && ok; ++n, ++g) {
+          const int sl = g & 1;
+          if (warp == 1) {
+            const int ks = g % KS;
+            ok = mbar_wait(&k_full[ks], (g / KS) & 1, wd, SITE_KVM_S);
+            for (int i = 0; i < QT && ok; ++i) {
+              if (n == sg.n0) ok = mbar_wait(&q_full[i], ul & 1, wd, SITE_KVM_S);
+              if (ok && g >= 2) ok = mbar_wait(&pv_done[2 * i + sl], ((g - 2) >> 1) & 1, wd, SITE_KVM_S);
+              if (!ok) break;
+              tc_fence_after();
+              const uint64_t qd = q_desc0 + static_cast<uint32_t>(i * (QB >> 4));
+              const uint64_t kd = k_desc0 + static_cast<uint32_t>((ks * TB) >> 4);
+              const uint32_t d_tmem = tmem_base + i * 128 + sl * KVM_TK;
+#pragma unroll
+              for (int kk = 0; kk < D / 16; ++kk)
+                umma_f16_ss(d_tmem, qd + (((kk >> 2) * 16384 + (kk & 3) * 32) >> 4),
+                            kd + (((kk >> 2) * (KVM_TK * 128) + (kk & 3) * 32) >> 4), IDESC_S, kk > 0 ? 1u : 0u);
+              umma_commit(&s_full[2 * i + sl]);
+              if (n == sg.n1 - 1) umma_commit(&q_empty[i]);
+              if (i == QT - 1) umma_commit(&k_empty[ks]);
+            }
+          } else {
+            const int vs = g % VS;
+            for (int i = 0; i < QT && ok; ++i) {
+              ok = mbar_wait(&p_full[2 * i + sl], (g >> 1) & 1, wd, SITE_KVM_PV);
+              if (ok && i == 0) ok = mbar_wait(&v_full[vs], (g / VS) & 1, wd, SITE_KVM_PV);
+              if (ok && n == sg.n0 && ul > 0) ok = mbar_wait(&o_empty[i], (ul - 1) & 1, wd, SITE_KVM_PV);
+              if (!ok) break;
+              tc_fence_after();
+              const uint64_t vd = v_desc0 + static_cast<uint32_t>((vs * TB) >> 4);
+              const uint32_t d_tmem = tmem_base + 256 + i * D;
+              const uint32_t p_tmem = tmem_base + i * 128 + sl * KVM_TK;
+#pragma unroll
+              for (int kk = 0; kk < KVM_TK / 16; ++kk)
+                umma_f16_ts(d_tmem, p_tmem + kk * 8, vd + static_cast<uint32_t>(kk * (2048 >> 4)), IDESC_O,
+                            (n > sg.n0 || kk > 0) ? 1u : 0u);
+              umma_commit(&pv_done[2 * i + sl]);
+              if (n == sg.n1 - 1) umma_commit(&o_full[i]);
+              if (i == QT - 1) umma_commit(&v_empty[vs]);
+            }
+          }
+        }
+      }
+      umma_commit(drain);
+      mbar_wait(drain, 0, wd, SITE_KVM_DRAIN);
+    }
+  } else if (warp < 4 + 4 * QT) {
+    // ---------------------------------------------------------- softmax
+    regs_inc<Cfg::REGS_SOFTMAX>();
+    const int ti = (warp - 4) >> 2;
+    const int q = warp & 3;  // TMEM lane quadrant
+    const int r = q * 32 + lane;
+    const uint32_t lane_off = static_cast<uint32_t>(q * 32) << 16;
+    const uint32_t tS = tmem_base + ti * 128 + lane_off;
+    const uint32_t tO = tmem_base + 256 + ti * D + lane_off;
+    const float sl2 = a.scale_log2;
+    bool ok = true;
+    int g = 0;
+    for (int ul = 0; ok && kvm_next(a, ROWS, walk, sg); ++ul) {
+      const int row = sg.rb * ROWS + ti * 128 + r;
+      const bool have = row < sg.s.n * a.group;
+      const int tok = have ? row / a.group : 0;
+      const int limit = have ? kv_limit(sg.s, tok, a.causal) : sg.s.len;
+      float m = KV_NO_MAX;  // running max, log2 domain (possibly stale by < 8)
+      float l = 0.f;
+      for (int n = sg.n0; n < sg.n1; ++n, ++g) {
+        const int sl = g & 1;
+        const uint32_t tSl = tS + sl * KVM_TK;
+        ok = __all_sync(0xffffffffu, mbar_wait(&s_full[2 * ti + sl], (g >> 1) & 1, wd, SITE_KVM_SOFTMAX));
+        if (!ok) break;
+        tc_fence_after();
+        float x[64];
+        {
+          uint32_t v0[32], v1[32];
+          tmem_ld_32x32b_x32(tSl + 0, v0);
+          tmem_ld_32x32b_x32(tSl + 32, v1);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            x[i] = __uint_as_float(v0[i]);
+            x[32 + i] = __uint_as_float(v1[i]);
+          }
+        }
+        const int valid = limit - n * KVM_TK;
+        if (__any_sync(0xffffffffu, valid < KVM_TK)) {
+#pragma unroll
+          for (int i = 0; i < 64; ++i)
+            if (i >= valid) x[i] = -INFINITY;
+        }
+        float part;
+        if (n == sg.n0) {
+          m = fmaxf(att_row_max64(x) * sl2, KV_NO_MAX);
+          part = att_exp_store64<EMU>(x, sl2, m, tSl);
+        } else {
+          // Exponentials against the running max, the new row max alongside.
+          part = att_exp_store64<EMU>(x, sl2, m, tSl);
+          const float mx = att_row_max64(x) * sl2;
+          const bool grow = (mx > m + 8.0f);
+          if (__any_sync(0xffffffffu, grow)) {
+            // Rescale this warp's O rows once the previous step's P V (the only
+            // MMA that may still write them) is done, and redo the exponentials.
+            ok = __all_sync(0xffffffffu,
+                            mbar_wait(&pv_done[2 * ti + (sl ^ 1)], ((g - 1) >> 1) & 1, wd, SITE_KVM_SOFTMAX));
+            if (!ok) break;
+            tc_fence_after();
+            const float m_new = grow ? mx : m;
+            const float factor = grow ? ex2_approx(m - m_new) : 1.0f;
+#pragma unroll 1
+            for (int c = 0; c < D / 16; ++c) {
+              uint32_t v[16];
+              tmem_ld_32x32b_x16(tO + c * 16, v);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * factor);
+              tmem_st_32x32b_x16(tO + c * 16, v);
+            }
+            l *= factor;
+            m = m_new;
+            tmem_st_wait();
+            part = att_exp_store64<EMU>(x, sl2, m, tSl);
+          }
+        }
+        l += part;
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(&p_full[2 * ti + sl]);
+      }
+      if (!ok) break;
+      // The segment's O: out, or into a partial if the unit goes on elsewhere.
+      ok = __all_sync(0xffffffffu, mbar_wait(&o_full[ti], ul & 1, wd, SITE_KVM_SOFTMAX));
+      if (!ok) break;
+      tc_fence_after();
+      const bool whole = sg.n0 == 0 && sg.n1 == sg.steps;
+      const float inv_l = l > 0.f ? 1.0f / l : 0.f;
+      const long long token = sg.s.first + tok;
+      const int head = sg.h * a.group + (have ? row % a.group : 0);
+      __half* out = a.O + token * a.o_stride + static_cast<long long>(head) * D;
+      float* part = a.partials + kvm_slot<D, ROWS>(2ll * blockIdx.x + (sg.n0 == 0 ? 1 : 0));
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+        __syncwarp();
+        tmem_ld_32x32b_x32(tO + c * 32, o);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 32; i += 8) {
+          if (!have) break;
+          // 4-bit values lie as elements 0 4 1 5 2 6 3 7 in each 8 columns.
+          float e[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            e[k] = __uint_as_float(o[i + (BITS == 4 ? (k < 4 ? 2 * k : 2 * (k - 4) + 1) : k)]);
+          if (whole) {
+            uint4 pk;
+            pk.x = pack_half2(e[0] * inv_l, e[1] * inv_l);
+            pk.y = pack_half2(e[2] * inv_l, e[3] * inv_l);
+            pk.z = pack_half2(e[4] * inv_l, e[5] * inv_l);
+            pk.w = pack_half2(e[6] * inv_l, e[7] * inv_l);
+            *reinterpret_cast<uint4*>(out + c * 32 + i) = pk;
+          } else {
+            float4* dst = reinterpret_cast<float4*>(part) + (c * 8 + i / 4) * ROWS + ti * 128 + r;
+            dst[0] = make_float4(e[0], e[1], e[2], e[3]);
+            dst[ROWS] = make_float4(e[4], e[5], e[6], e[7]);
+          }
+        }
+      }
+      __syncwarp();
+      tc_fence_before();
+      mbar_arrive(&o_empty[ti]);
+      if (have) {
+        if (whole) {
+          if (a.lse != nullptr) a.lse[token * a.heads_q + head] = (m + log2f(l)) * 0.6931471805599453f;
+        } else {
+          part[ROWS * D + ti * 128 + r] = m;
+          part[ROWS * D + ROWS + ti * 128 + r] = l;
+        }
+      }
+    }
+  } else {
+    // ---------------------------------------------------------- codes to fp16
+    regs_dec<Cfg::REGS_UNPACK>();
+    constexpr int GR = D / KV_GROUP;          // groups of a row
+    constexpr int RW = 32 / GR;               // rows of a warp at a time
+    constexpr int PASSES = KVM_TK / (RW * 4);
+    const int uw = (warp - (16 - Cfg::UNPACK_WARPS)) & 3;
+    const int kv0 = QT == 1 ? (warp - (16 - Cfg::UNPACK_WARPS)) >> 2 : 0, kv1 = QT == 1 ? kv0 : 1;
+    // Eight lanes take eight rows and one group: the row pitches (80, 144, 40,
+    // 72 bytes) and the swizzle then put their accesses on different banks.
+    const int sub = (lane & 7) + 8 * (lane / (8 * GR));
+    const int gr = (lane >> 3) % GR;
+    const uint32_t k1024 = __shfl_sync(0xffffffffu, a.k1024, 0);
+    int g = 0;
+    bool ok = true;
+    while (ok && kvm_next(a, ROWS, walk, sg)) {
+      for (int n = sg.n0; n < sg.n1 && ok; ++n, ++g) {
+        const int rs = g % RS, st[2] = {g % KS, g % VS};
+        ok = mbar_wait(&r_full[rs], (g / RS) & 1, wd, SITE_KVM_UNPACK);
+        const uint8_t* raw = sR + rs * Cfg::RAW_BYTES;
+        const int valid = sg.s.len - n * KVM_TK;
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          if (kv < kv0 || kv > kv1) continue;
+          const int depth = kv == 0 ? KS : VS;
+          if (ok && g >= depth)
+            ok = mbar_wait(kv == 0 ? &k_empty[st[0]] : &v_empty[st[1]], (g / depth - 1) & 1, wd, SITE_KVM_UNPACK);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          uint8_t* tile = kv == 0 ? sK + st[0] * TB : sV + st[1] * TB;
+#pragma unroll
+          for (int p = 0; p < PASSES; ++p) {
+            const int row = (p * 4 + uw) * RW + sub;
+            const uint8_t* src = raw + (kv * KVM_TK + row) * RB;
+            __half2 par = *reinterpret_cast<const __half2*>(src + Row::CODES + gr * 4);
+            // Rows behind the sequence hold anything; their values count as 0.
+            if (row >= valid) par = __float2half2_rn(0.f);
+            const __half2 s2 = __low2half2(par), z2 = __high2half2(par);
+            constexpr int WORDS = KV_GROUP * BITS / 32;
+            uint32_t w[WORDS];
+            if constexpr (RB % 16 == 0) {
+#pragma unroll
+              for (int i = 0; i < WORDS; i += 4) {
+                const uint4 v = *reinterpret_cast<const uint4*>(src + gr * (KV_GROUP * BITS / 8) + 4 * i);
+                w[i] = v.x;
+                w[i + 1] = v.y;
+                w[i + 2] = v.z;
+                w[i + 3] = v.w;
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < WORDS; i += 2) {
+                const uint2 v = *reinterpret_cast<const uint2*>(src + gr * (KV_GROUP * BITS / 8) + 4 * i);
+                w[i] = v.x;
+                w[i + 1] = v.y;
+              }
+            }
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {  // 8 elements, 16 bytes
+              uint4 out;
+              if constexpr (BITS == 4) {
+                __half2 h[4];
+                kv_codes4(w[c], h, k1024);
+                const uint32_t p0 = as_u32(__hfma2(h[0], s2, z2)), p1 = as_u32(__hfma2(h[1], s2, z2)),
+                               p2 = as_u32(__hfma2(h[2], s2, z2)), p3 = as_u32(__hfma2(h[3], s2, z2));
+                // K in the order of Q's elements; V as it comes (columns of O).
+                if (kv == 0)
+                  out = make_uint4(__byte_perm(p0, p1, 0x5410), __byte_perm(p2, p3, 0x5410),
+                                   __byte_perm(p0, p1, 0x7632), __byte_perm(p2, p3, 0x7632));
+                else
+                  out = make_uint4(p0, p1, p2, p3);
+              } else {
+                out.x = as_u32(__hfma2(kv_codes8(w[2 * c], 0x4140), s2, z2));
+                out.y = as_u32(__hfma2(kv_codes8(w[2 * c], 0x4342), s2, z2));
+                out.z = as_u32(__hfma2(kv_codes8(w[2 * c + 1], 0x4140), s2, z2));
+                out.w = as_u32(__hfma2(kv_codes8(w[2 * c + 1], 0x4342), s2, z2));
+              }
+              const int ch = gr * 4 + c;
+              *reinterpret_cast<uint4*>(tile + (ch >> 3) * (KVM_TK * 128) + row * 128 +
+                                        (((ch & 7) ^ (row & 7)) * 16)) = out;
+            }
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(kv == 0 ? &k_full[st[0]] : &v_full[st[1]]);
+        }
+        if (ok && lane == 0) mbar_arrive(&r_empty[rs]);
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+// Joins the partials of units that several CTAs share. Block (w, c) looks at
+// the border between workers w and w + 1: if it lies in a unit that worker w
+// began, the block joins 32 rows of that unit. Lane = row; a warp takes D / 8
+// elements of them.
+template <int D, int ROWS>
+__global__ void __launch_bounds__(256) kv_attention_many_join_kernel(const __grid_constant__ KvAttnArgs a) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int G4 = D / 32;  // groups of 4 elements a warp
+  const long long total = kvm_total(a, ROWS, lane);
+  const long long active = min(static_cast<long long>(a.workers), total);
+  const long long w = blockIdx.x;
+  bool mine = w + 1 < active;
+  KvmPlace p{};
+  long long begin = 0;
+  int steps = 0;
+  if (mine) {
+    const long long x = kv_range_begin(w + 1, total, active);
+    p = kvm_find(a, ROWS, x, lane, &begin, &steps);
+    // In the middle of a unit, and the first border in it.
+    mine = p.n > 0 && begin >= kv_range_begin(w, total, active) && p.b < a.kb.sequences;
+  }
+  kv_wait_for_previous();  // in every block: what follows this kernel also follows the one before it
+  if (!mine) return;
+  const int last = static_cast<int>(kv_worker_of(begin + steps - 1, total, active));
+  const KvSequence s = kvm_sequence(a, p.b);
+  const int local = blockIdx.y * 32 + lane;
+  const int row = p.rb * ROWS + local;
+  if (row >= s.n * a.group) return;
+  float m = KV_NO_MAX, l = 0.f, acc[G4][4];
+#pragma unroll
+  for (int i = 0; i < G4; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[i][e] = 0.f;
+  for (int k = static_cast<int>(w); k <= last; ++k) {
+    const float* part = a.partials + kvm_slot<D, ROWS>(2ll * k + (k == w ? 1 : 0));
+    const float pm = __ldcg(part + ROWS * D + local), pl = __ldcg(part + ROWS * D + ROWS + local);
+    const float m_new = fmaxf(m, pm), f = kv_ex2(m - m_new), fp = kv_ex2(pm - m_new);
+    m = m_new;
+    l = l * f + pl * fp;
+#pragma unroll
+    for (int i = 0; i < G4; ++i) {
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(part) + (warp * G4 + i) * ROWS + local);
+      acc[i][0] = acc[i][0] * f + v.x * fp;
+      acc[i][1] = acc[i][1] * f + v.y * fp;
+      acc[i][2] = acc[i][2] * f + v.z * fp;
+      acc[i][3] = acc[i][3] * f + v.w * fp;
+    }
+  }
+  const long long token = s.first + row / a.group;
+  const int head = p.h * a.group + row % a.group;
+  const float inv = l > 0.f ? 1.0f / l : 0.f;
+  __half* out = a.O + token * a.o_stride + static_cast<long long>(head) * D + warp * (D / 8);
+#pragma unroll
+  for (int i = 0; i < G4; ++i)
+    *reinterpret_cast<uint2*>(out + 4 * i) = make_uint2(pack_half2(acc[i][0] * inv, acc[i][1] * inv),
+                                                        pack_half2(acc[i][2] * inv, acc[i][3] * inv));
+  if (a.lse != nullptr && warp == 0) a.lse[token * a.heads_q + head] = (m + log2f(l)) * 0.6931471805599453f;
+}
+
+}  // namespace mm4

@@ -7,7 +7,7 @@
 #include <new>
 
 #include "kv_attention_few_sm100.cuh"
-#include "kv_attention_sm100.cuh"
+#include "kv_attention_many_sm100.cuh"
 #include "kv_cache_sm100.cuh"
 #include "mm4_internal.h"
 
@@ -118,7 +118,7 @@ mm4_status launch_io(const mm4_kv_cache_plan* p, KvIoArgs& a, bool write, cudaSt
 // Which kernel attention over a batch runs, from its sizes alone (the lengths
 // lie on the device).
 struct Form {
-  enum Kind { FEW8, FEW16, ROWS } kind;
+  enum Kind { FEW8, FEW16, MANY128, MANY256 } kind;
   bool team;         // FEW: whole units to a CTA, one launch
   size_t workspace;
   const char* name;
@@ -135,8 +135,14 @@ size_t few_workspace() {
 Form attention_form(const mm4_kv_cache_plan* p, const mm4_kv_cache_batch* b) {
   const int group = p->d.heads_q / p->d.heads_kv;
   const long long rows = static_cast<long long>(b->max_new) * group;
-  Form f{Form::ROWS, false, 0, "kv_attention_row"};
-  if (rows > 16) return f;
+  Form f{};
+  if (rows > 16) {
+    f.kind = rows <= 128 ? Form::MANY128 : Form::MANY256;
+    const int tile = rows <= 128 ? 128 : 256;
+    f.workspace = sizeof(float) * 2 * kMaxCtas * tile * (p->d.head_dim + 2);
+    f.name = rows <= 128 ? "kv_attention_many<128 rows>" : "kv_attention_many<256 rows>";
+    return f;
+  }
   const long long room = static_cast<long long>(b->pages_per_sequence) << p->page_shift;
   const bool eight = rows <= 8;
   f.kind = eight ? Form::FEW8 : Form::FEW16;
@@ -158,13 +164,10 @@ Form attention_form(const mm4_kv_cache_plan* p, const mm4_kv_cache_batch* b) {
   return f;
 }
 
-// The join of partials, allowed to start while the kernel before it ends.
-template <int D, int ROWS, int TK>
-mm4_status launch_join(const KvAttnArgs& a, cudaStream_t st) {
-  const long long units = static_cast<long long>(a.kb.sequences) * a.kb.heads_kv;
-  if (units > 0x7fffffffLL) return fail(MM4_ERR_UNSUPPORTED, "too many sequences for one launch");
+// Launches a join of partials, allowed to start while the kernel before it ends.
+mm4_status launch_join(void (*kernel)(KvAttnArgs), dim3 grid, const KvAttnArgs& a, cudaStream_t st) {
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(units), (ROWS + 7) / 8);
+  cfg.gridDim = grid;
   cfg.blockDim = dim3(256);
   cfg.stream = st;
   cudaLaunchAttribute attr{};
@@ -172,8 +175,8 @@ mm4_status launch_join(const KvAttnArgs& a, cudaStream_t st) {
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kv_attention_join_kernel<D, ROWS, TK>, a);
-  if (e != cudaSuccess) return cuda_fail(e, "kv_attention_join_kernel launch");
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
+  if (e != cudaSuccess) return cuda_fail(e, "launch of the join of partials");
   return MM4_OK;
 }
 
@@ -196,7 +199,33 @@ mm4_status launch_few(KvAttnArgs& a, bool team, int sms, cudaStream_t st) {
   kv_attention_few_kernel<D, BITS, NT, false><<<sms, Cfg::THREADS, Cfg::SMEM_BYTES, st>>>(a);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "kv_attention_few_kernel launch");
-  return launch_join<D, Cfg::ROWS, KVF_TK>(a, st);
+  const long long units = static_cast<long long>(a.kb.sequences) * a.kb.heads_kv;
+  return launch_join(kv_attention_join_kernel<D, Cfg::ROWS, KVF_TK>, dim3(static_cast<unsigned>(units), NT), a, st);
+}
+
+template <int D, int BITS, int QT>
+mm4_status launch_many(KvAttnArgs& a, int sms, cudaStream_t st) {
+  using Cfg = KvMany<D, BITS, QT>;
+  const void* kern = reinterpret_cast<const void*>(kv_attention_many_kernel<D, BITS, QT>);
+  mm4_status rc = ensure_smem_attr(kern, Cfg::SMEM_BYTES);
+  if (rc != MM4_OK) return rc;
+  {
+    // The kernel moves registers between warpgroups (setmaxnreg); that only
+    // completes if the launch allocates enough of them.
+    static const int launch_regs = [&] {
+      cudaFuncAttributes fa;
+      return cudaFuncGetAttributes(&fa, kern) == cudaSuccess ? fa.numRegs : -1;
+    }();
+    if (launch_regs < Cfg::REGS_NEEDED)
+      return fail(MM4_ERR_UNSUPPORTED, "attention kernel built with %d registers per thread, needs %d", launch_regs,
+                  Cfg::REGS_NEEDED);
+  }
+  a.workers = sms;
+  kv_attention_many_kernel<D, BITS, QT><<<sms, KVM_THREADS, Cfg::SMEM_BYTES, st>>>(a);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, "kv_attention_many_kernel launch");
+  if (sms < 2) return MM4_OK;
+  return launch_join(kv_attention_many_join_kernel<D, Cfg::ROWS>, dim3(sms - 1, Cfg::ROWS / 32), a, st);
 }
 
 }  // namespace
@@ -324,6 +353,9 @@ mm4_status mm4_kv_cache_attention(const mm4_kv_cache_plan* p, const mm4_kv_cache
   if ((rc = check_rows("O", O, o_stride, width)) != MM4_OK) return rc;
   if ((rc = check_cache(cache)) != MM4_OK) return rc;
   if ((reinterpret_cast<uintptr_t>(lse) & 3u) != 0) return fail(MM4_ERR_INVALID, "lse must be 4-byte aligned");
+  if (static_cast<long long>(b->max_new) * (p->d.heads_q / p->d.heads_kv) > (1 << 28) ||
+      static_cast<long long>(b->sequences) * p->d.heads_kv > 0x7fffffffLL)
+    return fail(MM4_ERR_UNSUPPORTED, "too many rows or sequences for one launch");
   const Form form = attention_form(p, b);
   if (form.workspace > 0) {
     if (!workspace || workspace_bytes < form.workspace)
@@ -349,19 +381,11 @@ mm4_status mm4_kv_cache_attention(const mm4_kv_cache_plan* p, const mm4_kv_cache
   a.timeout_ns = wait_timeout_ns();
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int sms = std::min(info.sm_count, kMaxCtas);
-  if (form.kind == Form::ROWS) {
-    const long long blocks = (static_cast<long long>(b->tokens) * p->d.heads_q + 3) / 4;
-    if (blocks > 0x7fffffffLL) return fail(MM4_ERR_UNSUPPORTED, "too many rows for one launch");
-    return by_row(p->d, [&](auto, auto D, auto B) -> mm4_status {
-      kv_attention_row_kernel<D.value, B.value><<<static_cast<unsigned>(blocks), 128, 0, st>>>(a);
-      cudaError_t e = cudaGetLastError();
-      if (e != cudaSuccess) return cuda_fail(e, "kv_attention_row_kernel launch");
-      return MM4_OK;
-    });
-  }
   return by_row(p->d, [&](auto, auto D, auto B) -> mm4_status {
     if (form.kind == Form::FEW8) return launch_few<D.value, B.value, 1>(a, form.team, sms, st);
-    return launch_few<D.value, B.value, 2>(a, form.team, sms, st);
+    if (form.kind == Form::FEW16) return launch_few<D.value, B.value, 2>(a, form.team, sms, st);
+    if (form.kind == Form::MANY128) return launch_many<D.value, B.value, 1>(a, sms, st);
+    return launch_many<D.value, B.value, 2>(a, sms, st);
   });
 }
 
