@@ -15,9 +15,11 @@
 //   warp 1        TMEM allocation; one lane issues S_i(g) = Q_i K(g)^T (M = 128,
 //                 N = 64) into slot g % 2 of row tile i.
 //   warp 2        one lane issues O_i += P_i(g) V(g) (P from TMEM).
-//   warp 3        copies the next unit's rows of Q when the last S has read them.
+//   warp 3        finds the CTA's range.
 //   QT x 4 warps  softmax, one row a thread: P = 2^(S scale log2 e - m), rescaling
-//                 O only when the maximum grew by more than 2^8; results out.
+//                 O only when the maximum grew by more than 2^8; results out. A
+//                 thread also copies its row of the next unit's Q, as soon as it has
+//                 the last scores of the unit, so the copy overlaps the results.
 //   the others    codes to fp16: a lane takes 32 elements (one scale and zero).
 // TMEM: two 64-column S slots for each row tile, then O_i (D columns each). Steps
 // of 64 keys are counted across a CTA's units (g), which fixes slots and
@@ -46,8 +48,8 @@ struct KvMany {
   static constexpr int UNPACK_WARPS = 12 - 4 * QT;
   // Registers: 128 threads each of warps 0-3, the softmax warps and the
   // unpacking warps; the sum must not exceed what the block is launched with.
-  static constexpr int REGS_LOW = 64;
-  static constexpr int REGS_SOFTMAX = QT == 2 ? 176 : 192;
+  static constexpr int REGS_LOW = 96;
+  static constexpr int REGS_SOFTMAX = 160;
   static constexpr int REGS_UNPACK = QT == 2 ? 96 : 128;
   static constexpr int REGS_NEEDED = (REGS_LOW + QT * REGS_SOFTMAX + (3 - QT) * REGS_UNPACK) / 4;
   static_assert(REGS_NEEDED <= 128, "register split");
@@ -56,7 +58,6 @@ struct KvMany {
 
 enum : int {
   SITE_KVM_RAW = 120,
-  SITE_KVM_Q = 121,
   SITE_KVM_S = 122,
   SITE_KVM_PV = 123,
   SITE_KVM_SOFTMAX = 124,
@@ -85,13 +86,31 @@ __device__ __forceinline__ KvSequence kvm_sequence(const KvAttnArgs& a, int b) {
   }
   return s;
 }
-__device__ __forceinline__ int kvm_sequence_steps(const KvAttnArgs& a, int b, int rows) {
+// Steps of a sequence for one head. The lanes of a warp share either the
+// sequences or, where those are fewer than the row blocks that a sequence may
+// have, the blocks of one sequence after the other.
+__device__ __forceinline__ bool kvm_by_block(const KvAttnArgs& a, int rows) {
+  return a.kb.sequences < kvm_blocks(KvSequence{0, 0, a.kb.max_new}, a.group, rows);
+}
+__device__ __forceinline__ long long kvm_warp_sum(long long x) {
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) x += __shfl_xor_sync(0xffffffffu, x, s);
+  return x;
+}
+__device__ __forceinline__ int kvm_lane_steps(const KvAttnArgs& a, int b, int rows) {  // lanes: sequences
   if (b >= a.kb.sequences) return 0;
   const KvSequence s = kvm_sequence(a, b);
   const int blocks = kvm_blocks(s, a.group, rows);
   int sum = 0;
   for (int rb = 0; rb < blocks; ++rb) sum += kvm_steps(s, rb, a, rows);
   return sum;
+}
+__device__ __forceinline__ long long kvm_block_steps(const KvAttnArgs& a, const KvSequence& s, int rows,
+                                                     int lane) {  // lanes: blocks
+  const int blocks = kvm_blocks(s, a.group, rows);
+  long long sum = 0;
+  for (int rb = lane; rb < blocks; rb += 32) sum += kvm_steps(s, rb, a, rows);
+  return kvm_warp_sum(sum);
 }
 
 // A place on the line of all steps: sequences, their row blocks, heads, steps.
@@ -100,47 +119,76 @@ struct KvmPlace {
 };
 __device__ __forceinline__ long long kvm_total(const KvAttnArgs& a, int rows, int lane) {
   long long sum = 0;
-  for (int b = lane; b < a.kb.sequences; b += 32) sum += kvm_sequence_steps(a, b, rows);
-#pragma unroll
-  for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
-  return sum * a.kb.heads_kv;
+  if (kvm_by_block(a, rows)) {
+    for (int b = 0; b < a.kb.sequences; ++b) {
+      const KvSequence s = kvm_sequence(a, b);
+      const int blocks = kvm_blocks(s, a.group, rows);
+      for (int rb = lane; rb < blocks; rb += 32) sum += kvm_steps(s, rb, a, rows);
+    }
+  } else {
+    for (int b = lane; b < a.kb.sequences; b += 32) sum += kvm_lane_steps(a, b, rows);
+  }
+  return kvm_warp_sum(sum) * a.kb.heads_kv;
 }
-// Place x (by one warp); also where its unit begins.
+// Place x (by one warp); also where its unit begins and how many steps it has.
 __device__ __forceinline__ KvmPlace kvm_find(const KvAttnArgs& a, int rows, long long x, int lane,
                                              long long* unit_begin, int* unit_steps) {
   const int heads = a.kb.heads_kv;
-  long long done = 0;  // of whole sequences, for one head
-  for (int b0 = 0; b0 < a.kb.sequences; b0 += 32) {
-    const int t = kvm_sequence_steps(a, b0 + lane, rows);
-    long long inc = t;
-#pragma unroll
-    for (int s = 1; s < 32; s <<= 1) {
-      const long long up = __shfl_up_sync(0xffffffffu, inc, s);
-      if (lane >= s) inc += up;
+  KvmPlace p{0, 0, 0, 0};
+  long long at = 0;  // where sequence p.b begins
+  if (kvm_by_block(a, rows)) {
+    for (; p.b < a.kb.sequences; ++p.b) {
+      const long long all = kvm_block_steps(a, kvm_sequence(a, p.b), rows, lane) * heads;
+      if (at + all > x) break;
+      at += all;
     }
-    const unsigned over = __ballot_sync(0xffffffffu, (done + inc) * heads > x);
+  } else {
+    for (; p.b < a.kb.sequences; p.b += 32) {
+      const int t = kvm_lane_steps(a, p.b + lane, rows);
+      long long inc = t;
+#pragma unroll
+      for (int s = 1; s < 32; s <<= 1) {
+        const long long up = __shfl_up_sync(0xffffffffu, inc, s);
+        if (lane >= s) inc += up;
+      }
+      const unsigned over = __ballot_sync(0xffffffffu, at + inc * heads > x);
+      if (over != 0) {
+        const int k = __ffs(over) - 1;
+        at += __shfl_sync(0xffffffffu, inc - t, k) * heads;
+        p.b += k;
+        break;
+      }
+      at += __shfl_sync(0xffffffffu, inc, 31) * heads;
+    }
+  }
+  *unit_begin = x;
+  *unit_steps = 1;
+  if (p.b >= a.kb.sequences) return KvmPlace{a.kb.sequences, 0, 0, 0};
+  // The row block: a scan over 32 blocks at a time.
+  const KvSequence s = kvm_sequence(a, p.b);
+  const int blocks = kvm_blocks(s, a.group, rows);
+  for (; p.rb < blocks; p.rb += 32) {
+    const int t = p.rb + lane < blocks ? kvm_steps(s, p.rb + lane, a, rows) : 0;
+    int inc = t;
+#pragma unroll
+    for (int k = 1; k < 32; k <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, inc, k);
+      if (lane >= k) inc += up;
+    }
+    const unsigned over = __ballot_sync(0xffffffffu, at + static_cast<long long>(inc) * heads > x);
     if (over != 0) {
       const int k = __ffs(over) - 1;
-      long long at = (done + __shfl_sync(0xffffffffu, inc - t, k)) * heads;
-      KvmPlace p{b0 + k, 0, 0, 0};
-      const KvSequence s = kvm_sequence(a, p.b);
-      const int blocks = kvm_blocks(s, a.group, rows);
-      for (; p.rb < blocks; ++p.rb) {
-        const long long all = static_cast<long long>(kvm_steps(s, p.rb, a, rows)) * heads;
-        if (at + all > x) break;
-        at += all;
-      }
-      const int steps = kvm_steps(s, p.rb, a, rows);
+      const int steps = __shfl_sync(0xffffffffu, t, k);
+      at += static_cast<long long>(__shfl_sync(0xffffffffu, inc - t, k)) * heads;
+      p.rb += k;
       p.h = static_cast<int>((x - at) / steps);
       p.n = static_cast<int>((x - at) % steps);
       *unit_begin = x - p.n;
       *unit_steps = steps;
       return p;
     }
-    done += __shfl_sync(0xffffffffu, inc, 31);
+    at += static_cast<long long>(__shfl_sync(0xffffffffu, inc, 31)) * heads;
   }
-  *unit_begin = x;
-  *unit_steps = 1;
   return KvmPlace{a.kb.sequences, 0, 0, 0};
 }
 
@@ -207,7 +255,6 @@ __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const
   uint8_t* sR = sV + VS * TB;               // [RS] pages as they lie in the cache: K rows, V rows
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::BAR_OFFSET);
   uint64_t* q_full = bars;                  // [tile] the unit's Q_i in place
-  uint64_t* q_empty = bars + 2;             // [tile] its last S_i complete
   uint64_t* s_full = bars + 4;              // [tile][slot] S_i(g) in TMEM
   uint64_t* p_full = bars + 8;              // [tile][slot] P_i(g) in TMEM, O_i rescaled
   uint64_t* pv_done = bars + 12;            // [tile][slot] O_i += P_i(g) V(g) complete
@@ -230,8 +277,7 @@ __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&q_full[i], 32);
-      mbar_init(&q_empty[i], 1);
+      mbar_init(&q_full[i], 128);
       mbar_init(&o_full[i], 1);
       mbar_init(&o_empty[i], 128);
       for (int sl = 0; sl < 2; ++sl) {
@@ -259,7 +305,7 @@ __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
-  if (warp == 2) {
+  if (warp == 3) {
     const long long total = kvm_total(a, ROWS, lane);
     const long long active = min(static_cast<long long>(a.workers), total);
     KvmWalk w{KvmPlace{0, 0, 0, 0}, 0};
@@ -329,49 +375,24 @@ __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const
       }
       // The last copies land before the CTA ends.
       for (int t = max(0, cnt - RS); t < cnt; ++t) mbar_wait(&r_full[t % RS], (t / RS) & 1, wd, SITE_KVM_DRAIN);
-    } else if (warp == 3) {
-      // ---------------------------------------------------------- rows of Q
-      int ul = 0;
-      bool ok = true;
-      while (ok && kvm_next(a, ROWS, walk, sg)) {
-        for (int i = 0; i < QT && ok; ++i) {
-          ok = ul == 0 || mbar_wait(&q_empty[i], (ul - 1) & 1, wd, SITE_KVM_Q);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          const int rows = sg.s.n * a.group;
-          constexpr int CH = D / 8;  // 16-byte chunks of a row
-          for (int j = lane; j < 128 * CH; j += 32) {
-            const int r = j / CH, ch = j % CH;
-            const int row = (sg.rb * QT + i) * 128 + r;
-            const uint32_t dst = smem_u32(sQ + i * QB + (ch >> 3) * 16384 + r * 128 + (((ch & 7) ^ (r & 7)) * 16));
-            const bool have = row < rows;
-            const int tok = have ? row / a.group : 0, hd = have ? row % a.group : 0;
-            const __half* src = a.Q + (sg.s.first + tok) * a.q_stride +
-                                static_cast<long long>(sg.h * a.group + hd) * D + ch * 8;
-            const uint32_t n = have ? 16u : 0u;  // 0: filled with zeros
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-          }
-          asm volatile("cp.async.wait_all;" ::: "memory");
-          fence_proxy_async_smem();
-          mbar_arrive(&q_full[i]);
-        }
-        ++ul;
-      }
-    } else if (elect_one()) {
+    } else if (warp != 3 && elect_one()) {
       // ---------------------------------------------------------- MMA issuers
       const uint64_t q_desc0 = sw128_desc(smem_u32(sQ), 16, 1024);
       const uint64_t k_desc0 = sw128_desc(smem_u32(sK), 16, 1024);
       const uint64_t v_desc0 = sw128_desc(smem_u32(sV), KVM_TK * 128, 1024);
       bool ok = true;
       int g = 0;  // steps across segments
-      for (int ul = 0; ok && kvm_next(a, ROWS, walk, sg); ++ul) {
-        for (int n = sg.n0; n < sg.n1 && ok; ++n, ++g) {
+      bool more = kvm_next(a, ROWS, walk, sg);
+      for (int ul = 0; ok && more; ++ul) {
+        const int n0 = sg.n0, n1 = sg.n1;
+        more = kvm_next(a, ROWS, walk, sg);  // while this segment's first steps are on their way
+        for (int n = n0; n < n1 && ok; ++n, ++g) {
           const int sl = g & 1;
           if (warp == 1) {
             const int ks = g % KS;
             ok = mbar_wait(&k_full[ks], (g / KS) & 1, wd, SITE_KVM_S);
             for (int i = 0; i < QT && ok; ++i) {
-              if (n == sg.n0) ok = mbar_wait(&q_full[i], ul & 1, wd, SITE_KVM_S);
+              if (n == n0) ok = mbar_wait(&q_full[i], ul & 1, wd, SITE_KVM_S);
               if (ok && g >= 2) ok = mbar_wait(&pv_done[2 * i + sl], ((g - 2) >> 1) & 1, wd, SITE_KVM_S);
               if (!ok) break;
               tc_fence_after();
@@ -383,7 +404,6 @@ __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const
                 umma_f16_ss(d_tmem, qd + (((kk >> 2) * 16384 + (kk & 3) * 32) >> 4),
                             kd + (((kk >> 2) * (KVM_TK * 128) + (kk & 3) * 32) >> 4), IDESC_S, kk > 0 ? 1u : 0u);
               umma_commit(&s_full[2 * i + sl]);
-              if (n == sg.n1 - 1) umma_commit(&q_empty[i]);
               if (i == QT - 1) umma_commit(&k_empty[ks]);
             }
           } else {
@@ -391,7 +411,7 @@ __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const
             for (int i = 0; i < QT && ok; ++i) {
               ok = mbar_wait(&p_full[2 * i + sl], (g >> 1) & 1, wd, SITE_KVM_PV);
               if (ok && i == 0) ok = mbar_wait(&v_full[vs], (g / VS) & 1, wd, SITE_KVM_PV);
-              if (ok && n == sg.n0 && ul > 0) ok = mbar_wait(&o_empty[i], (ul - 1) & 1, wd, SITE_KVM_PV);
+              if (ok && n == n0 && ul > 0) ok = mbar_wait(&o_empty[i], (ul - 1) & 1, wd, SITE_KVM_PV);
               if (!ok) break;
               tc_fence_after();
               const uint64_t vd = v_desc0 + static_cast<uint32_t>((vs * TB) >> 4);
@@ -400,9 +420,9 @@ __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const
 #pragma unroll
               for (int kk = 0; kk < KVM_TK / 16; ++kk)
                 umma_f16_ts(d_tmem, p_tmem + kk * 8, vd + static_cast<uint32_t>(kk * (2048 >> 4)), IDESC_O,
-                            (n > sg.n0 || kk > 0) ? 1u : 0u);
+                            (n > n0 || kk > 0) ? 1u : 0u);
               umma_commit(&pv_done[2 * i + sl]);
-              if (n == sg.n1 - 1) umma_commit(&o_full[i]);
+              if (n == n1 - 1) umma_commit(&o_full[i]);
               if (i == QT - 1) umma_commit(&v_empty[vs]);
             }
           }
@@ -423,14 +443,51 @@ __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const
     const float sl2 = a.scale_log2;
     bool ok = true;
     int g = 0;
-    for (int ul = 0; ok && kvm_next(a, ROWS, walk, sg); ++ul) {
-      const int row = sg.rb * ROWS + ti * 128 + r;
-      const bool have = row < sg.s.n * a.group;
-      const int tok = have ? row / a.group : 0;
-      const int limit = have ? kv_limit(sg.s, tok, a.causal) : sg.s.len;
+    // This thread's row of a segment, and its copy of it into Q_i.
+    struct RowOf {
+      bool have;
+      int tok, head, limit;
+    };
+    auto row_of = [&](const KvmSegment& u) {
+      const int row = u.rb * ROWS + ti * 128 + r;
+      RowOf x;
+      x.have = row < u.s.n * a.group;
+      const int tok = x.have ? row / a.group : 0;
+      x.tok = u.s.first + tok;
+      x.head = u.h * a.group + (x.have ? row - tok * a.group : 0);
+      x.limit = x.have ? kv_limit(u.s, tok, a.causal) : u.s.len;
+      return x;
+    };
+    auto copy_q = [&](const RowOf& x) {
+      const __half* src = a.Q + x.tok * a.q_stride + static_cast<long long>(x.head) * D;
+      const uint32_t dst = smem_u32(sQ + ti * QB) + r * 128, n = x.have ? 16u : 0u;  // 0: filled with zeros
+#pragma unroll
+      for (int ch = 0; ch < D / 8; ++ch)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + (ch >> 3) * 16384 +
+                                                                           (((ch & 7) ^ (r & 7)) * 16)),
+                     "l"(src + ch * 8), "r"(n)
+                     : "memory");
+    };
+    auto q_in_place = [&]() {
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      fence_proxy_async_smem();
+      mbar_arrive(&q_full[ti]);
+    };
+    bool more = kvm_next(a, ROWS, walk, sg);
+    RowOf me = row_of(sg);
+    if (more) {
+      copy_q(me);
+      q_in_place();
+    }
+    for (int ul = 0; ok && more; ++ul) {
+      const KvmSegment cur = sg;
+      more = kvm_next(a, ROWS, walk, sg);
+      RowOf next{};
+      if (more) next = row_of(sg);
+      const int limit = me.limit;
       float m = KV_NO_MAX;  // running max, log2 domain (possibly stale by < 8)
       float l = 0.f;
-      for (int n = sg.n0; n < sg.n1; ++n, ++g) {
+      for (int n = cur.n0; n < cur.n1; ++n, ++g) {
         const int sl = g & 1;
         const uint32_t tSl = tS + sl * KVM_TK;
         ok = __all_sync(0xffffffffu, mbar_wait(&s_full[2 * ti + sl], (g >> 1) & 1, wd, SITE_KVM_SOFTMAX));
@@ -448,6 +505,8 @@ __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const
             x[32 + i] = __uint_as_float(v1[i]);
           }
         }
+        // The unit's last S_i is complete: Q_i may take the next unit's rows.
+        if (n == cur.n1 - 1 && more) copy_q(next);
         const int valid = limit - n * KVM_TK;
         if (__any_sync(0xffffffffu, valid < KVM_TK)) {
 #pragma unroll
@@ -455,7 +514,7 @@ __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const
             if (i >= valid) x[i] = -INFINITY;
         }
         float part;
-        if (n == sg.n0) {
+        if (n == cur.n0) {
           m = fmaxf(att_row_max64(x) * sl2, KV_NO_MAX);
           part = att_exp_store64<EMU>(x, sl2, m, tSl);
         } else {
@@ -493,55 +552,63 @@ __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const
         mbar_arrive(&p_full[2 * ti + sl]);
       }
       if (!ok) break;
+      if (more) q_in_place();
       // The segment's O: out, or into a partial if the unit goes on elsewhere.
       ok = __all_sync(0xffffffffu, mbar_wait(&o_full[ti], ul & 1, wd, SITE_KVM_SOFTMAX));
       if (!ok) break;
       tc_fence_after();
-      const bool whole = sg.n0 == 0 && sg.n1 == sg.steps;
-      const float inv_l = l > 0.f ? 1.0f / l : 0.f;
-      const long long token = sg.s.first + tok;
-      const int head = sg.h * a.group + (have ? row % a.group : 0);
-      __half* out = a.O + token * a.o_stride + static_cast<long long>(head) * D;
-      float* part = a.partials + kvm_slot<D, ROWS>(2ll * blockIdx.x + (sg.n0 == 0 ? 1 : 0));
+      const bool whole = cur.n0 == 0 && cur.n1 == cur.steps;
+      // 4-bit values lie as elements 0 4 1 5 2 6 3 7 in each 8 columns.
+      auto column = [](int k) { return BITS == 4 ? (k < 4 ? 2 * k : 2 * (k - 4) + 1) : k; };
+      if (whole) {
+        const float inv_l = l > 0.f ? 1.0f / l : 0.f;
+        uint32_t out[D / 2];  // the row in fp16: O's columns are free before it is stored
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          tmem_ld_32x32b_x32(tO + c * 32, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; i += 2)
+            out[c * 16 + i / 2] = pack_half2(__uint_as_float(o[(i & ~7) + column(i & 7)]) * inv_l,
+                                             __uint_as_float(o[(i & ~7) + column((i & 7) + 1)]) * inv_l);
+        }
+        tc_fence_before();
+        mbar_arrive(&o_empty[ti]);
+        if (me.have) {
+          uint4* dst = reinterpret_cast<uint4*>(a.O + me.tok * a.o_stride + static_cast<long long>(me.head) * D);
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i)
+            dst[i] = make_uint4(out[4 * i], out[4 * i + 1], out[4 * i + 2], out[4 * i + 3]);
+          if (a.lse != nullptr)
+            a.lse[static_cast<long long>(me.tok) * a.heads_q + me.head] = (m + log2f(l)) * 0.6931471805599453f;
+        }
+      } else {
+        float* part = a.partials + kvm_slot<D, ROWS>(2ll * blockIdx.x + (cur.n0 == 0 ? 1 : 0));
+        float4* dst = reinterpret_cast<float4*>(part) + ti * 128 + r;
 #pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t o[32];
-        __syncwarp();
-        tmem_ld_32x32b_x32(tO + c * 32, o);
-        tmem_ld_wait();
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          __syncwarp();
+          tmem_ld_32x32b_x32(tO + c * 32, o);
+          tmem_ld_wait();
+          if (me.have) {
 #pragma unroll
-        for (int i = 0; i < 32; i += 8) {
-          if (!have) break;
-          // 4-bit values lie as elements 0 4 1 5 2 6 3 7 in each 8 columns.
-          float e[8];
-#pragma unroll
-          for (int k = 0; k < 8; ++k)
-            e[k] = __uint_as_float(o[i + (BITS == 4 ? (k < 4 ? 2 * k : 2 * (k - 4) + 1) : k)]);
-          if (whole) {
-            uint4 pk;
-            pk.x = pack_half2(e[0] * inv_l, e[1] * inv_l);
-            pk.y = pack_half2(e[2] * inv_l, e[3] * inv_l);
-            pk.z = pack_half2(e[4] * inv_l, e[5] * inv_l);
-            pk.w = pack_half2(e[6] * inv_l, e[7] * inv_l);
-            *reinterpret_cast<uint4*>(out + c * 32 + i) = pk;
-          } else {
-            float4* dst = reinterpret_cast<float4*>(part) + (c * 8 + i / 4) * ROWS + ti * 128 + r;
-            dst[0] = make_float4(e[0], e[1], e[2], e[3]);
-            dst[ROWS] = make_float4(e[4], e[5], e[6], e[7]);
+            for (int i = 0; i < 32; i += 4)
+              dst[(c * 8 + i / 4) * ROWS] = make_float4(
+                  __uint_as_float(o[(i & ~7) + column(i & 7)]), __uint_as_float(o[(i & ~7) + column((i & 7) + 1)]),
+                  __uint_as_float(o[(i & ~7) + column((i & 7) + 2)]), __uint_as_float(o[(i & ~7) + column((i & 7) + 3)]));
           }
         }
-      }
-      __syncwarp();
-      tc_fence_before();
-      mbar_arrive(&o_empty[ti]);
-      if (have) {
-        if (whole) {
-          if (a.lse != nullptr) a.lse[token * a.heads_q + head] = (m + log2f(l)) * 0.6931471805599453f;
-        } else {
+        __syncwarp();
+        tc_fence_before();
+        mbar_arrive(&o_empty[ti]);
+        if (me.have) {
           part[ROWS * D + ti * 128 + r] = m;
           part[ROWS * D + ROWS + ti * 128 + r] = l;
         }
       }
+      me = next;
     }
   } else {
     // ---------------------------------------------------------- codes to fp16
@@ -650,22 +717,32 @@ template <int D, int ROWS>
 __global__ void __launch_bounds__(256) kv_attention_many_join_kernel(const __grid_constant__ KvAttnArgs a) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int G4 = D / 32;  // groups of 4 elements a warp
-  const long long total = kvm_total(a, ROWS, lane);
-  const long long active = min(static_cast<long long>(a.workers), total);
-  const long long w = blockIdx.x;
-  bool mine = w + 1 < active;
-  KvmPlace p{};
-  long long begin = 0;
-  int steps = 0;
-  if (mine) {
-    const long long x = kv_range_begin(w + 1, total, active);
-    p = kvm_find(a, ROWS, x, lane, &begin, &steps);
-    // In the middle of a unit, and the first border in it.
-    mine = p.n > 0 && begin >= kv_range_begin(w, total, active) && p.b < a.kb.sequences;
+  __shared__ KvmPlace place;
+  __shared__ int last_worker;
+  const int w = blockIdx.x;
+  if (warp == 0) {
+    const long long total = kvm_total(a, ROWS, lane);
+    const long long active = min(static_cast<long long>(a.workers), total);
+    int last = -1;
+    KvmPlace f{};
+    if (w + 1 < active) {
+      long long begin;
+      int steps;
+      f = kvm_find(a, ROWS, kv_range_begin(w + 1, total, active), lane, &begin, &steps);
+      // In the middle of a unit, and the first border in it.
+      if (f.n > 0 && begin >= kv_range_begin(w, total, active) && f.b < a.kb.sequences)
+        last = static_cast<int>(kv_worker_of(begin + steps - 1, total, active));
+    }
+    if (lane == 0) {
+      place = f;
+      last_worker = last;
+    }
   }
+  __syncthreads();
   kv_wait_for_previous();  // in every block: what follows this kernel also follows the one before it
-  if (!mine) return;
-  const int last = static_cast<int>(kv_worker_of(begin + steps - 1, total, active));
+  const KvmPlace p = place;
+  const int last = last_worker;
+  if (last < 0) return;
   const KvSequence s = kvm_sequence(a, p.b);
   const int local = blockIdx.y * 32 + lane;
   const int row = p.rb * ROWS + local;
@@ -675,7 +752,7 @@ __global__ void __launch_bounds__(256) kv_attention_many_join_kernel(const __gri
   for (int i = 0; i < G4; ++i)
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[i][e] = 0.f;
-  for (int k = static_cast<int>(w); k <= last; ++k) {
+  for (int k = w; k <= last; ++k) {
     const float* part = a.partials + kvm_slot<D, ROWS>(2ll * k + (k == w ? 1 : 0));
     const float pm = __ldcg(part + ROWS * D + local), pl = __ldcg(part + ROWS * D + ROWS + local);
     const float m_new = fmaxf(m, pm), f = kv_ex2(m - m_new), fp = kv_ex2(pm - m_new);
