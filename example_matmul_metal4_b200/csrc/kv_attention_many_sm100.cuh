@@ -42,7 +42,10 @@ struct KvMany {
   static constexpr int RAW_BYTES = 2 * KVM_TK * KvRow<D, BITS>::BYTES;
   static constexpr int KS = 3, VS = 3;
   static constexpr int RS = RAW_BYTES <= 10240 ? 3 : 2;
-  static constexpr int BAR_OFFSET = QT * Q_BYTES + (KS + VS) * TILE_BYTES + RS * RAW_BYTES;
+  static constexpr int OUT_ROW = 64 + 16;              // a row of 32 results, on banks of its own
+  static constexpr int OUT_BYTES = 32 * OUT_ROW;       // a softmax warp's results on their way out
+  static constexpr int OUT_OFFSET = QT * Q_BYTES + (KS + VS) * TILE_BYTES + RS * RAW_BYTES;
+  static constexpr int BAR_OFFSET = OUT_OFFSET + 4 * QT * OUT_BYTES;
   static constexpr int SMEM_BYTES = BAR_OFFSET + 512 + 1024;
   // Four warps unpack K and V in turn; with one row tile, four each.
   static constexpr int UNPACK_WARPS = 12 - 4 * QT;
@@ -203,13 +206,15 @@ struct KvmWalk {
 };
 __device__ __forceinline__ bool kvm_next(const KvAttnArgs& a, int rows, KvmWalk& w, KvmSegment& g) {
   while (w.left > 0 && w.p.b < a.kb.sequences) {
-    g.s = kvm_sequence(a, w.p.b);
+    if (g.b != w.p.b) {
+      g.s = kvm_sequence(a, w.p.b);
+      g.b = w.p.b;
+    }
     const int blocks = kvm_blocks(g.s, a.group, rows);
     if (w.p.rb >= blocks) {
       w.p = KvmPlace{w.p.b + 1, 0, 0, 0};
       continue;
     }
-    g.b = w.p.b;
     g.rb = w.p.rb;
     g.h = w.p.h;
     g.n0 = w.p.n;
@@ -324,6 +329,7 @@ __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const
   const uint32_t tmem_base = *tmem_slot;
   KvmWalk walk = *start;
   KvmSegment sg;
+  sg.b = -1;
 
   if (warp < 4) {
     regs_dec<Cfg::REGS_LOW>();
@@ -458,15 +464,24 @@ __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const
       x.limit = x.have ? kv_limit(u.s, tok, a.causal) : u.s.len;
       return x;
     };
+    // The warp's 32 rows of Q: D / 8 lanes a row, so that a copy instruction
+    // touches few lines (a thread copying its own row: 32 of them; 4 us a unit).
     auto copy_q = [&](const RowOf& x) {
-      const __half* src = a.Q + x.tok * a.q_stride + static_cast<long long>(x.head) * D;
-      const uint32_t dst = smem_u32(sQ + ti * QB) + r * 128, n = x.have ? 16u : 0u;  // 0: filled with zeros
+      constexpr int CH = D / 8, RPI = 32 / CH;
+      const long long mine = x.tok * a.q_stride + static_cast<long long>(x.head) * D;
+      const int ch = lane % CH;
+      const uint32_t dst = smem_u32(sQ + ti * QB) + (ch >> 3) * 16384 + q * 32 * 128;
 #pragma unroll
-      for (int ch = 0; ch < D / 8; ++ch)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + (ch >> 3) * 16384 +
-                                                                           (((ch & 7) ^ (r & 7)) * 16)),
-                     "l"(src + ch * 8), "r"(n)
+      for (int i = 0; i < CH; ++i) {
+        const int rr = i * RPI + lane / CH;
+        const long long off = __shfl_sync(0xffffffffu, mine, rr);
+        const bool have = __shfl_sync(0xffffffffu, static_cast<int>(x.have), rr) != 0;
+        const uint32_t n = have ? 16u : 0u;  // 0: filled with zeros
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + rr * 128 +
+                                                                           (((ch & 7) ^ (rr & 7)) * 16)),
+                     "l"(a.Q + off + ch * 8), "r"(n)
                      : "memory");
+      }
     };
     auto q_in_place = [&]() {
       asm volatile("cp.async.wait_all;" ::: "memory");
@@ -480,10 +495,10 @@ __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const
       q_in_place();
     }
     for (int ul = 0; ok && more; ++ul) {
-      const KvmSegment cur = sg;
-      more = kvm_next(a, ROWS, walk, sg);
+      struct {
+        int n0, n1, steps;
+      } const cur{sg.n0, sg.n1, sg.steps};
       RowOf next{};
-      if (more) next = row_of(sg);
       const int limit = me.limit;
       float m = KV_NO_MAX;  // running max, log2 domain (possibly stale by < 8)
       float l = 0.f;
@@ -506,7 +521,13 @@ __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const
           }
         }
         // The unit's last S_i is complete: Q_i may take the next unit's rows.
-        if (n == cur.n1 - 1 && more) copy_q(next);
+        if (n == cur.n1 - 1) {
+          more = kvm_next(a, ROWS, walk, sg);
+          if (more) {
+            next = row_of(sg);
+            copy_q(next);
+          }
+        }
         const int valid = limit - n * KVM_TK;
         if (__any_sync(0xffffffffu, valid < KVM_TK)) {
 #pragma unroll
@@ -575,14 +596,31 @@ __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const
         }
         tc_fence_before();
         mbar_arrive(&o_empty[ti]);
-        if (me.have) {
-          uint4* dst = reinterpret_cast<uint4*>(a.O + me.tok * a.o_stride + static_cast<long long>(me.head) * D);
+        // Rows go out through shared memory, 32 elements at a time, four lanes to
+        // a row.
+        uint8_t* stage = smem + Cfg::OUT_OFFSET + (warp - 4) * Cfg::OUT_BYTES;
+        const long long mine = me.tok * a.o_stride + static_cast<long long>(me.head) * D;
 #pragma unroll
-          for (int i = 0; i < D / 8; ++i)
-            dst[i] = make_uint4(out[4 * i], out[4 * i + 1], out[4 * i + 2], out[4 * i + 3]);
-          if (a.lse != nullptr)
-            a.lse[static_cast<long long>(me.tok) * a.heads_q + me.head] = (m + log2f(l)) * 0.6931471805599453f;
+        for (int c = 0; c < D / 32; ++c) {
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<uint4*>(stage + lane * Cfg::OUT_ROW + i * 16) =
+                make_uint4(out[c * 16 + 4 * i], out[c * 16 + 4 * i + 1], out[c * 16 + 4 * i + 2],
+                           out[c * 16 + 4 * i + 3]);
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int rr = i * 8 + (lane >> 2);
+            const long long off = __shfl_sync(0xffffffffu, mine, rr);
+            const bool have = __shfl_sync(0xffffffffu, static_cast<int>(me.have), rr) != 0;
+            if (have)
+              *reinterpret_cast<uint4*>(a.O + off + c * 32 + (lane & 3) * 8) =
+                  *reinterpret_cast<const uint4*>(stage + rr * Cfg::OUT_ROW + (lane & 3) * 16);
+          }
         }
+        if (me.have && a.lse != nullptr)
+          a.lse[static_cast<long long>(me.tok) * a.heads_q + me.head] = (m + log2f(l)) * 0.6931471805599453f;
       } else {
         float* part = a.partials + kvm_slot<D, ROWS>(2ll * blockIdx.x + (cur.n0 == 0 ? 1 : 0));
         float4* dst = reinterpret_cast<float4*>(part) + ti * 128 + r;
