@@ -508,6 +508,22 @@ __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const
         ok = __all_sync(0xffffffffu, mbar_wait(&s_full[2 * ti + sl], (g >> 1) & 1, wd, SITE_KVM_SOFTMAX));
         if (!ok) break;
         tc_fence_after();
+        // Masked scores are rewritten in place, off the path of the steps that
+        // have none (most: a unit's last ROWS / group / 64 steps of many).
+        const int valid = limit - n * KVM_TK;
+        if (__any_sync(0xffffffffu, valid < KVM_TK)) {
+#pragma unroll 1
+          for (int c = 0; c < KVM_TK; c += 16) {
+            uint32_t v[16];
+            tmem_ld_32x32b_x16(tSl + c, v);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (c + i >= valid) v[i] = __float_as_uint(-INFINITY);
+            tmem_st_32x32b_x16(tSl + c, v);
+          }
+          tmem_st_wait();
+        }
         float x[64];
         {
           uint32_t v0[32], v1[32];
@@ -528,30 +544,20 @@ __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const
             copy_q(next);
           }
         }
-        const int valid = limit - n * KVM_TK;
-        if (__any_sync(0xffffffffu, valid < KVM_TK)) {
-#pragma unroll
-          for (int i = 0; i < 64; ++i)
-            if (i >= valid) x[i] = -INFINITY;
-        }
-        float part;
-        if (n == cur.n0) {
-          m = fmaxf(att_row_max64(x) * sl2, KV_NO_MAX);
-          part = att_exp_store64<EMU>(x, sl2, m, tSl);
-        } else {
-          // Exponentials against the running max, the new row max alongside.
-          part = att_exp_store64<EMU>(x, sl2, m, tSl);
-          const float mx = att_row_max64(x) * sl2;
-          const bool grow = (mx > m + 8.0f);
-          if (__any_sync(0xffffffffu, grow)) {
+        const float mx = att_row_max64(x) * sl2;
+        const bool grow = mx > m + 8.0f;
+        if (__any_sync(0xffffffffu, grow)) {
+          const float m_new = grow ? mx : m;
+          const float factor = grow ? ex2_approx(m - m_new) : 1.0f;
+          l *= factor;
+          m = m_new;
+          if (n > cur.n0) {
             // Rescale this warp's O rows once the previous step's P V (the only
-            // MMA that may still write them) is done, and redo the exponentials.
+            // MMA that may still write them) is done.
             ok = __all_sync(0xffffffffu,
                             mbar_wait(&pv_done[2 * ti + (sl ^ 1)], ((g - 1) >> 1) & 1, wd, SITE_KVM_SOFTMAX));
             if (!ok) break;
             tc_fence_after();
-            const float m_new = grow ? mx : m;
-            const float factor = grow ? ex2_approx(m - m_new) : 1.0f;
 #pragma unroll 1
             for (int c = 0; c < D / 16; ++c) {
               uint32_t v[16];
@@ -561,12 +567,10 @@ __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const
               for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * factor);
               tmem_st_32x32b_x16(tO + c * 16, v);
             }
-            l *= factor;
-            m = m_new;
             tmem_st_wait();
-            part = att_exp_store64<EMU>(x, sl2, m, tSl);
           }
         }
+        const float part = att_exp_store64<EMU>(x, sl2, m, tSl);
         l += part;
         tmem_st_wait();
         tc_fence_before();
