@@ -33,6 +33,11 @@ namespace mm4 {
 
 constexpr int KVM_TK = 64;        // keys of a step
 constexpr int KVM_THREADS = 512;
+// What a unit costs beyond its steps (its Q, its masked steps, its results, the
+// pipeline run empty and filled), in steps: a CTA's range is cut by steps
+// plus this for each unit, or the first blocks of causal prompts, 4 steps
+// each, would take twice the time of the last ones.
+constexpr int KVM_UNIT = 4;
 
 template <int D, int BITS, int QT>
 struct KvMany {
@@ -89,7 +94,7 @@ __device__ __forceinline__ KvSequence kvm_sequence(const KvAttnArgs& a, int b) {
   }
   return s;
 }
-// Steps of a sequence for one head. The lanes of a warp share either the
+// Cost of a sequence for one head. The lanes of a warp share either the
 // sequences or, where those are fewer than the row blocks that a sequence may
 // have, the blocks of one sequence after the other.
 __device__ __forceinline__ bool kvm_by_block(const KvAttnArgs& a, int rows) {
@@ -100,25 +105,26 @@ __device__ __forceinline__ long long kvm_warp_sum(long long x) {
   for (int s = 16; s > 0; s >>= 1) x += __shfl_xor_sync(0xffffffffu, x, s);
   return x;
 }
-__device__ __forceinline__ int kvm_lane_steps(const KvAttnArgs& a, int b, int rows) {  // lanes: sequences
+__device__ __forceinline__ int kvm_lane_cost(const KvAttnArgs& a, int b, int rows) {  // lanes: sequences
   if (b >= a.kb.sequences) return 0;
   const KvSequence s = kvm_sequence(a, b);
   const int blocks = kvm_blocks(s, a.group, rows);
   int sum = 0;
-  for (int rb = 0; rb < blocks; ++rb) sum += kvm_steps(s, rb, a, rows);
+  for (int rb = 0; rb < blocks; ++rb) sum += KVM_UNIT + kvm_steps(s, rb, a, rows);
   return sum;
 }
-__device__ __forceinline__ long long kvm_block_steps(const KvAttnArgs& a, const KvSequence& s, int rows,
+__device__ __forceinline__ long long kvm_block_cost(const KvAttnArgs& a, const KvSequence& s, int rows,
                                                      int lane) {  // lanes: blocks
   const int blocks = kvm_blocks(s, a.group, rows);
   long long sum = 0;
-  for (int rb = lane; rb < blocks; rb += 32) sum += kvm_steps(s, rb, a, rows);
+  for (int rb = lane; rb < blocks; rb += 32) sum += KVM_UNIT + kvm_steps(s, rb, a, rows);
   return kvm_warp_sum(sum);
 }
 
-// A place on the line of all steps: sequences, their row blocks, heads, steps.
+// A place on the line of all units: sequences, their row blocks, heads, and
+// the offset in the unit: KVM_UNIT before its first step.
 struct KvmPlace {
-  int b, rb, h, n;
+  int b, rb, h, off;
 };
 __device__ __forceinline__ long long kvm_total(const KvAttnArgs& a, int rows, int lane) {
   long long sum = 0;
@@ -126,28 +132,28 @@ __device__ __forceinline__ long long kvm_total(const KvAttnArgs& a, int rows, in
     for (int b = 0; b < a.kb.sequences; ++b) {
       const KvSequence s = kvm_sequence(a, b);
       const int blocks = kvm_blocks(s, a.group, rows);
-      for (int rb = lane; rb < blocks; rb += 32) sum += kvm_steps(s, rb, a, rows);
+      for (int rb = lane; rb < blocks; rb += 32) sum += KVM_UNIT + kvm_steps(s, rb, a, rows);
     }
   } else {
-    for (int b = lane; b < a.kb.sequences; b += 32) sum += kvm_lane_steps(a, b, rows);
+    for (int b = lane; b < a.kb.sequences; b += 32) sum += kvm_lane_cost(a, b, rows);
   }
   return kvm_warp_sum(sum) * a.kb.heads_kv;
 }
-// Place x (by one warp); also where its unit begins and how many steps it has.
+// Place x (by one warp); also where its unit begins and what it costs.
 __device__ __forceinline__ KvmPlace kvm_find(const KvAttnArgs& a, int rows, long long x, int lane,
-                                             long long* unit_begin, int* unit_steps) {
+                                             long long* unit_begin, int* unit_cost) {
   const int heads = a.kb.heads_kv;
   KvmPlace p{0, 0, 0, 0};
   long long at = 0;  // where sequence p.b begins
   if (kvm_by_block(a, rows)) {
     for (; p.b < a.kb.sequences; ++p.b) {
-      const long long all = kvm_block_steps(a, kvm_sequence(a, p.b), rows, lane) * heads;
+      const long long all = kvm_block_cost(a, kvm_sequence(a, p.b), rows, lane) * heads;
       if (at + all > x) break;
       at += all;
     }
   } else {
     for (; p.b < a.kb.sequences; p.b += 32) {
-      const int t = kvm_lane_steps(a, p.b + lane, rows);
+      const int t = kvm_lane_cost(a, p.b + lane, rows);
       long long inc = t;
 #pragma unroll
       for (int s = 1; s < 32; s <<= 1) {
@@ -165,13 +171,13 @@ __device__ __forceinline__ KvmPlace kvm_find(const KvAttnArgs& a, int rows, long
     }
   }
   *unit_begin = x;
-  *unit_steps = 1;
+  *unit_cost = 1;
   if (p.b >= a.kb.sequences) return KvmPlace{a.kb.sequences, 0, 0, 0};
   // The row block: a scan over 32 blocks at a time.
   const KvSequence s = kvm_sequence(a, p.b);
   const int blocks = kvm_blocks(s, a.group, rows);
   for (; p.rb < blocks; p.rb += 32) {
-    const int t = p.rb + lane < blocks ? kvm_steps(s, p.rb + lane, a, rows) : 0;
+    const int t = p.rb + lane < blocks ? KVM_UNIT + kvm_steps(s, p.rb + lane, a, rows) : 0;
     int inc = t;
 #pragma unroll
     for (int k = 1; k < 32; k <<= 1) {
@@ -181,13 +187,13 @@ __device__ __forceinline__ KvmPlace kvm_find(const KvAttnArgs& a, int rows, long
     const unsigned over = __ballot_sync(0xffffffffu, at + static_cast<long long>(inc) * heads > x);
     if (over != 0) {
       const int k = __ffs(over) - 1;
-      const int steps = __shfl_sync(0xffffffffu, t, k);
+      const int cost = __shfl_sync(0xffffffffu, t, k);
       at += static_cast<long long>(__shfl_sync(0xffffffffu, inc - t, k)) * heads;
       p.rb += k;
-      p.h = static_cast<int>((x - at) / steps);
-      p.n = static_cast<int>((x - at) % steps);
-      *unit_begin = x - p.n;
-      *unit_steps = steps;
+      p.h = static_cast<int>((x - at) / cost);
+      p.off = static_cast<int>((x - at) % cost);
+      *unit_begin = x - p.off;
+      *unit_cost = cost;
       return p;
     }
     at += static_cast<long long>(__shfl_sync(0xffffffffu, inc, 31)) * heads;
@@ -217,18 +223,21 @@ __device__ __forceinline__ bool kvm_next(const KvAttnArgs& a, int rows, KvmWalk&
     }
     g.rb = w.p.rb;
     g.h = w.p.h;
-    g.n0 = w.p.n;
     g.steps = kvm_steps(g.s, g.rb, a, rows);
-    g.n1 = static_cast<int>(min(static_cast<long long>(g.steps), g.n0 + w.left));
-    w.left -= g.n1 - g.n0;
-    w.p.n = g.n1;
-    if (g.n1 == g.steps) {
-      w.p.n = 0;
+    const int cost = KVM_UNIT + g.steps;
+    const int end = static_cast<int>(min(static_cast<long long>(cost), w.p.off + w.left));
+    g.n0 = max(0, w.p.off - KVM_UNIT);
+    g.n1 = end - KVM_UNIT;
+    w.left -= end - w.p.off;
+    w.p.off = end;
+    if (end == cost) {
+      w.p.off = 0;
       if (++w.p.h == a.kb.heads_kv) {
         w.p.h = 0;
         ++w.p.rb;
       }
     }
+    if (g.n1 <= g.n0) continue;  // the range ends before the unit's first step
     return true;
   }
   return false;
@@ -317,8 +326,8 @@ __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const
     if (blockIdx.x < active) {
       const long long x = kv_range_begin(blockIdx.x, total, active);
       long long begin;
-      int steps;
-      w.p = kvm_find(a, ROWS, x, lane, &begin, &steps);
+      int cost;
+      w.p = kvm_find(a, ROWS, x, lane, &begin, &cost);
       w.left = kv_range_begin(blockIdx.x + 1, total, active) - x;
     }
     if (lane == 0) *start = w;
@@ -508,22 +517,6 @@ __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const
         ok = __all_sync(0xffffffffu, mbar_wait(&s_full[2 * ti + sl], (g >> 1) & 1, wd, SITE_KVM_SOFTMAX));
         if (!ok) break;
         tc_fence_after();
-        // Masked scores are rewritten in place, off the path of the steps that
-        // have none (most: a unit's last ROWS / group / 64 steps of many).
-        const int valid = limit - n * KVM_TK;
-        if (__any_sync(0xffffffffu, valid < KVM_TK)) {
-#pragma unroll 1
-          for (int c = 0; c < KVM_TK; c += 16) {
-            uint32_t v[16];
-            tmem_ld_32x32b_x16(tSl + c, v);
-            tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              if (c + i >= valid) v[i] = __float_as_uint(-INFINITY);
-            tmem_st_32x32b_x16(tSl + c, v);
-          }
-          tmem_st_wait();
-        }
         float x[64];
         {
           uint32_t v0[32], v1[32];
@@ -536,12 +529,14 @@ __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const
             x[32 + i] = __uint_as_float(v1[i]);
           }
         }
-        // The unit's last S_i is complete: Q_i may take the next unit's rows.
-        if (n == cur.n1 - 1) {
-          more = kvm_next(a, ROWS, walk, sg);
-          if (more) {
-            next = row_of(sg);
-            copy_q(next);
+        const int valid = limit - n * KVM_TK;
+        if (__any_sync(0xffffffffu, valid < KVM_TK)) {
+          const uint64_t seen = valid <= 0 ? 0ull : valid >= 64 ? ~0ull : (1ull << valid) - 1;
+          const uint32_t lo = static_cast<uint32_t>(seen), hi = static_cast<uint32_t>(seen >> 32);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            if ((lo & (1u << i)) == 0) x[i] = -INFINITY;
+            if ((hi & (1u << i)) == 0) x[32 + i] = -INFINITY;
           }
         }
         const float mx = att_row_max64(x) * sl2;
@@ -577,7 +572,12 @@ __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const
         mbar_arrive(&p_full[2 * ti + sl]);
       }
       if (!ok) break;
-      if (more) q_in_place();
+      // The unit's last S_i is complete: Q_i takes the next unit's rows.
+      more = kvm_next(a, ROWS, walk, sg);
+      if (more) {
+        next = row_of(sg);
+        copy_q(next);
+      }
       // The segment's O: out, or into a partial if the unit goes on elsewhere.
       ok = __all_sync(0xffffffffu, mbar_wait(&o_full[ti], ul & 1, wd, SITE_KVM_SOFTMAX));
       if (!ok) break;
@@ -600,6 +600,7 @@ __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const
         }
         tc_fence_before();
         mbar_arrive(&o_empty[ti]);
+        if (more) q_in_place();
         // Rows go out through shared memory, 32 elements at a time, four lanes to
         // a row.
         uint8_t* stage = smem + Cfg::OUT_OFFSET + (warp - 4) * Cfg::OUT_BYTES;
@@ -645,6 +646,7 @@ __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const
         __syncwarp();
         tc_fence_before();
         mbar_arrive(&o_empty[ti]);
+        if (more) q_in_place();
         if (me.have) {
           part[ROWS * D + ti * 128 + r] = m;
           part[ROWS * D + ROWS + ti * 128 + r] = l;
@@ -665,49 +667,58 @@ __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const
     const int sub = (lane & 7) + 8 * (lane / (8 * GR));
     const int gr = (lane >> 3) % GR;
     const uint32_t k1024 = __shfl_sync(0xffffffffu, a.k1024, 0);
-    int g = 0;
+    // Places of this thread's first row in a raw stage and of its four chunks in
+    // a tile; later passes and V lie at constant distances (rows go up by a
+    // multiple of 8, so the swizzle stays).
+    constexpr int PASS_ROWS = 4 * RW;
+    const int row0 = uw * RW + sub;
+    const uint32_t raw0 = smem_u32(sR) + row0 * RB, codes0 = raw0 + gr * (KV_GROUP * BITS / 8),
+                   par0 = raw0 + Row::CODES + gr * 4;
+    uint32_t chunk0[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int ch = gr * 4 + c;
+      chunk0[c] = smem_u32(sK) + (ch >> 3) * (KVM_TK * 128) + row0 * 128 + (((ch & 7) ^ (row0 & 7)) * 16);
+    }
+    int g = 0, rs = 0, ks = 0, vs = 0;  // step, and its place in each ring
     bool ok = true;
     while (ok && kvm_next(a, ROWS, walk, sg)) {
       for (int n = sg.n0; n < sg.n1 && ok; ++n, ++g) {
-        const int rs = g % RS, st[2] = {g % KS, g % VS};
         ok = mbar_wait(&r_full[rs], (g / RS) & 1, wd, SITE_KVM_UNPACK);
-        const uint8_t* raw = sR + rs * Cfg::RAW_BYTES;
         const int valid = sg.s.len - n * KVM_TK;
+        const bool tail = valid < KVM_TK;
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
           if (kv < kv0 || kv > kv1) continue;
           const int depth = kv == 0 ? KS : VS;
           if (ok && g >= depth)
-            ok = mbar_wait(kv == 0 ? &k_empty[st[0]] : &v_empty[st[1]], (g / depth - 1) & 1, wd, SITE_KVM_UNPACK);
+            ok = mbar_wait(kv == 0 ? &k_empty[ks] : &v_empty[vs], (g / depth - 1) & 1, wd, SITE_KVM_UNPACK);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
-          uint8_t* tile = kv == 0 ? sK + st[0] * TB : sV + st[1] * TB;
+          const uint32_t to = kv == 0 ? ks * TB : KS * TB + vs * TB;
+          const uint32_t from = rs * Cfg::RAW_BYTES;
 #pragma unroll
           for (int p = 0; p < PASSES; ++p) {
-            const int row = (p * 4 + uw) * RW + sub;
-            const uint8_t* src = raw + (kv * KVM_TK + row) * RB;
-            __half2 par = *reinterpret_cast<const __half2*>(src + Row::CODES + gr * 4);
+            const int skip = (kv * KVM_TK + p * PASS_ROWS) * RB;
+            uint32_t par;
+            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(par) : "r"(par0 + from + skip));
             // Rows behind the sequence hold anything; their values count as 0.
-            if (row >= valid) par = __float2half2_rn(0.f);
-            const __half2 s2 = __low2half2(par), z2 = __high2half2(par);
+            if (tail && row0 + p * PASS_ROWS >= valid) par = 0u;
+            const __half2 s2 = __low2half2(as_half2(par)), z2 = __high2half2(as_half2(par));
             constexpr int WORDS = KV_GROUP * BITS / 32;
             uint32_t w[WORDS];
             if constexpr (RB % 16 == 0) {
 #pragma unroll
-              for (int i = 0; i < WORDS; i += 4) {
-                const uint4 v = *reinterpret_cast<const uint4*>(src + gr * (KV_GROUP * BITS / 8) + 4 * i);
-                w[i] = v.x;
-                w[i + 1] = v.y;
-                w[i + 2] = v.z;
-                w[i + 3] = v.w;
-              }
+              for (int i = 0; i < WORDS; i += 4)
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3])
+                             : "r"(codes0 + from + skip + 4 * i));
             } else {
 #pragma unroll
-              for (int i = 0; i < WORDS; i += 2) {
-                const uint2 v = *reinterpret_cast<const uint2*>(src + gr * (KV_GROUP * BITS / 8) + 4 * i);
-                w[i] = v.x;
-                w[i + 1] = v.y;
-              }
+              for (int i = 0; i < WORDS; i += 2)
+                asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];"
+                             : "=r"(w[i]), "=r"(w[i + 1])
+                             : "r"(codes0 + from + skip + 4 * i));
             }
 #pragma unroll
             for (int c = 0; c < 4; ++c) {  // 8 elements, 16 bytes
@@ -729,16 +740,19 @@ __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const
                 out.z = as_u32(__hfma2(kv_codes8(w[2 * c + 1], 0x4140), s2, z2));
                 out.w = as_u32(__hfma2(kv_codes8(w[2 * c + 1], 0x4342), s2, z2));
               }
-              const int ch = gr * 4 + c;
-              *reinterpret_cast<uint4*>(tile + (ch >> 3) * (KVM_TK * 128) + row * 128 +
-                                        (((ch & 7) ^ (row & 7)) * 16)) = out;
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(chunk0[c] + to + p * PASS_ROWS * 128),
+                           "r"(out.x), "r"(out.y), "r"(out.z), "r"(out.w)
+                           : "memory");
             }
           }
           fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0) mbar_arrive(kv == 0 ? &k_full[st[0]] : &v_full[st[1]]);
+          if (lane == 0) mbar_arrive(kv == 0 ? &k_full[ks] : &v_full[vs]);
         }
         if (ok && lane == 0) mbar_arrive(&r_empty[rs]);
+        rs = rs + 1 == RS ? 0 : rs + 1;
+        ks = ks + 1 == KS ? 0 : ks + 1;
+        vs = vs + 1 == VS ? 0 : vs + 1;
       }
     }
   }
@@ -769,11 +783,11 @@ __global__ void __launch_bounds__(256) kv_attention_many_join_kernel(const __gri
     KvmPlace f{};
     if (w + 1 < active) {
       long long begin;
-      int steps;
-      f = kvm_find(a, ROWS, kv_range_begin(w + 1, total, active), lane, &begin, &steps);
-      // In the middle of a unit, and the first border in it.
-      if (f.n > 0 && begin >= kv_range_begin(w, total, active) && f.b < a.kb.sequences)
-        last = static_cast<int>(kv_worker_of(begin + steps - 1, total, active));
+      int cost;
+      f = kvm_find(a, ROWS, kv_range_begin(w + 1, total, active), lane, &begin, &cost);
+      // Behind the unit's first step, and the first border that is.
+      if (f.off > KVM_UNIT && begin + KVM_UNIT >= kv_range_begin(w, total, active) && f.b < a.kb.sequences)
+        last = static_cast<int>(kv_worker_of(begin + cost - 1, total, active));
     }
     if (lane == 0) {
       place = f;
