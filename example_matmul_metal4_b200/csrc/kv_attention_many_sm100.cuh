@@ -250,6 +250,39 @@ __device__ __forceinline__ long long kvm_slot(long long slot) {
   return slot * KvPartial<D, ROWS>::FLOATS;
 }
 
+// As att_exp_store64, calling between() behind the first half.
+template <int EMU, typename F>
+__device__ __forceinline__ float kvm_exp_store64(const float (&x)[64], float sl2, float m, uint32_t tP, F&& between) {
+  const float2 sc = make_float2(sl2, sl2);
+  const float2 nm = make_float2(-m, -m);
+  float2 acc[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    uint32_t pk[16];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int idx = half * 32 + c * 8 + 2 * e;
+        const float2 y = ffma2(make_float2(x[idx], x[idx + 1]), sc, nm);
+        float2 p;
+        if (2 * e >= 8 - EMU) {
+          p = ex2_poly2(y);
+        } else {
+          p.x = ex2_approx(y.x);
+          p.y = ex2_approx(y.y);
+        }
+        acc[e] = fadd2(acc[e], p);
+        pk[c * 4 + e] = pack_half2(p.x, p.y);
+      }
+    }
+    tmem_st_32x32b_x16(tP + half * 16, pk);
+    if (half == 0) between();
+  }
+  const float2 sum = fadd2(fadd2(acc[0], acc[1]), fadd2(acc[2], acc[3]));
+  return sum.x + sum.y;
+}
+
 template <int D, int BITS, int QT>
 __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const __grid_constant__ KvAttnArgs a) {
   using Cfg = KvMany<D, BITS, QT>;
@@ -259,6 +292,7 @@ __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const
   constexpr uint32_t IDESC_S = idesc_f16_f32(128, KVM_TK, false, false);
   constexpr uint32_t IDESC_O = idesc_f16_f32(128, D, false, true);
   constexpr int EMU = AttFwdCfg<D>::EMU_PER8;
+  constexpr bool TURNS = QT == 2 && D == 128;  // at D = 64 turns cost more than they give (186 -> 201 us)
 
   extern __shared__ uint8_t kvm_smem_raw[];
   const uint32_t raw_addr = smem_u32(kvm_smem_raw);
@@ -281,8 +315,9 @@ __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const
   uint64_t* v_empty = v_full + VS;          // [VS]
   uint64_t* r_full = v_empty + VS;          // [RS] copied
   uint64_t* r_empty = r_full + RS;          // [RS] unpacked
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(r_empty + RS);
-  KvmWalk* start = reinterpret_cast<KvmWalk*>(smem + Cfg::BAR_OFFSET + 384);
+  uint64_t* turn = r_empty + RS;            // [tile][quadrant] exponentials of this tile's warp done
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(turn + 8);
+  KvmWalk* start = reinterpret_cast<KvmWalk*>(smem + Cfg::BAR_OFFSET + 448);
 
   const KvBatch& kb = a.kb;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -301,6 +336,7 @@ __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const
       }
     }
     mbar_init(drain, 2);
+    for (int i = 0; i < 8; ++i) mbar_init(&turn[i], 1);
     for (int i = 0; i < KS; ++i) {
       mbar_init(&k_full[i], 4);
       mbar_init(&k_empty[i], 1);
@@ -565,7 +601,18 @@ __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const
             tmem_st_wait();
           }
         }
-        const float part = att_exp_store64<EMU>(x, sl2, m, tSl);
+        // The two row tiles' warps of an SM quarter take turns at the
+        // exponentials: at the same time each would take twice as long, and
+        // neither would load scores or find maxima meanwhile.
+        if (TURNS) {
+          if (ti == 1 || g > 0)
+            ok = mbar_wait(&turn[(1 - ti) * 4 + q], (ti == 1 ? g : g - 1) & 1, wd, SITE_KVM_SOFTMAX);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+        }
+        const float part = kvm_exp_store64<EMU>(x, sl2, m, tSl, [&] {
+          if (TURNS && lane == 0) mbar_arrive(&turn[ti * 4 + q]);
+        });
         l += part;
         tmem_st_wait();
         tc_fence_before();
