@@ -494,8 +494,12 @@ __global__ void __launch_bounds__(KvFew<D, BITS, NT>::THREADS, 1) kv_attention_f
         kv_load_words<VW, RB % 16 == 0>(row + g * (VC * BITS / 8), w4[i]);
         par[i] = *reinterpret_cast<const __half2*>(row + Row::CODES + (g * VC / KV_GROUP) * 4);
       }
-      const __half2 s01 = __lows2half2(par[0], par[1]), z01 = __highs2half2(par[0], par[1]);
-      const __half2 s23 = __lows2half2(par[2], par[3]), z23 = __highs2half2(par[2], par[3]);
+      // Scales and zeros of the two keys of a pair. The shuffle (of a lane with
+      // itself) keeps the compiler from merging them again for each of their
+      // uses, which costs more than the unpacking (106 -> 96 us).
+      auto keep = [&](__half2 v) { return as_half2(__shfl_sync(0xffffffffu, as_u32(v), lane)); };
+      const __half2 s01 = keep(__lows2half2(par[0], par[1])), z01 = keep(__highs2half2(par[0], par[1]));
+      const __half2 s23 = keep(__lows2half2(par[2], par[3])), z23 = keep(__highs2half2(par[2], par[3]));
 #pragma unroll
       for (int i = 0; i < VW; ++i) {
         uint32_t x[32 / BITS], y[32 / BITS];

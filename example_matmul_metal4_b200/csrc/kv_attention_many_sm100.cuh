@@ -292,7 +292,7 @@ __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const
   constexpr uint32_t IDESC_S = idesc_f16_f32(128, KVM_TK, false, false);
   constexpr uint32_t IDESC_O = idesc_f16_f32(128, D, false, true);
   constexpr int EMU = AttFwdCfg<D>::EMU_PER8;
-  constexpr bool TURNS = QT == 2 && D == 128;  // at D = 64 turns cost more than they give (186 -> 201 us)
+  constexpr bool TURNS = QT == 2;
 
   extern __shared__ uint8_t kvm_smem_raw[];
   const uint32_t raw_addr = smem_u32(kvm_smem_raw);
