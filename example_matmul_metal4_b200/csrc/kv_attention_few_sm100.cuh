@@ -28,21 +28,25 @@ namespace mm4 {
 
 constexpr int KVF_TK = 32;  // keys of a tile
 
-template <int D, int BITS, int NT>
+template <int D, int BITS, int NT, bool TEAM>
 struct KvFew {
   static constexpr int ROWS = 8 * NT;
   static constexpr int ROW_BYTES = KvRow<D, BITS>::BYTES;
-  static constexpr int STAGE_BYTES = 2 * KVF_TK * ROW_BYTES;  // K rows, then V rows
-  // Warps that compute, and tiles in flight for each: up to 164 KB of copies in
-  // flight. 16 warps in all with 128 registers a thread, or 8 with more.
-  static constexpr int WARPS = NT == 1 && STAGE_BYTES <= 5120 ? 15 : 7;
+  static constexpr int STAGE_BYTES = 2 * KVF_TK * ROW_BYTES;  // K rows of a tile, then V rows
+  // Warps that compute: 14 with 128 registers a thread, or 7 with more. What
+  // bounds the arithmetic is the SM's logic and fp16 instructions, not their
+  // number; fewer warps leave more of the ring to each.
+  static constexpr int WARPS = NT == 1 && STAGE_BYTES <= 5120 ? 14 : 7;
   static constexpr int THREADS = 32 * (WARPS + 1);
-  static constexpr int STAGES = STAGE_BYTES * WARPS * 4 <= 168 * 1024 ? 4 : 2;
-  static constexpr int SLOTS = (WARPS + 1) / 2;               // of the join inside a CTA
+  static constexpr int PARTS = (WARPS + 1) / 2;               // of the join inside a CTA (TEAM)
+  static constexpr int JOIN_BYTES = TEAM ? PARTS * KvPartial<D, ROWS>::FLOATS * 4 : 0;
+  // Tiles of a warp's ring: what shared memory holds, at most 5.
+  static constexpr int FIT = (225 * 1024 - JOIN_BYTES - WARPS * (32 + 2 * 5 * 8)) / (WARPS * STAGE_BYTES);
+  static constexpr int STAGES = FIT < 5 ? FIT : 5;
   static constexpr int RING_BYTES = WARPS * STAGES * STAGE_BYTES;
-  static constexpr int JOIN_BYTES = SLOTS * KvPartial<D, ROWS>::FLOATS * 4;
   static constexpr int BAR_BYTES = 2 * WARPS * STAGES * 8;
   static constexpr int SMEM_BYTES = RING_BYTES + JOIN_BYTES + BAR_BYTES + WARPS * 32;
+  static_assert(STAGES >= 2 && SMEM_BYTES <= 232448 && BAR_BYTES % 16 == 0, "shared memory");
 };
 
 // Where a warp's range begins: unit (sequence b, head h), tile n, and how much
@@ -143,8 +147,8 @@ __device__ __forceinline__ void kv_value_pairs(uint32_t wa, uint32_t wb, __half2
 // hold few keys a sequence. Otherwise a worker is a warp (worker index =
 // warp * CTAs + CTA, so few workers spread over the SMs).
 template <int D, int BITS, int NT, bool TEAM>
-__global__ void __launch_bounds__(KvFew<D, BITS, NT>::THREADS, 1) kv_attention_few_kernel(const KvAttnArgs a) {
-  using Cfg = KvFew<D, BITS, NT>;
+__global__ void __launch_bounds__(KvFew<D, BITS, NT, TEAM>::THREADS, 1) kv_attention_few_kernel(const KvAttnArgs a) {
+  using Cfg = KvFew<D, BITS, NT, TEAM>;
   using Row = KvRow<D, BITS>;
   constexpr int W = Cfg::WARPS, ST = Cfg::STAGES, RB = Cfg::ROW_BYTES;
   constexpr int KC = D / 4;               // elements of a lane's share of a key row
@@ -264,11 +268,10 @@ __global__ void __launch_bounds__(KvFew<D, BITS, NT>::THREADS, 1) kv_attention_f
       if (copies > 1) page[1] = __ldg(t + 1);
     };
     if (have) look_up();
-    int issued = 0;
+    int issued = 0, st = 0, phase = 1;  // copies; the next one's slot and the parity of its last use
     uint64_t since = globaltimer_ns();
     while (__any_sync(0xffffffffu, have)) {
-      const int st = issued % ST;
-      const bool go = have && (issued < ST || mbar_test_wait(&my_empty[st], (issued / ST - 1) & 1));
+      const bool go = have && (issued < ST || mbar_test_wait(&my_empty[st], phase));
       if (go) {
         uint8_t* dst = ring + st * Cfg::STAGE_BYTES;
         const uint32_t bytes = static_cast<uint32_t>(chunk * RB);
@@ -290,6 +293,10 @@ __global__ void __launch_bounds__(KvFew<D, BITS, NT>::THREADS, 1) kv_attention_f
           }
         }
         ++issued;
+        if (++st == ST) {
+          st = 0;
+          phase ^= 1;
+        }
         if constexpr (TEAM) {
           p.n += W;
           if (p.n >= p.tiles) {
@@ -333,7 +340,7 @@ __global__ void __launch_bounds__(KvFew<D, BITS, NT>::THREADS, 1) kv_attention_f
   float raise[NT][2];        // the score above which the maximum is raised
   int limit[NT][2];
   int clear = 0;             // keys before this one are masked in no row
-  int used = 0;              // tiles consumed
+  int st = 0, phase = 0;     // the ring's next tile and its parity
   bool ok = true;
   const float sl2 = a.scale_log2, inv_sl2 = 1.0f / sl2;
   const uint32_t k1024 = __shfl_sync(0xffffffffu, a.k1024, 0);
@@ -385,7 +392,7 @@ __global__ void __launch_bounds__(KvFew<D, BITS, NT>::THREADS, 1) kv_attention_f
   };
 
   auto tile = [&](const Place& p) {
-    const uint8_t* sk = ring + (used % ST) * Cfg::STAGE_BYTES;
+    const uint8_t* sk = ring + st * Cfg::STAGE_BYTES;
     const uint8_t* sv = sk + KVF_TK * RB;
     const int key0 = p.n * KVF_TK;
     const bool masked = key0 + KVF_TK > clear;
@@ -517,15 +524,16 @@ __global__ void __launch_bounds__(KvFew<D, BITS, NT>::THREADS, 1) kv_attention_f
   };
   // Waits for the next tile, computes it and gives its stage back.
   auto take = [&](const Place& p) -> bool {
-    if (!mbar_try_wait(&my_full[used % ST], (used / ST) & 1) &&
-        !mbar_wait(&my_full[used % ST], (used / ST) & 1, wd, 110))
-      ok = false;
+    if (!mbar_try_wait(&my_full[st], phase) && !mbar_wait(&my_full[st], phase, wd, 110)) ok = false;
     ok = __all_sync(0xffffffffu, ok);
     if (!ok) return false;
     tile(p);
     __syncwarp();
-    if (lane == 0) mbar_arrive(&my_empty[used % ST]);
-    ++used;
+    if (lane == 0) mbar_arrive(&my_empty[st]);
+    if (++st == ST) {
+      st = 0;
+      phase ^= 1;
+    }
     return true;
   };
 
@@ -612,11 +620,11 @@ __global__ void __launch_bounds__(KvFew<D, BITS, NT>::THREADS, 1) kv_attention_f
           if (!take(at)) break;
         sum_l();
         // Two rounds: the upper half of the warps hands over to the lower, then
-        // all threads sum the lower half's slots.
+        // all threads sum the lower half's parts.
         constexpr int F = KvPartial<D, Cfg::ROWS>::FLOATS;
-        if (warp >= Cfg::SLOTS) store_partial(join + (warp - Cfg::SLOTS) * F, rows);
+        if (warp >= Cfg::PARTS) store_partial(join + (warp - Cfg::PARTS) * F, rows);
         named_barrier(1, W * 32);
-        if (warp + Cfg::SLOTS < W) {
+        if (warp + Cfg::PARTS < W) {
           const float* other = join + warp * F;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
@@ -636,16 +644,16 @@ __global__ void __launch_bounds__(KvFew<D, BITS, NT>::THREADS, 1) kv_attention_f
             }
         }
         __syncwarp();
-        if (warp < Cfg::SLOTS) store_partial(join + warp * F, rows);
+        if (warp < Cfg::PARTS) store_partial(join + warp * F, rows);
         named_barrier(1, W * 32);
         for (int i = threadIdx.x; i < rows * (D / 2); i += W * 32) {
           const int row = i / (D / 2), d = (i % (D / 2)) * 2;
           float mm = KV_NO_MAX;
 #pragma unroll
-          for (int k = 0; k < Cfg::SLOTS; ++k) mm = fmaxf(mm, join[k * F + Cfg::ROWS * D + 2 * row]);
+          for (int k = 0; k < Cfg::PARTS; ++k) mm = fmaxf(mm, join[k * F + Cfg::ROWS * D + 2 * row]);
           float ls = 0.f, x = 0.f, y = 0.f;
 #pragma unroll
-          for (int k = 0; k < Cfg::SLOTS; ++k) {
+          for (int k = 0; k < Cfg::PARTS; ++k) {
             const float f = kv_ex2(join[k * F + Cfg::ROWS * D + 2 * row] - mm);
             ls += f * join[k * F + Cfg::ROWS * D + 2 * row + 1];
             x += f * join[k * F + row * D + d];
@@ -658,7 +666,7 @@ __global__ void __launch_bounds__(KvFew<D, BITS, NT>::THREADS, 1) kv_attention_f
           *reinterpret_cast<__half2*>(o + d) = __floats2half2_rn(x * inv, y * inv);
           if (lse != nullptr && d == 0) *lse = (mm + log2f(ls)) * 0.6931471805599453f;
         }
-        named_barrier(1, W * 32);  // the slots are free for the next unit
+        named_barrier(1, W * 32);  // the parts are free for the next unit
       }
       next_unit(at, warp);
     }

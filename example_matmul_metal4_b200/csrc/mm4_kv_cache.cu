@@ -128,7 +128,7 @@ constexpr int kMaxCtas = 160;  // workspaces are sized for this many SMs
 
 template <int D, int BITS, int NT>
 size_t few_workspace() {
-  using Cfg = KvFew<D, BITS, NT>;
+  using Cfg = KvFew<D, BITS, NT, false>;
   return sizeof(float) * 2 * kMaxCtas * Cfg::WARPS * KvPartial<D, Cfg::ROWS>::FLOATS;
 }
 
@@ -146,10 +146,10 @@ Form attention_form(const mm4_kv_cache_plan* p, const mm4_kv_cache_batch* b) {
   const long long room = static_cast<long long>(b->pages_per_sequence) << p->page_shift;
   const bool eight = rows <= 8;
   f.kind = eight ? Form::FEW8 : Form::FEW16;
-  const int warps = p->d.head_dim == 128 && p->d.bits == 4 ? (eight ? KvFew<128, 4, 1>::WARPS : KvFew<128, 4, 2>::WARPS)
-                    : p->d.head_dim == 128                 ? (eight ? KvFew<128, 8, 1>::WARPS : KvFew<128, 8, 2>::WARPS)
-                    : p->d.bits == 4                       ? (eight ? KvFew<64, 4, 1>::WARPS : KvFew<64, 4, 2>::WARPS)
-                                                           : (eight ? KvFew<64, 8, 1>::WARPS : KvFew<64, 8, 2>::WARPS);
+  const int warps = p->d.head_dim == 128 && p->d.bits == 4 ? (eight ? KvFew<128, 4, 1, true>::WARPS : KvFew<128, 4, 2, true>::WARPS)
+                    : p->d.head_dim == 128                 ? (eight ? KvFew<128, 8, 1, true>::WARPS : KvFew<128, 8, 2, true>::WARPS)
+                    : p->d.bits == 4                       ? (eight ? KvFew<64, 4, 1, true>::WARPS : KvFew<64, 4, 2, true>::WARPS)
+                                                           : (eight ? KvFew<64, 8, 1, true>::WARPS : KvFew<64, 8, 2, true>::WARPS);
   f.team = room <= 2 * KVF_TK * warps;
   f.name = f.team ? (eight ? "kv_attention_few<8 rows, team>" : "kv_attention_few<16 rows, team>")
                   : (eight ? "kv_attention_few<8 rows, split>" : "kv_attention_few<16 rows, split>");
@@ -180,26 +180,19 @@ mm4_status launch_join(void (*kernel)(KvAttnArgs), dim3 grid, const KvAttnArgs& 
   return MM4_OK;
 }
 
-template <int D, int BITS, int NT>
-mm4_status launch_few(KvAttnArgs& a, bool team, int sms, cudaStream_t st) {
-  using Cfg = KvFew<D, BITS, NT>;
-  const void* kern = team ? reinterpret_cast<const void*>(kv_attention_few_kernel<D, BITS, NT, true>)
-                          : reinterpret_cast<const void*>(kv_attention_few_kernel<D, BITS, NT, false>);
-  mm4_status rc = ensure_smem_attr(kern, Cfg::SMEM_BYTES);
+template <int D, int BITS, int NT, bool TEAM>
+mm4_status launch_few(KvAttnArgs& a, int sms, cudaStream_t st) {
+  using Cfg = KvFew<D, BITS, NT, TEAM>;
+  mm4_status rc = ensure_smem_attr(reinterpret_cast<const void*>(kv_attention_few_kernel<D, BITS, NT, TEAM>),
+                                   Cfg::SMEM_BYTES);
   if (rc != MM4_OK) return rc;
-  if (team) {
-    const long long units = static_cast<long long>(a.kb.sequences) * a.kb.heads_kv;
-    const unsigned grid = static_cast<unsigned>(std::min<long long>(units, sms));
-    kv_attention_few_kernel<D, BITS, NT, true><<<grid, Cfg::THREADS, Cfg::SMEM_BYTES, st>>>(a);
-    cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return cuda_fail(e, "kv_attention_few_kernel launch");
-    return MM4_OK;
-  }
+  const long long units = static_cast<long long>(a.kb.sequences) * a.kb.heads_kv;
+  const unsigned grid = static_cast<unsigned>(TEAM ? std::min<long long>(units, sms) : sms);
   a.workers = sms * Cfg::WARPS;
-  kv_attention_few_kernel<D, BITS, NT, false><<<sms, Cfg::THREADS, Cfg::SMEM_BYTES, st>>>(a);
+  kv_attention_few_kernel<D, BITS, NT, TEAM><<<grid, Cfg::THREADS, Cfg::SMEM_BYTES, st>>>(a);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "kv_attention_few_kernel launch");
-  const long long units = static_cast<long long>(a.kb.sequences) * a.kb.heads_kv;
+  if (TEAM) return MM4_OK;
   return launch_join(kv_attention_join_kernel<D, Cfg::ROWS, KVF_TK>, dim3(static_cast<unsigned>(units), NT), a, st);
 }
 
@@ -382,8 +375,12 @@ mm4_status mm4_kv_cache_attention(const mm4_kv_cache_plan* p, const mm4_kv_cache
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int sms = std::min(info.sm_count, kMaxCtas);
   return by_row(p->d, [&](auto, auto D, auto B) -> mm4_status {
-    if (form.kind == Form::FEW8) return launch_few<D.value, B.value, 1>(a, form.team, sms, st);
-    if (form.kind == Form::FEW16) return launch_few<D.value, B.value, 2>(a, form.team, sms, st);
+    if (form.kind == Form::FEW8)
+      return form.team ? launch_few<D.value, B.value, 1, true>(a, sms, st)
+                       : launch_few<D.value, B.value, 1, false>(a, sms, st);
+    if (form.kind == Form::FEW16)
+      return form.team ? launch_few<D.value, B.value, 2, true>(a, sms, st)
+                       : launch_few<D.value, B.value, 2, false>(a, sms, st);
     if (form.kind == Form::MANY128) return launch_many<D.value, B.value, 1>(a, sms, st);
     return launch_many<D.value, B.value, 2>(a, sms, st);
   });

@@ -282,6 +282,29 @@ def test_long_axis_is_split_and_joined(cuda, new, length):
     s.check(*s.attend())
 
 
+@pytest.mark.parametrize("new,maxNew", [(1, 1), (2, 2), (5, 5)])
+def test_many_sequences_on_shared_pages(cuda, new, maxNew):
+    """600 sequences that share one prefix's pages: every worker's range crosses heads and sequences of more than
+    32 pages each, and page-table reads start over at each of them."""
+    import torch
+    Hq, Hk, D, page, longest = 8, 4, 64, 16, 800
+    base = Setup(cuda, [longest], [new], Hq, Hk, D=D, page=page)
+    B = 600
+    lengths = [520 + (37 * b) % 281 for b in range(B)]
+    offsets = np.arange(B + 1, dtype=np.int32) * new
+    Q = data.normal((B * new, Hq, D), 1.0, 9, 0)
+    batch = KVCacheBatch(torch.from_numpy(np.repeat(base.table, B, axis=0)).to(cuda),
+                         torch.tensor(lengths, dtype=torch.int32, device=cuda), torch.from_numpy(offsets).to(cuda),
+                         B * new, maxNew)
+    O = base.plan.attention(torch.from_numpy(Q).to(cuda), base.cache, batch)
+    sync_check()
+    got = O.double().cpu().numpy()
+    for b in range(0, B, 7):
+        r = slice(b * new, (b + 1) * new)
+        eO, _, tO, _ = ref.attention(Q[r], base.K[0][:lengths[b]], base.V[0][:lengths[b]], new, True, base.plan.scale)
+        assert (np.abs(got[r] - eO) <= tO).all(), b
+
+
 @pytest.mark.parametrize("new", [1, 5, 200])
 def test_repeated_calls_give_the_same_bits(cuda, new):
     import torch
