@@ -1,5 +1,6 @@
-// Attention over the key / value cache for few rows: up to 16 rows of a unit
-// (a token or a few, times the query heads that share a key / value head).
+// Attention over the key / value cache for few rows (a token or a few, times the
+// query heads that share a key / value head): units of 8, 16 or 24 rows, and
+// several units of 24 for up to 96 rows.
 //
 // Bound by the cache's bytes: each is read once, 160 a token and head at
 // D = 128 in 4 bits, and the arithmetic has to hide behind them: at 6.4 TB/s
@@ -10,8 +11,8 @@
 //    range of warp i, so finding places and page numbers costs one instruction
 //    stream for all of them.
 //  - S^T = K Q^T and O^T += V^T P^T on m16n8k16 tensor instructions, with the
-//    cache as the 16-row operand and the rows of Q as the 8 columns: half
-//    the tensor work of a form with 16 padded rows of Q.
+//    cache as the 16-row operand and the rows of Q as 8 columns, or 2 or 3
+//    times 8: unpacking the cache costs the same for any number of rows.
 //  - A lane takes the elements of one word for its share of the contraction
 //    (Q's fragments are built in the same order), so codes go from a word to
 //    operand registers by logic instructions and one fp16 fused multiply-add a
@@ -49,10 +50,10 @@ struct KvFew {
   static_assert(STAGES >= 2 && SMEM_BYTES <= 232448 && BAR_BYTES % 16 == 0, "shared memory");
 };
 
-// Where a warp's range begins: unit (sequence b, head h), tile n, and how much
-// there is (tiles, or units where a CTA takes whole units).
+// Where a warp's range begins: unit u (head, then row block) of sequence b,
+// tile n, and how much there is (tiles, or units where a CTA takes whole units).
 struct alignas(16) KvStart {
-  int b, h, n, pad;
+  int b, u, n, pad;
   long long todo;
 };
 
@@ -173,21 +174,23 @@ __global__ void __launch_bounds__(KvFew<D, BITS, NT, TEAM>::THREADS, 1) kv_atten
       const long long units = static_cast<long long>(kb.sequences) * kb.heads_kv;
       s.todo = (units - blockIdx.x + gridDim.x - 1) / gridDim.x;
       s.b = static_cast<int>(blockIdx.x / kb.heads_kv);
-      s.h = static_cast<int>(blockIdx.x % kb.heads_kv);
+      s.u = static_cast<int>(blockIdx.x % kb.heads_kv);
       s.n = warp;
     } else {
-      const long long total = kv_total_tiles<KVF_TK>(kb, lane) * kb.heads_kv;
+      constexpr int R = Cfg::ROWS;
+      const long long total = kv_total_tiles<KVF_TK, R>(kb, kb.sequences, a.group, lane) * kb.heads_kv;
       const long long active = min(static_cast<long long>(a.workers), total);
       const long long w = static_cast<long long>(warp) * gridDim.x + blockIdx.x;
       if (w < active) {
         const long long x = kv_range_begin(w, total, active);
         s.todo = kv_range_begin(w + 1, total, active) - x;
         long long before;
-        // Sequence b has heads * tiles(b) places on the line, from heads * before.
-        s.b = kv_find_tile<KVF_TK>(kb, x / kb.heads_kv, lane, &before);
-        const int tiles = s.b < kb.sequences ? max(1, kv_tiles<KVF_TK>(kv_sequence(kb, s.b))) : 1;
+        // Sequence b has heads * blocks * tiles places on the line, from heads *
+        // (those before it, for one head).
+        s.b = kv_find_tile<KVF_TK, R>(kb, x / kb.heads_kv, a.group, lane, &before);
+        const int tiles = s.b < kb.sequences ? kv_tiles<KVF_TK>(kv_sequence(kb, s.b)) : 1;
         const long long in = x - before * kb.heads_kv;
-        s.h = static_cast<int>(in / tiles);
+        s.u = static_cast<int>(in / tiles);
         s.n = static_cast<int>(in % tiles);
       }
     }
@@ -204,7 +207,7 @@ __global__ void __launch_bounds__(KvFew<D, BITS, NT, TEAM>::THREADS, 1) kv_atten
 
   // A place on the line, and the walk over units.
   struct Place {
-    int b, h, n, tiles;
+    int b, u, n, tiles, blocks;
     KvSequence s;
     long long todo;  // tiles left (TEAM: units)
   };
@@ -212,22 +215,27 @@ __global__ void __launch_bounds__(KvFew<D, BITS, NT, TEAM>::THREADS, 1) kv_atten
     const KvStart s = starts[w];
     Place p{};
     p.b = s.b;
-    p.h = s.h;
+    p.u = s.u;
     p.n = s.n;
     p.todo = s.todo;
     return p;
   };
+  auto read_sequence = [&](Place& p) {
+    p.s = kv_sequence(kb, p.b);
+    p.tiles = kv_tiles<KVF_TK>(p.s);
+    p.blocks = kv_blocks<Cfg::ROWS>(kb, p.s, a.group);
+  };
   auto next_unit = [&](Place& p, int w) {
     if constexpr (TEAM) {
-      const long long u = static_cast<long long>(p.b) * kb.heads_kv + p.h + gridDim.x;
+      const long long u = static_cast<long long>(p.b) * kb.heads_kv + p.u + gridDim.x;
       p.b = static_cast<int>(u / kb.heads_kv);
-      p.h = static_cast<int>(u % kb.heads_kv);
+      p.u = static_cast<int>(u % kb.heads_kv);
       p.n = w;
       --p.todo;
     } else {
       p.n = 0;
-      if (++p.h == kb.heads_kv) {
-        p.h = 0;
+      if (++p.u >= kb.heads_kv * p.blocks) {
+        p.u = 0;
         ++p.b;
       }
     }
@@ -236,13 +244,15 @@ __global__ void __launch_bounds__(KvFew<D, BITS, NT, TEAM>::THREADS, 1) kv_atten
   // TEAM a unit may end before this warp's first); false at the range's end.
   auto settle = [&](Place& p, int w) -> bool {
     while (p.todo > 0 && p.b < kb.sequences) {
-      p.s = kv_sequence(kb, p.b);
-      p.tiles = kv_tiles<KVF_TK>(p.s);
-      if (p.n < p.tiles) return true;
+      read_sequence(p);
+      if (p.blocks > 0 && p.n < p.tiles) return true;
       next_unit(p, w);
     }
     return false;
   };
+  // Head and first row of a unit.
+  auto head_of = [&](const Place& p) { return NT < 3 ? p.u : p.u / p.blocks; };
+  auto row_of = [&](const Place& p) { return NT < 3 ? 0 : (p.u % p.blocks) * Cfg::ROWS; };
 
   if (warp == W) {
     // ------------------------------------------------------------ copies
@@ -256,13 +266,14 @@ __global__ void __launch_bounds__(KvFew<D, BITS, NT, TEAM>::THREADS, 1) kv_atten
     if (lane >= W) p.todo = 0;
     bool have = settle(p, w);
     int page[2] = {0, 0};               // of the next tile
-    int copies = 0;
+    int copies = 0, head = 0;
     // Reads the page numbers of the next tile; they are looked at when it is
     // copied, so their latency is not waited for here.
     auto look_up = [&]() {
       const int key0 = p.n * KVF_TK;
       const int valid = p.s.len - key0;  // <= 0 only for a sequence of length 0
       copies = valid <= 0 ? 0 : (valid > chunk && chunk < KVF_TK) ? 2 : 1;
+      head = head_of(p);
       const int* t = kb.table + static_cast<long long>(p.b) * kb.pages_per_seq + (key0 >> kb.page_shift);
       if (copies > 0) page[0] = __ldg(t);
       if (copies > 1) page[1] = __ldg(t + 1);
@@ -286,7 +297,7 @@ __global__ void __launch_bounds__(KvFew<D, BITS, NT, TEAM>::THREADS, 1) kv_atten
               id = 0;  // read in place of the page outside the pool
             }
             const uint8_t* src = a.cache + id * kb.page_bytes +
-                                 (static_cast<long long>(p.h * 2 << kb.page_shift) + (p.n * KVF_TK & (ps - 1))) * RB;
+                                 (static_cast<long long>(head * 2 << kb.page_shift) + (p.n * KVF_TK & (ps - 1))) * RB;
             bulk_load(dst + i * chunk * RB, src, bytes, &my_full[st]);
             bulk_load(dst + (KVF_TK + i * chunk) * RB, src + (static_cast<long long>(RB) << kb.page_shift), bytes,
                       &my_full[st]);
@@ -345,17 +356,20 @@ __global__ void __launch_bounds__(KvFew<D, BITS, NT, TEAM>::THREADS, 1) kv_atten
   const float sl2 = a.scale_log2, inv_sl2 = 1.0f / sl2;
   const uint32_t k1024 = __shfl_sync(0xffffffffu, a.k1024, 0);
 
+  // Rows of the unit at p: at most ROWS, and none behind max_new tokens.
+  auto rows_of = [&](const Place& p) { return min(min(p.s.n, kb.max_new) * a.group - row_of(p), Cfg::ROWS); };
   auto start_unit = [&](const Place& p) {
-    const int rows = min(p.s.n * a.group, Cfg::ROWS);
-    if (static_cast<long long>(p.s.n) * a.group > Cfg::ROWS || p.s.n > kb.max_new) kv_note(KV_DATA_NEW);
+    const int row0 = row_of(p), rows = rows_of(p);
+    if (p.s.n > kb.max_new) kv_note(KV_DATA_NEW);
+    const int head0 = head_of(p) * a.group;
     clear = p.s.len;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int r = nt * 8 + g;
       const bool have = r < rows;
-      const int tok = have ? r / a.group : 0, hd = have ? r % a.group : 0;
+      const int tok = have ? (row0 + r) / a.group : 0, hd = have ? (row0 + r) % a.group : 0;
       const uint4* src = reinterpret_cast<const uint4*>(
-          a.Q + (p.s.first + tok) * a.q_stride + static_cast<long long>(p.h * a.group + hd) * D + c * KC);
+          a.Q + (p.s.first + tok) * a.q_stride + static_cast<long long>(head0 + hd) * D + c * KC);
       uint4 v[KC / 8];
 #pragma unroll
       for (int i = 0; i < KC / 8; ++i) v[i] = have ? __ldg(src + i) : make_uint4(0u, 0u, 0u, 0u);
@@ -376,7 +390,7 @@ __global__ void __launch_bounds__(KvFew<D, BITS, NT, TEAM>::THREADS, 1) kv_atten
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int row = nt * 8 + 2 * c + e;
-        limit[nt][e] = row < rows ? kv_limit(p.s, row / a.group, a.causal) : p.s.len;
+        limit[nt][e] = row < rows ? kv_limit(p.s, (row0 + row) / a.group, a.causal) : p.s.len;
         clear = min(clear, limit[nt][e]);
         m[nt][e] = KV_NO_MAX;
         raise[nt][e] = -INFINITY;
@@ -567,8 +581,9 @@ __global__ void __launch_bounds__(KvFew<D, BITS, NT, TEAM>::THREADS, 1) kv_atten
       }
   };
   auto output_row = [&](const Place& p, int row, __half** o, float** lse) {
+    row += row_of(p);
     const long long tok = p.s.first + row / a.group;
-    const int head = p.h * a.group + row % a.group;
+    const int head = head_of(p) * a.group + row % a.group;
     *o = a.O + tok * a.o_stride + static_cast<long long>(head) * D;
     *lse = a.lse ? a.lse + tok * a.heads_q + head : nullptr;
   };
@@ -583,7 +598,7 @@ __global__ void __launch_bounds__(KvFew<D, BITS, NT, TEAM>::THREADS, 1) kv_atten
         if (!take(at)) break;
       at.todo -= n1 - n0;
       sum_l();
-      const int rows = min(at.s.n * a.group, Cfg::ROWS);
+      const int rows = rows_of(at);
       if (n0 == 0 && n1 == at.tiles) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -611,10 +626,9 @@ __global__ void __launch_bounds__(KvFew<D, BITS, NT, TEAM>::THREADS, 1) kv_atten
     }
   } else {
     while (at.todo > 0) {  // every computing warp of the CTA walks the same units
-      at.s = kv_sequence(kb, at.b);
-      at.tiles = kv_tiles<KVF_TK>(at.s);
-      if (at.tiles > 0) {
-        const int rows = min(at.s.n * a.group, Cfg::ROWS);
+      read_sequence(at);
+      if (at.blocks > 0) {
+        const int rows = rows_of(at);
         start_unit(at);
         for (; ok && at.n < at.tiles; at.n += W)
           if (!take(at)) break;
@@ -686,14 +700,16 @@ __global__ void __launch_bounds__(256) kv_attention_join_kernel(const KvAttnArgs
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = static_cast<int>(blockIdx.x / kb.heads_kv), h = static_cast<int>(blockIdx.x % kb.heads_kv);
   const KvSequence s = kv_sequence(kb, b);
-  const int row0 = blockIdx.y * 8;
-  const int rows = min(min(s.n * a.group, ROWS) - row0, 8);
-  const long long total = kv_total_tiles<TK>(kb, lane) * kb.heads_kv;
+  const int blocks = kv_blocks<ROWS>(kb, s, a.group), block = blockIdx.y / (ROWS / 8);
+  const int row0 = blockIdx.y % (ROWS / 8) * 8;  // in the unit
+  const int rows = min(min(min(s.n, kb.max_new) * a.group - block * ROWS, ROWS) - row0, 8);
+  const long long total = kv_total_tiles<TK, ROWS>(kb, kb.sequences, a.group, lane) * kb.heads_kv;
   const long long active = min(static_cast<long long>(a.workers), total);
   const int tiles = kv_tiles<TK>(s);
   long long first = 0, last = 0;
   if (rows > 0) {
-    const long long x0 = kv_tiles_before<TK>(kb, b, lane) * kb.heads_kv + static_cast<long long>(h) * tiles;
+    const long long x0 = kv_total_tiles<TK, ROWS>(kb, b, a.group, lane) * kb.heads_kv +
+                         (static_cast<long long>(h) * blocks + block) * tiles;
     first = kv_worker_of(x0, total, active);
     last = kv_worker_of(x0 + tiles - 1, total, active);
   }
@@ -767,7 +783,7 @@ __global__ void __launch_bounds__(256) kv_attention_join_kernel(const KvAttnArgs
     }
   }
   if (mine == 0 && row < rows) {
-    const int r = row0 + row;
+    const int r = block * ROWS + row0 + row;
     const long long tok = s.first + r / a.group;
     const int head = h * a.group + r % a.group;
     const float inv = ls > 0.f ? 1.0f / ls : 0.f;

@@ -4,23 +4,24 @@
 // Bound by the tensor cores and the exponentials, as attention over fp16 K and
 // V is (4 D FLOP and one exponential per row and key); what the cache adds is
 // turning its codes into fp16 operands. That is done once per 64 keys for all
-// 128 x QT rows of a CTA by warps of its own, into the 128-byte-swizzled layout
+// 256 rows of a CTA by warps of its own, into the 128-byte-swizzled layout
 // that tcgen05.mma reads, and overlaps the products of earlier keys.
 //
 // A row is one query head of one token, rows of a unit ordered by token and
 // then head, so grouped heads fill the 128-row tiles and share the unpacked
-// keys. A unit is one key / value head of one sequence and 128 QT rows. 16 warps:
+// keys. A unit is one key / value head of one sequence and 256 rows, two tiles of
+// 128. 16 warps:
 //   warp 0        copies pages as they lie in the cache into a ring (untiled bulk
 //                 copies).
 //   warp 1        TMEM allocation; one lane issues S_i(g) = Q_i K(g)^T (M = 128,
 //                 N = 64) into slot g % 2 of row tile i.
 //   warp 2        one lane issues O_i += P_i(g) V(g) (P from TMEM).
 //   warp 3        finds the CTA's range.
-//   QT x 4 warps  softmax, one row a thread: P = 2^(S scale log2 e - m), rescaling
+//   warps 4-11    softmax, one row a thread: P = 2^(S scale log2 e - m), rescaling
 //                 O only when the maximum grew by more than 2^8; results out. A
 //                 thread also copies its row of the next unit's Q, as soon as it has
 //                 the last scores of the unit, so the copy overlaps the results.
-//   the others    codes to fp16: a lane takes 32 elements (one scale and zero).
+//   warps 12-15   codes to fp16: a lane takes 32 elements (one scale and zero).
 // TMEM: two 64-column S slots for each row tile, then O_i (D columns each). Steps
 // of 64 keys are counted across a CTA's units (g), which fixes slots and
 // mbarrier phases; S runs two steps ahead of the softmax.
@@ -39,8 +40,9 @@ constexpr int KVM_THREADS = 512;
 // each, would take twice the time of the last ones.
 constexpr int KVM_UNIT = 4;
 
-template <int D, int BITS, int QT>
+template <int D, int BITS>
 struct KvMany {
+  static constexpr int QT = 2;                         // row tiles of 128
   static constexpr int ROWS = 128 * QT;
   static constexpr int Q_BYTES = 128 * D * 2;          // a row tile of Q
   static constexpr int TILE_BYTES = KVM_TK * D * 2;    // unpacked K or V of a step
@@ -52,14 +54,12 @@ struct KvMany {
   static constexpr int OUT_OFFSET = QT * Q_BYTES + (KS + VS) * TILE_BYTES + RS * RAW_BYTES;
   static constexpr int BAR_OFFSET = OUT_OFFSET + 4 * QT * OUT_BYTES;
   static constexpr int SMEM_BYTES = BAR_OFFSET + 512 + 1024;
-  // Four warps unpack K and V in turn; with one row tile, four each.
-  static constexpr int UNPACK_WARPS = 12 - 4 * QT;
   // Registers: 128 threads each of warps 0-3, the softmax warps and the
   // unpacking warps; the sum must not exceed what the block is launched with.
   static constexpr int REGS_LOW = 96;
   static constexpr int REGS_SOFTMAX = 160;
-  static constexpr int REGS_UNPACK = QT == 2 ? 96 : 128;
-  static constexpr int REGS_NEEDED = (REGS_LOW + QT * REGS_SOFTMAX + (3 - QT) * REGS_UNPACK) / 4;
+  static constexpr int REGS_UNPACK = 96;
+  static constexpr int REGS_NEEDED = (REGS_LOW + 2 * REGS_SOFTMAX + REGS_UNPACK) / 4;
   static_assert(REGS_NEEDED <= 128, "register split");
   static_assert(SMEM_BYTES <= 232448, "shared memory");
 };
@@ -283,16 +283,15 @@ __device__ __forceinline__ float kvm_exp_store64(const float (&x)[64], float sl2
   return sum.x + sum.y;
 }
 
-template <int D, int BITS, int QT>
+template <int D, int BITS>
 __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const __grid_constant__ KvAttnArgs a) {
-  using Cfg = KvMany<D, BITS, QT>;
+  using Cfg = KvMany<D, BITS>;
   using Row = KvRow<D, BITS>;
-  constexpr int ROWS = Cfg::ROWS, KS = Cfg::KS, VS = Cfg::VS, RS = Cfg::RS, RB = Row::BYTES;
+  constexpr int QT = Cfg::QT, ROWS = Cfg::ROWS, KS = Cfg::KS, VS = Cfg::VS, RS = Cfg::RS, RB = Row::BYTES;
   constexpr int TB = Cfg::TILE_BYTES, QB = Cfg::Q_BYTES;
   constexpr uint32_t IDESC_S = idesc_f16_f32(128, KVM_TK, false, false);
   constexpr uint32_t IDESC_O = idesc_f16_f32(128, D, false, true);
   constexpr int EMU = AttFwdCfg<D>::EMU_PER8;
-  constexpr bool TURNS = QT == 2;
 
   extern __shared__ uint8_t kvm_smem_raw[];
   const uint32_t raw_addr = smem_u32(kvm_smem_raw);
@@ -347,7 +346,7 @@ __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const
     }
     for (int i = 0; i < RS; ++i) {
       mbar_init(&r_full[i], 1);
-      mbar_init(&r_empty[i], Cfg::UNPACK_WARPS);
+      mbar_init(&r_empty[i], 4);
     }
     fence_mbar_init();
   }
@@ -604,14 +603,12 @@ __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const
         // The two row tiles' warps of an SM quarter take turns at the
         // exponentials: at the same time each would take twice as long, and
         // neither would load scores or find maxima meanwhile.
-        if (TURNS) {
-          if (ti == 1 || g > 0)
-            ok = mbar_wait(&turn[(1 - ti) * 4 + q], (ti == 1 ? g : g - 1) & 1, wd, SITE_KVM_SOFTMAX);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-        }
+        if (ti == 1 || g > 0)
+          ok = mbar_wait(&turn[(1 - ti) * 4 + q], (ti == 1 ? g : g - 1) & 1, wd, SITE_KVM_SOFTMAX);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
         const float part = kvm_exp_store64<EMU>(x, sl2, m, tSl, [&] {
-          if (TURNS && lane == 0) mbar_arrive(&turn[ti * 4 + q]);
+          if (lane == 0) mbar_arrive(&turn[ti * 4 + q]);
         });
         l += part;
         tmem_st_wait();
@@ -707,8 +704,7 @@ __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const
     constexpr int GR = D / KV_GROUP;          // groups of a row
     constexpr int RW = 32 / GR;               // rows of a warp at a time
     constexpr int PASSES = KVM_TK / (RW * 4);
-    const int uw = (warp - (16 - Cfg::UNPACK_WARPS)) & 3;
-    const int kv0 = QT == 1 ? (warp - (16 - Cfg::UNPACK_WARPS)) >> 2 : 0, kv1 = QT == 1 ? kv0 : 1;
+    const int uw = warp - 12;
     // Eight lanes take eight rows and one group: the row pitches (80, 144, 40,
     // 72 bytes) and the swizzle then put their accesses on different banks.
     const int sub = (lane & 7) + 8 * (lane / (8 * GR));
@@ -736,7 +732,6 @@ __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const
         const bool tail = valid < KVM_TK;
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
-          if (kv < kv0 || kv > kv1) continue;
           const int depth = kv == 0 ? KS : VS;
           if (ok && g >= depth)
             ok = mbar_wait(kv == 0 ? &k_empty[ks] : &v_empty[vs], (g / depth - 1) & 1, wd, SITE_KVM_UNPACK);

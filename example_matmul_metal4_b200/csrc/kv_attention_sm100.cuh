@@ -53,34 +53,44 @@ struct KvPartial {
 
 constexpr float KV_NO_MAX = -1e30f;  // running maximum of a row that has seen no key
 
-// Tiles of TK keys of sequence b (0 if it has no rows in this call; a row
-// block with no key still takes one tile, which writes its zeros).
+// Tiles of TK keys of a sequence (at least one: a row block with no key still
+// takes a tile, which writes its zeros), and its row blocks of ROWS rows (none if
+// it has no rows in this call). Blocks of few rows walk all tiles alike.
 template <int TK>
 __device__ __forceinline__ int kv_tiles(const KvSequence& s) {
-  return s.n == 0 ? 0 : max(1, (s.len + TK - 1) / TK);
+  return max(1, (s.len + TK - 1) / TK);
+}
+template <int ROWS>
+__device__ __forceinline__ int kv_blocks(const KvBatch& kb, const KvSequence& s, int group) {
+  return (min(s.n, kb.max_new) * group + ROWS - 1) / ROWS;
+}
+template <int TK, int ROWS>
+__device__ __forceinline__ int kv_sequence_tiles(const KvBatch& kb, int b, int group) {
+  const KvSequence s = kv_sequence(kb, b);
+  return kv_tiles<TK>(s) * kv_blocks<ROWS>(kb, s, group);
 }
 
-// Sum of kv_tiles over all sequences, by one warp.
-template <int TK>
-__device__ __forceinline__ long long kv_total_tiles(const KvBatch& kb, int lane) {
+// Sum of kv_sequence_tiles over the first n sequences, by one warp.
+template <int TK, int ROWS>
+__device__ __forceinline__ long long kv_total_tiles(const KvBatch& kb, int n, int group, int lane) {
   long long sum = 0;
-  for (int b = lane; b < kb.sequences; b += 32) sum += kv_tiles<TK>(kv_sequence(kb, b));
+  for (int b = lane; b < n; b += 32) sum += kv_sequence_tiles<TK, ROWS>(kb, b, group);
 #pragma unroll
   for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
   return sum;
 }
 
 // Sequence b whose tiles hold x (x < the total), and the tiles before it.
-template <int TK>
-__device__ __forceinline__ int kv_find_tile(const KvBatch& kb, long long x, int lane, long long* before) {
+template <int TK, int ROWS>
+__device__ __forceinline__ int kv_find_tile(const KvBatch& kb, long long x, int group, int lane, long long* before) {
   long long done = 0;
   for (int b0 = 0; b0 < kb.sequences; b0 += 32) {
     const int b = b0 + lane;
-    const int t = b < kb.sequences ? kv_tiles<TK>(kv_sequence(kb, b)) : 0;
-    int inc = t;
+    const int t = b < kb.sequences ? kv_sequence_tiles<TK, ROWS>(kb, b, group) : 0;
+    long long inc = t;
 #pragma unroll
     for (int s = 1; s < 32; s <<= 1) {
-      const int up = __shfl_up_sync(0xffffffffu, inc, s);
+      const long long up = __shfl_up_sync(0xffffffffu, inc, s);
       if (lane >= s) inc += up;
     }
     const unsigned over = __ballot_sync(0xffffffffu, done + inc > x);
@@ -93,16 +103,6 @@ __device__ __forceinline__ int kv_find_tile(const KvBatch& kb, long long x, int 
   }
   *before = done;
   return kb.sequences;  // not reached for x < the total
-}
-
-// Tiles of all sequences before b, by one warp.
-template <int TK>
-__device__ __forceinline__ long long kv_tiles_before(const KvBatch& kb, int b, int lane) {
-  long long sum = 0;
-  for (int i = lane; i < b; i += 32) sum += kv_tiles<TK>(kv_sequence(kb, i));
-#pragma unroll
-  for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
-  return sum;
 }
 
 // Keys that row r of a unit sees: those before limit (<= 0: none).

@@ -116,51 +116,45 @@ mm4_status launch_io(const mm4_kv_cache_plan* p, KvIoArgs& a, bool write, cudaSt
 }
 
 // Which kernel attention over a batch runs, from its sizes alone (the lengths
-// lie on the device).
+// lie on the device). Rows are the most that one key / value head has in one
+// sequence: max_new tokens times the query heads that share it.
+//   FEW    up to 8, 16 or 24 rows of a unit, and 4 units of 24 rows: a 32-key tile
+//          costs an SM about 250 clocks for each 24 rows.
+//   MANY   more than 96 rows: about 1050 clocks for up to 256 rows.
+//   TEAM   FEW of at most 16 rows, if no sequence can hold more than two tiles a
+//          warp: whole units to a CTA, one launch (13 us against 17 for a call
+//          alone).
 struct Form {
-  enum Kind { FEW8, FEW16, MANY128, MANY256 } kind;
-  bool team;         // FEW: whole units to a CTA, one launch
+  enum Kind { FEW8, FEW16, FEW24, MANY } kind;
+  bool team;
   size_t workspace;
   const char* name;
 };
 
-constexpr int kMaxCtas = 160;  // workspaces are sized for this many SMs
-
-template <int D, int BITS, int NT>
-size_t few_workspace() {
-  using Cfg = KvFew<D, BITS, NT, false>;
-  return sizeof(float) * 2 * kMaxCtas * Cfg::WARPS * KvPartial<D, Cfg::ROWS>::FLOATS;
-}
+constexpr int kMaxCtas = 160;    // workspaces are sized for this many SMs
+constexpr int kFewRows = 96;     // the most rows that FEW takes
+constexpr int kTeamTokens = 448;  // the most tokens of a sequence for TEAM: 2 tiles of 32 for each of 7 warps
 
 Form attention_form(const mm4_kv_cache_plan* p, const mm4_kv_cache_batch* b) {
   const int group = p->d.heads_q / p->d.heads_kv;
   const long long rows = static_cast<long long>(b->max_new) * group;
+  const long long room = static_cast<long long>(b->pages_per_sequence) << p->page_shift;
   Form f{};
-  if (rows > 16) {
-    f.kind = rows <= 128 ? Form::MANY128 : Form::MANY256;
-    const int tile = rows <= 128 ? 128 : 256;
-    f.workspace = sizeof(float) * 2 * kMaxCtas * tile * (p->d.head_dim + 2);
-    f.name = rows <= 128 ? "kv_attention_many<128 rows>" : "kv_attention_many<256 rows>";
+  if (rows > kFewRows) {
+    f.kind = Form::MANY;
+    f.workspace = sizeof(float) * 2 * kMaxCtas * 256 * (p->d.head_dim + 2);
+    f.name = "kv_attention_many";
     return f;
   }
-  const long long room = static_cast<long long>(b->pages_per_sequence) << p->page_shift;
-  const bool eight = rows <= 8;
-  f.kind = eight ? Form::FEW8 : Form::FEW16;
-  const int warps = p->d.head_dim == 128 && p->d.bits == 4 ? (eight ? KvFew<128, 4, 1, true>::WARPS : KvFew<128, 4, 2, true>::WARPS)
-                    : p->d.head_dim == 128                 ? (eight ? KvFew<128, 8, 1, true>::WARPS : KvFew<128, 8, 2, true>::WARPS)
-                    : p->d.bits == 4                       ? (eight ? KvFew<64, 4, 1, true>::WARPS : KvFew<64, 4, 2, true>::WARPS)
-                                                           : (eight ? KvFew<64, 8, 1, true>::WARPS : KvFew<64, 8, 2, true>::WARPS);
-  f.team = room <= 2 * KVF_TK * warps;
-  f.name = f.team ? (eight ? "kv_attention_few<8 rows, team>" : "kv_attention_few<16 rows, team>")
-                  : (eight ? "kv_attention_few<8 rows, split>" : "kv_attention_few<16 rows, split>");
-  if (!f.team) {
-    if (p->d.head_dim == 128)
-      f.workspace = p->d.bits == 4 ? (eight ? few_workspace<128, 4, 1>() : few_workspace<128, 4, 2>())
-                                   : (eight ? few_workspace<128, 8, 1>() : few_workspace<128, 8, 2>());
-    else
-      f.workspace = p->d.bits == 4 ? (eight ? few_workspace<64, 4, 1>() : few_workspace<64, 4, 2>())
-                                   : (eight ? few_workspace<64, 8, 1>() : few_workspace<64, 8, 2>());
-  }
+  f.kind = rows <= 8 ? Form::FEW8 : rows <= 16 ? Form::FEW16 : Form::FEW24;
+  f.team = rows <= 16 && room <= kTeamTokens;
+  const int nt = rows <= 8 ? 1 : rows <= 16 ? 2 : 3;
+  const int warps = nt == 1 ? 14 : 7;  // at most
+  if (!f.team) f.workspace = sizeof(float) * 2 * kMaxCtas * warps * 8 * nt * (p->d.head_dim + 2);
+  static const char* const names[3][2] = {{"kv_attention_few<8 rows, split>", "kv_attention_few<8 rows, team>"},
+                                          {"kv_attention_few<16 rows, split>", "kv_attention_few<16 rows, team>"},
+                                          {"kv_attention_few<24 rows, split>", ""}};
+  f.name = names[nt - 1][f.team ? 1 : 0];
   return f;
 }
 
@@ -182,24 +176,26 @@ mm4_status launch_join(void (*kernel)(KvAttnArgs), dim3 grid, const KvAttnArgs& 
 
 template <int D, int BITS, int NT, bool TEAM>
 mm4_status launch_few(KvAttnArgs& a, int sms, cudaStream_t st) {
+  const int blocks = (a.kb.max_new * a.group + 8 * NT - 1) / (8 * NT);
   using Cfg = KvFew<D, BITS, NT, TEAM>;
   mm4_status rc = ensure_smem_attr(reinterpret_cast<const void*>(kv_attention_few_kernel<D, BITS, NT, TEAM>),
                                    Cfg::SMEM_BYTES);
   if (rc != MM4_OK) return rc;
   const long long units = static_cast<long long>(a.kb.sequences) * a.kb.heads_kv;
   const unsigned grid = static_cast<unsigned>(TEAM ? std::min<long long>(units, sms) : sms);
+  static_assert(Cfg::WARPS <= (NT == 1 ? 14 : 7), "attention_form sizes the workspace for this many");
   a.workers = sms * Cfg::WARPS;
   kv_attention_few_kernel<D, BITS, NT, TEAM><<<grid, Cfg::THREADS, Cfg::SMEM_BYTES, st>>>(a);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "kv_attention_few_kernel launch");
   if (TEAM) return MM4_OK;
-  return launch_join(kv_attention_join_kernel<D, Cfg::ROWS, KVF_TK>, dim3(static_cast<unsigned>(units), NT), a, st);
+  return launch_join(kv_attention_join_kernel<D, Cfg::ROWS, KVF_TK>, dim3(static_cast<unsigned>(units), NT * blocks), a, st);
 }
 
-template <int D, int BITS, int QT>
+template <int D, int BITS>
 mm4_status launch_many(KvAttnArgs& a, int sms, cudaStream_t st) {
-  using Cfg = KvMany<D, BITS, QT>;
-  const void* kern = reinterpret_cast<const void*>(kv_attention_many_kernel<D, BITS, QT>);
+  using Cfg = KvMany<D, BITS>;
+  const void* kern = reinterpret_cast<const void*>(kv_attention_many_kernel<D, BITS>);
   mm4_status rc = ensure_smem_attr(kern, Cfg::SMEM_BYTES);
   if (rc != MM4_OK) return rc;
   {
@@ -214,7 +210,7 @@ mm4_status launch_many(KvAttnArgs& a, int sms, cudaStream_t st) {
                   Cfg::REGS_NEEDED);
   }
   a.workers = sms;
-  kv_attention_many_kernel<D, BITS, QT><<<sms, KVM_THREADS, Cfg::SMEM_BYTES, st>>>(a);
+  kv_attention_many_kernel<D, BITS><<<sms, KVM_THREADS, Cfg::SMEM_BYTES, st>>>(a);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "kv_attention_many_kernel launch");
   if (sms < 2) return MM4_OK;
@@ -381,8 +377,8 @@ mm4_status mm4_kv_cache_attention(const mm4_kv_cache_plan* p, const mm4_kv_cache
     if (form.kind == Form::FEW16)
       return form.team ? launch_few<D.value, B.value, 2, true>(a, sms, st)
                        : launch_few<D.value, B.value, 2, false>(a, sms, st);
-    if (form.kind == Form::MANY128) return launch_many<D.value, B.value, 1>(a, sms, st);
-    return launch_many<D.value, B.value, 2>(a, sms, st);
+    if (form.kind == Form::FEW24) return launch_few<D.value, B.value, 3, false>(a, sms, st);
+    return launch_many<D.value, B.value>(a, sms, st);
   });
 }
 
