@@ -688,7 +688,7 @@ __global__ void __launch_bounds__(KvFew<D, BITS, NT, TEAM>::THREADS, 1) kv_atten
 }
 
 // Joins the partials of the units that several workers share: a block of 8
-// warps per unit and 8 rows, (row, part of the partials) to a warp, parts
+// warps per unit and join_rows rows, (row, part of the partials) to a warp, parts
 // joined in shared memory in order. Launched to overlap the tail of the
 // kernel before it, which it waits for before it reads a partial.
 template <int D, int ROWS, int TK>
@@ -700,9 +700,10 @@ __global__ void __launch_bounds__(256) kv_attention_join_kernel(const KvAttnArgs
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = static_cast<int>(blockIdx.x / kb.heads_kv), h = static_cast<int>(blockIdx.x % kb.heads_kv);
   const KvSequence s = kv_sequence(kb, b);
-  const int blocks = kv_blocks<ROWS>(kb, s, a.group), block = blockIdx.y / (ROWS / 8);
-  const int row0 = blockIdx.y % (ROWS / 8) * 8;  // in the unit
-  const int rows = min(min(min(s.n, kb.max_new) * a.group - block * ROWS, ROWS) - row0, 8);
+  const int chunks = (min(ROWS, kb.max_new * a.group) + a.join_rows - 1) / a.join_rows;  // of a row block
+  const int blocks = kv_blocks<ROWS>(kb, s, a.group), block = blockIdx.y / chunks;
+  const int row0 = blockIdx.y % chunks * a.join_rows;  // in the unit
+  const int rows = min(min(min(s.n, kb.max_new) * a.group - block * ROWS, ROWS) - row0, a.join_rows);
   const long long total = kv_total_tiles<TK, ROWS>(kb, kb.sequences, a.group, lane) * kb.heads_kv;
   const long long active = min(static_cast<long long>(a.workers), total);
   const int tiles = kv_tiles<TK>(s);

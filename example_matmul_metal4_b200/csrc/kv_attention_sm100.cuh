@@ -31,6 +31,7 @@ struct KvAttnArgs {
   float scale_log2;      // scale * log2(e)
   float* partials;       // workspace
   int workers;           // of the launch
+  int join_rows;         // few rows: rows of a unit to a block of the join
   uint32_t k1024;        // KV_1024
   unsigned long long timeout_ns;
 };

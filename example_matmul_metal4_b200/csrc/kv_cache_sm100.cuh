@@ -72,46 +72,42 @@ __device__ __forceinline__ KvSequence kv_sequence(const KvBatch& kb, int b) {
   return s;
 }
 
-// The sequence whose rows hold row t (all lanes of the warp call it with the
-// same t): a 32-way search of the ascending offsets, two steps for up to 1024
-// sequences, then a check, so offsets that are out of order find nothing
-// rather than something wrong. -1 for padding rows.
-__device__ __forceinline__ int kv_find_sequence(const KvBatch& kb, int t, int lane) {
-  int lo = 0, n = kb.sequences;
-  while (n > 1) {
-    const int step = (n + 31) / 32;
-    const int probe = lane * step;
-    const unsigned hit = __ballot_sync(0xffffffffu, probe < n && __ldg(kb.offsets + lo + probe) <= t);
-    if (hit == 0) return -1;
-    const int k = (31 - __clz(hit)) * step;
-    lo += k;
-    n = min(step, n - k);
+// The sequence whose rows hold row t: a binary search of the ascending offsets,
+// then a check, so offsets that are out of order find nothing rather than
+// something wrong. -1 for padding rows.
+__device__ __forceinline__ int kv_find_sequence(const KvBatch& kb, int t) {
+  int lo = 0, hi = kb.sequences;  // offsets[lo] <= t is assumed, offsets[hi] > t or hi = sequences
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (__ldg(kb.offsets + mid) <= t)
+      lo = mid;
+    else
+      hi = mid;
   }
   const int first = __ldg(kb.offsets + lo), end = __ldg(kb.offsets + lo + 1);
   if (end < first) kv_note(KV_DATA_OFFSETS);
   return first <= t && t < end ? lo : -1;
 }
 
-// Address of the K rows of one token's page and head 0, plus its row number;
-// nullptr if the row has no place (padding, before position 0, beyond the page
-// table, a page outside the pool).
-__device__ __forceinline__ uint8_t* kv_place(const KvBatch& kb, uint8_t* cache, int t, int lane, int* row) {
-  const int b = kv_find_sequence(kb, t, lane);
-  if (b < 0) return nullptr;
+// Where the K row of token t lies for head 0, as an offset into the cache; -1 if
+// the row has no place (padding, before position 0, beyond the page table, a
+// page outside the pool).
+__device__ __forceinline__ long long kv_place(const KvBatch& kb, int t, int row_bytes) {
+  const int b = kv_find_sequence(kb, t);
+  if (b < 0) return -1;
   const int end = __ldg(kb.offsets + b + 1);
   const int len = __ldg(kb.lengths + b);
   const long long pos = static_cast<long long>(len) - (end - t);
   const int room = kb.pages_per_seq << kb.page_shift;
   if (len < 0 || len > room) kv_note(KV_DATA_LENGTH);
-  if (pos < 0 || pos >= room) return nullptr;
+  if (pos < 0 || pos >= room) return -1;
   const int p = static_cast<int>(pos);
   const int page = __ldg(kb.table + static_cast<long long>(b) * kb.pages_per_seq + (p >> kb.page_shift));
   if (page < 0 || page >= kb.pages) {
     kv_note(KV_DATA_PAGE);
-    return nullptr;
+    return -1;
   }
-  *row = p & ((1 << kb.page_shift) - 1);
-  return cache + page * kb.page_bytes;
+  return page * kb.page_bytes + static_cast<long long>(p & ((1 << kb.page_shift) - 1)) * row_bytes;
 }
 
 // ---------------------------------------------------------------------------
@@ -156,8 +152,8 @@ __device__ __forceinline__ __half2 kv_codes8(uint32_t w, uint32_t selector) {
 // ---------------------------------------------------------------------------
 
 constexpr int KV_IO_WARPS = 4;                // warps of a block
-constexpr int KV_IO_VECS = 4;                 // 8-element vectors of a lane, all in flight
-constexpr int KV_IO_PART = 32 * KV_IO_VECS;   // vectors of a warp
+constexpr int KV_IO_VECS = 4;                 // 8-element vectors of a lane and token, all in flight
+constexpr int KV_IO_PART = 32 * KV_IO_VECS;   // vectors of a warp and token
 
 struct KvIoArgs {
   KvBatch kb;
@@ -167,89 +163,158 @@ struct KvIoArgs {
   __half* out_v;
   long long k_stride, v_stride;
   uint8_t* cache;
-  int parts;            // warps of one token
+  int parts;            // warps that share a token
+  int tokens_per_warp;  // 1 .. 32: looked up by a lane each, so that their places cost one latency
 };
 
-// Quantises one token's K and V. A warp takes 128 vectors of 8 elements (of the
-// 2 * heads_kv * D / 8 that a token has, K first), four to a lane; the four
-// lanes of a group of 32 elements find its minimum and maximum by two
-// shuffles. Bound by the bytes it moves: 512 in and 160 out per token and head
-// at D = 128 in 4 bits.
+// The work of a warp: tokens t0 .. t0 + n - 1 (lane i has the place of token
+// t0 + i), vectors vec0 + 32 i. False if it has none.
+struct KvIoWork {
+  int t0, n, vec0;
+  long long place;
+};
+template <int ROW_BYTES>
+__device__ __forceinline__ bool kv_io_work(const KvIoArgs& a, int lane, KvIoWork* w) {
+  const long long id = static_cast<long long>(blockIdx.x) * KV_IO_WARPS + (threadIdx.x >> 5);
+  const long long t0 = id / a.parts * a.tokens_per_warp;
+  if (t0 >= a.kb.tokens) return false;
+  w->t0 = static_cast<int>(t0);
+  w->n = min(a.tokens_per_warp, a.kb.tokens - w->t0);
+  w->vec0 = static_cast<int>(id % a.parts) * KV_IO_PART + lane;
+  w->place = lane < w->n ? kv_place(a.kb, w->t0 + lane, ROW_BYTES) : -1;
+  return true;
+}
+
+// Where vector v of a token (8 elements; K's, then as many of V) lies: head and
+// K or V in the page, element in the row.
+template <int D, int BITS>
+__device__ __forceinline__ int kv_vector_row(const KvBatch& kb, int v, int half_vecs, int* d) {
+  const int kv = v >= half_vecs ? 1 : 0;
+  const int e = (v - kv * half_vecs) * 8;
+  *d = e % D;
+  return ((e / D * 2 + kv) << kb.page_shift) * KvRow<D, BITS>::BYTES;
+}
+
+// The smallest and the largest of a group's fp16 values, as (min, -max) in one
+// register, from the 8 in `w` and those of the three lanes beside.
+__device__ __forceinline__ __half2 kv_group_range(const uint32_t (&w)[4]) {
+  __half2 lo = __hmin2(__hmin2(as_half2(w[0]), as_half2(w[1])), __hmin2(as_half2(w[2]), as_half2(w[3])));
+  __half2 hi = __hmax2(__hmax2(as_half2(w[0]), as_half2(w[1])), __hmax2(as_half2(w[2]), as_half2(w[3])));
+  // (lo.x, -hi.x) and (lo.y, -hi.y)
+  hi = __hneg2(hi);
+  __half2 r = __hmin2(__lows2half2(lo, hi), __highs2half2(lo, hi));
+  r = __hmin2(r, as_half2(__shfl_xor_sync(0xffffffffu, as_u32(r), 1)));
+  return __hmin2(r, as_half2(__shfl_xor_sync(0xffffffffu, as_u32(r), 2)));
+}
+
+// Codes of 8 values: min(top, round_half_even((x - lo) / s)). The quotient is
+// first formed with the reciprocal: two roundings of 2^-24 each, so off by less than
+// 2^-14.9 below 260. Where that could decide between two codes (closer than 2^-14
+// to a half), the division itself decides. out[j] holds 0x4B400000 + code.
+__device__ __forceinline__ void kv_quantise8(const uint32_t (&w)[4], float lo, float s, float top,
+                                             uint32_t (&out)[8]) {
+  constexpr float ROUND = 12582912.0f;  // 1.5 * 2^23: adding it rounds to an integer, half to even
+  const float inv = s > 0.f ? __frcp_rn(s) : 0.f;
+  bool close = false;
+  float d[8];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 f = __half22float2(as_half2(w[j]));
+    d[2 * j] = __fsub_rn(f.x, lo);
+    d[2 * j + 1] = __fsub_rn(f.y, lo);
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float q = fminf(__fmul_rn(d[j], inv), top);
+    const float r = __fadd_rn(q, ROUND);
+    close = close || fabsf(__fsub_rn(q, __fsub_rn(r, ROUND))) > 0.5f - 6.103515625e-5f;
+    out[j] = __float_as_uint(r);
+  }
+  if (close && s > 0.f) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      out[j] = __float_as_uint(__fadd_rn(fminf(__fdiv_rn(d[j], s), top), ROUND));
+  }
+}
+
+// Quantises K and V of the batch's rows. A warp takes 128 vectors of 8 elements of
+// each of its tokens; the four lanes of a group of 32 find its range by two
+// shuffles of one register. Bound by the bytes it moves: 512 in and 160 out per
+// token and head at D = 128 in 4 bits.
 template <int D, int BITS>
 __global__ void __launch_bounds__(KV_IO_WARPS * 32) kv_append_kernel(const KvIoArgs a) {
   constexpr float TOP = static_cast<float>((1 << BITS) - 1);
   using Row = KvRow<D, BITS>;
   const int lane = threadIdx.x & 31;
-  const long long w = static_cast<long long>(blockIdx.x) * KV_IO_WARPS + (threadIdx.x >> 5);
-  const long long t64 = w / a.parts;
-  if (t64 >= a.kb.tokens) return;
-  const int t = static_cast<int>(t64);
-  const int vec0 = static_cast<int>(w % a.parts) * KV_IO_PART + lane;
   const int half_vecs = a.kb.heads_kv * (D / 8);  // vectors of K; as many of V
-  // The inputs do not wait for the page number.
-  uint4 in[KV_IO_VECS];
+  KvIoWork work;
+  if (!kv_io_work<Row::BYTES>(a, lane, &work)) return;
+#pragma unroll 2
+  for (int i = 0; i < work.n; ++i) {
+    const long long t = work.t0 + i;
+    uint4 in[KV_IO_VECS];
 #pragma unroll
-  for (int i = 0; i < KV_IO_VECS; ++i) {
-    const int v = vec0 + 32 * i;
-    if (v >= 2 * half_vecs) continue;
-    const __half* src = v < half_vecs ? a.in_k + t * a.k_stride + v * 8 : a.in_v + t * a.v_stride + (v - half_vecs) * 8;
-    in[i] = __ldg(reinterpret_cast<const uint4*>(src));
-  }
-  int row = 0;
-  uint8_t* page = kv_place(a.kb, a.cache, t, lane, &row);
-  if (page == nullptr) return;
+    for (int k = 0; k < KV_IO_VECS; ++k) {
+      const int v = work.vec0 + 32 * k;
+      in[k] = make_uint4(0u, 0u, 0u, 0u);
+      if (v >= 2 * half_vecs) continue;
+      const __half* src =
+          v < half_vecs ? a.in_k + t * a.k_stride + v * 8 : a.in_v + t * a.v_stride + (v - half_vecs) * 8;
+      in[k] = __ldg(reinterpret_cast<const uint4*>(src));
+    }
+    const long long place = __shfl_sync(0xffffffffu, work.place, i);
+    if (place < 0) continue;
+    uint8_t* page = a.cache + place;
 #pragma unroll
-  for (int i = 0; i < KV_IO_VECS; ++i) {
-    const int v = vec0 + 32 * i;
-    const bool have = v < 2 * half_vecs;
-    float x[8];
-    if (have) {
-      const uint32_t words[4] = {in[i].x, in[i].y, in[i].z, in[i].w};
+    for (int k = 0; k < KV_IO_VECS; ++k) {
+      const int v = work.vec0 + 32 * k;
+      uint32_t w[4] = {in[k].x, in[k].y, in[k].z, in[k].w};
+      // NaN counts as 0 and infinities as the largest finite value: exponents of
+      // all ones carry into the sign bit here.
+      uint32_t odd = 0;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 f = __half22float2(as_half2(words[j]));
-        x[2 * j] = f.x;
-        x[2 * j + 1] = f.y;
+      for (int j = 0; j < 4; ++j) odd |= (w[j] & 0x7FFF7FFFu) + 0x04000400u;
+      if ((odd & 0x80008000u) != 0) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t fixed = 0;
+#pragma unroll
+          for (int h = 0; h < 32; h += 16) {
+            uint32_t x = (w[j] >> h) & 0xFFFFu;
+            if ((x & 0x7FFFu) > 0x7C00u) x = 0;                                  // NaN
+            if ((x & 0x7FFFu) == 0x7C00u) x = (x & 0x8000u) | 0x7BFFu;           // infinity
+            fixed |= x << h;
+          }
+          w[j] = fixed;
+        }
       }
-    } else {
+      const __half2 range = kv_group_range(w);
+      const __half zero = __low2half(range);
+      const float lo = __half2float(zero), hi = -__half2float(__high2half(range));
+      const __half scale = __float2half_rz(__fdiv_rn(__fsub_rn(hi, lo), TOP));
+      uint32_t code[8];
+      kv_quantise8(w, lo, __half2float(scale), TOP, code);
+      if (v >= 2 * half_vecs) continue;
+      int d;
+      uint8_t* dst = page + kv_vector_row<D, BITS>(a.kb, v, half_vecs, &d);
+      // The constant part of the codes' bits falls away modulo 2^32.
+      if constexpr (BITS == 4) {
+        uint32_t packed = 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = 0.f;
+        for (int j = 7; j >= 0; --j) packed = packed * 16u + (code[j] - 0x4B400000u);
+        *reinterpret_cast<uint32_t*>(dst + d / 2) = packed;
+      } else {
+        uint32_t packed[2] = {0, 0};
+#pragma unroll
+        for (int j = 3; j >= 0; --j) {
+          packed[0] = packed[0] * 256u + (code[j] - 0x4B400000u);
+          packed[1] = packed[1] * 256u + (code[4 + j] - 0x4B400000u);
+        }
+        *reinterpret_cast<uint2*>(dst + d) = make_uint2(packed[0], packed[1]);
+      }
+      if ((lane & 3) == 0)
+        *reinterpret_cast<__half2*>(dst + Row::CODES + d / KV_GROUP * 4) = __halves2half2(scale, zero);
     }
-    float lo = INFINITY, hi = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      x[j] = x[j] != x[j] ? 0.f : fminf(fmaxf(x[j], -65504.f), 65504.f);
-      lo = fminf(lo, x[j]);
-      hi = fmaxf(hi, x[j]);
-    }
-#pragma unroll
-    for (int s = 1; s <= 2; s <<= 1) {
-      lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, s));
-      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, s));
-    }
-    const __half scale = __float2half_rz(__fdiv_rn(__fsub_rn(hi, lo), TOP));
-    const float s = __half2float(scale);
-    uint32_t code[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      code[j] = s > 0.f ? static_cast<uint32_t>(fminf(rintf(__fdiv_rn(__fsub_rn(x[j], lo), s)), TOP)) : 0u;
-    if (!have) continue;
-    const int kv = v >= half_vecs ? 1 : 0;
-    const int e = (v - kv * half_vecs) * 8;
-    const int head = e / D, d = e % D;
-    uint8_t* dst = page + (static_cast<long long>((head * 2 + kv) << a.kb.page_shift) + row) * Row::BYTES;
-    if constexpr (BITS == 4) {
-      uint32_t packed = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) packed |= code[j] << (4 * j);
-      *reinterpret_cast<uint32_t*>(dst + d / 2) = packed;
-    } else {
-      *reinterpret_cast<uint2*>(dst + d) =
-          make_uint2(code[0] | (code[1] << 8) | (code[2] << 16) | (code[3] << 24),
-                     code[4] | (code[5] << 8) | (code[6] << 16) | (code[7] << 24));
-    }
-    if ((lane & 3) == 0)
-      *reinterpret_cast<__half2*>(dst + Row::CODES + d / KV_GROUP * 4) = __halves2half2(scale, __float2half_rn(lo));
   }
 }
 
@@ -258,52 +323,51 @@ template <int D, int BITS>
 __global__ void __launch_bounds__(KV_IO_WARPS * 32) kv_read_kernel(const KvIoArgs a) {
   using Row = KvRow<D, BITS>;
   const int lane = threadIdx.x & 31;
-  const long long w = static_cast<long long>(blockIdx.x) * KV_IO_WARPS + (threadIdx.x >> 5);
-  const long long t64 = w / a.parts;
-  if (t64 >= a.kb.tokens) return;
-  const int t = static_cast<int>(t64);
-  const int vec0 = static_cast<int>(w % a.parts) * KV_IO_PART + lane;
   const int half_vecs = a.kb.heads_kv * (D / 8);
-  int row = 0;
-  const uint8_t* page = kv_place(a.kb, a.cache, t, lane, &row);
-  if (page == nullptr) return;
-  uint2 codes[KV_IO_VECS];
-  __half2 par[KV_IO_VECS];
+  KvIoWork work;
+  if (!kv_io_work<Row::BYTES>(a, lane, &work)) return;
+#pragma unroll 2
+  for (int i = 0; i < work.n; ++i) {
+    const long long t = work.t0 + i;
+    const long long place = __shfl_sync(0xffffffffu, work.place, i);
+    if (place < 0) continue;
+    const uint8_t* page = a.cache + place;
+    uint2 codes[KV_IO_VECS];
+    __half2 par[KV_IO_VECS];
 #pragma unroll
-  for (int i = 0; i < KV_IO_VECS; ++i) {
-    const int v = vec0 + 32 * i;
-    if (v >= 2 * half_vecs) continue;
-    const int kv = v >= half_vecs ? 1 : 0;
-    const int e = (v - kv * half_vecs) * 8;
-    const int head = e / D, d = e % D;
-    const uint8_t* src = page + (static_cast<long long>((head * 2 + kv) << a.kb.page_shift) + row) * Row::BYTES;
-    if constexpr (BITS == 4)
-      codes[i] = make_uint2(*reinterpret_cast<const uint32_t*>(src + d / 2), 0u);
-    else
-      codes[i] = *reinterpret_cast<const uint2*>(src + d);
-    par[i] = *reinterpret_cast<const __half2*>(src + Row::CODES + d / KV_GROUP * 4);
-  }
-#pragma unroll
-  for (int i = 0; i < KV_IO_VECS; ++i) {
-    const int v = vec0 + 32 * i;
-    if (v >= 2 * half_vecs) continue;
-    const __half2 s2 = __low2half2(par[i]), z2 = __high2half2(par[i]);
-    uint4 out;
-    if constexpr (BITS == 4) {
-      __half2 c[4];
-      kv_codes4(codes[i].x, c, KV_1024);  // pairs (0,4) (1,5) (2,6) (3,7)
-      const uint32_t p0 = as_u32(__hfma2(c[0], s2, z2)), p1 = as_u32(__hfma2(c[1], s2, z2)),
-                     p2 = as_u32(__hfma2(c[2], s2, z2)), p3 = as_u32(__hfma2(c[3], s2, z2));
-      out = make_uint4(__byte_perm(p0, p1, 0x5410), __byte_perm(p2, p3, 0x5410), __byte_perm(p0, p1, 0x7632),
-                       __byte_perm(p2, p3, 0x7632));
-    } else {
-      out.x = as_u32(__hfma2(kv_codes8(codes[i].x, 0x4140), s2, z2));
-      out.y = as_u32(__hfma2(kv_codes8(codes[i].x, 0x4342), s2, z2));
-      out.z = as_u32(__hfma2(kv_codes8(codes[i].y, 0x4140), s2, z2));
-      out.w = as_u32(__hfma2(kv_codes8(codes[i].y, 0x4342), s2, z2));
+    for (int k = 0; k < KV_IO_VECS; ++k) {
+      const int v = work.vec0 + 32 * k;
+      if (v >= 2 * half_vecs) continue;
+      int d;
+      const uint8_t* src = page + kv_vector_row<D, BITS>(a.kb, v, half_vecs, &d);
+      if constexpr (BITS == 4)
+        codes[k] = make_uint2(__ldg(reinterpret_cast<const uint32_t*>(src + d / 2)), 0u);
+      else
+        codes[k] = __ldg(reinterpret_cast<const uint2*>(src + d));
+      par[k] = as_half2(__ldg(reinterpret_cast<const uint32_t*>(src + Row::CODES + d / KV_GROUP * 4)));
     }
-    __half* dst = v < half_vecs ? a.out_k + t * a.k_stride + v * 8 : a.out_v + t * a.v_stride + (v - half_vecs) * 8;
-    *reinterpret_cast<uint4*>(dst) = out;
+#pragma unroll
+    for (int k = 0; k < KV_IO_VECS; ++k) {
+      const int v = work.vec0 + 32 * k;
+      if (v >= 2 * half_vecs) continue;
+      const __half2 s2 = __low2half2(par[k]), z2 = __high2half2(par[k]);
+      uint4 out;
+      if constexpr (BITS == 4) {
+        __half2 c[4];
+        kv_codes4(codes[k].x, c, KV_1024);  // pairs (0,4) (1,5) (2,6) (3,7)
+        const uint32_t p0 = as_u32(__hfma2(c[0], s2, z2)), p1 = as_u32(__hfma2(c[1], s2, z2)),
+                       p2 = as_u32(__hfma2(c[2], s2, z2)), p3 = as_u32(__hfma2(c[3], s2, z2));
+        out = make_uint4(__byte_perm(p0, p1, 0x5410), __byte_perm(p2, p3, 0x5410), __byte_perm(p0, p1, 0x7632),
+                         __byte_perm(p2, p3, 0x7632));
+      } else {
+        out.x = as_u32(__hfma2(kv_codes8(codes[k].x, 0x4140), s2, z2));
+        out.y = as_u32(__hfma2(kv_codes8(codes[k].x, 0x4342), s2, z2));
+        out.z = as_u32(__hfma2(kv_codes8(codes[k].y, 0x4140), s2, z2));
+        out.w = as_u32(__hfma2(kv_codes8(codes[k].y, 0x4342), s2, z2));
+      }
+      __half* dst = v < half_vecs ? a.out_k + t * a.k_stride + v * 8 : a.out_v + t * a.v_stride + (v - half_vecs) * 8;
+      *reinterpret_cast<uint4*>(dst) = out;
+    }
   }
 }
 

@@ -102,7 +102,11 @@ mm4_status launch_io(const mm4_kv_cache_plan* p, KvIoArgs& a, bool write, cudaSt
   if (rc != MM4_OK) return rc;
   const int vecs = 2 * p->d.heads_kv * p->d.head_dim / 8;
   a.parts = (vecs + KV_IO_PART - 1) / KV_IO_PART;
-  const long long blocks = (static_cast<long long>(a.kb.tokens) * a.parts + KV_IO_WARPS - 1) / KV_IO_WARPS;
+  // One token a warp until every SM has its 64 warps, then up to 8.
+  const long long warps = static_cast<long long>(a.kb.tokens) * a.parts;
+  a.tokens_per_warp = static_cast<int>(std::max(1ll, std::min(8ll, warps / (64ll * info.sm_count))));
+  const long long groups = (a.kb.tokens + a.tokens_per_warp - 1) / a.tokens_per_warp;
+  const long long blocks = (groups * a.parts + KV_IO_WARPS - 1) / KV_IO_WARPS;
   if (blocks > 0x7fffffffLL) return fail(MM4_ERR_UNSUPPORTED, "too many tokens for one launch");
   return by_row(p->d, [&](auto, auto D, auto B) -> mm4_status {
     if (write)
@@ -121,9 +125,9 @@ mm4_status launch_io(const mm4_kv_cache_plan* p, KvIoArgs& a, bool write, cudaSt
 //   FEW    up to 8, 16 or 24 rows of a unit, and 4 units of 24 rows: a 32-key tile
 //          costs an SM about 250 clocks for each 24 rows.
 //   MANY   more than 96 rows: about 1050 clocks for up to 256 rows.
-//   TEAM   FEW of at most 16 rows, if no sequence can hold more than two tiles a
-//          warp: whole units to a CTA, one launch (13 us against 17 for a call
-//          alone).
+//   TEAM   FEW of at most 16 rows, if no sequence can hold more than a few tiles a
+//          warp and there are no more units than SMs: whole units to a CTA, one
+//          launch.
 struct Form {
   enum Kind { FEW8, FEW16, FEW24, MANY } kind;
   bool team;
@@ -133,7 +137,8 @@ struct Form {
 
 constexpr int kMaxCtas = 160;    // workspaces are sized for this many SMs
 constexpr int kFewRows = 96;     // the most rows that FEW takes
-constexpr int kTeamTokens = 448;  // the most tokens of a sequence for TEAM: 2 tiles of 32 for each of 7 warps
+constexpr int kTeamTokens = 32 * KVF_TK;  // the most tokens of a sequence for TEAM: 3 or 5 tiles a warp
+constexpr long long kTeamUnits = 148;     // and the most units (heads of sequences): one for each SM
 
 Form attention_form(const mm4_kv_cache_plan* p, const mm4_kv_cache_batch* b) {
   const int group = p->d.heads_q / p->d.heads_kv;
@@ -147,7 +152,7 @@ Form attention_form(const mm4_kv_cache_plan* p, const mm4_kv_cache_batch* b) {
     return f;
   }
   f.kind = rows <= 8 ? Form::FEW8 : rows <= 16 ? Form::FEW16 : Form::FEW24;
-  f.team = rows <= 16 && room <= kTeamTokens;
+  f.team = rows <= 16 && room <= kTeamTokens && static_cast<long long>(b->sequences) * p->d.heads_kv <= kTeamUnits;
   const int nt = rows <= 8 ? 1 : rows <= 16 ? 2 : 3;
   const int warps = nt == 1 ? 14 : 7;  // at most
   if (!f.team) f.workspace = sizeof(float) * 2 * kMaxCtas * warps * 8 * nt * (p->d.head_dim + 2);
@@ -189,7 +194,12 @@ mm4_status launch_few(KvAttnArgs& a, int sms, cudaStream_t st) {
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "kv_attention_few_kernel launch");
   if (TEAM) return MM4_OK;
-  return launch_join(kv_attention_join_kernel<D, Cfg::ROWS, KVF_TK>, dim3(static_cast<unsigned>(units), NT * blocks), a, st);
+  // Up to 8 rows of a unit to a block of the join, one where that leaves SMs idle.
+  const long long rows = std::min(8 * NT, a.kb.max_new * a.group);
+  a.join_rows = 8;
+  while (a.join_rows > 1 && units * blocks * ((rows + a.join_rows - 1) / a.join_rows) < 2 * sms) a.join_rows /= 2;
+  const unsigned chunks = static_cast<unsigned>(blocks * ((rows + a.join_rows - 1) / a.join_rows));
+  return launch_join(kv_attention_join_kernel<D, Cfg::ROWS, KVF_TK>, dim3(static_cast<unsigned>(units), chunks), a, st);
 }
 
 template <int D, int BITS>
