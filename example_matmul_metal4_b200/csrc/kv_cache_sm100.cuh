@@ -72,17 +72,27 @@ __device__ __forceinline__ KvSequence kv_sequence(const KvBatch& kb, int b) {
   return s;
 }
 
-// The sequence whose rows hold row t: a binary search of the ascending offsets,
-// then a check, so offsets that are out of order find nothing rather than
-// something wrong. -1 for padding rows.
-__device__ __forceinline__ int kv_find_sequence(const KvBatch& kb, int t) {
-  int lo = 0, hi = kb.sequences;  // offsets[lo] <= t is assumed, offsets[hi] > t or hi = sequences
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (__ldg(kb.offsets + mid) <= t)
-      lo = mid;
-    else
-      hi = mid;
+// The sequence whose rows hold row t: a search of the ascending offsets, then a
+// check, so offsets that are out of order find nothing rather than something
+// wrong. -1 for padding rows. Lanes with tokens of their own search binary; a
+// warp with one token searches 32-way, two steps for up to 1024 sequences.
+template <bool WARP>
+__device__ __forceinline__ int kv_find_sequence(const KvBatch& kb, int t, int lane) {
+  int lo = 0, n = kb.sequences;
+  while (n > 1) {
+    if constexpr (WARP) {
+      const int step = (n + 31) / 32, probe = lane * step;
+      const unsigned hit = __ballot_sync(0xffffffffu, probe < n && __ldg(kb.offsets + lo + probe) <= t);
+      if (hit == 0) return -1;
+      const int k = (31 - __clz(hit)) * step;
+      lo += k;
+      n = min(step, n - k);
+    } else {
+      const int half = n >> 1;
+      const bool right = __ldg(kb.offsets + lo + half) <= t;
+      lo = right ? lo + half : lo;
+      n = right ? n - half : half;
+    }
   }
   const int first = __ldg(kb.offsets + lo), end = __ldg(kb.offsets + lo + 1);
   if (end < first) kv_note(KV_DATA_OFFSETS);
@@ -92,8 +102,9 @@ __device__ __forceinline__ int kv_find_sequence(const KvBatch& kb, int t) {
 // Where the K row of token t lies for head 0, as an offset into the cache; -1 if
 // the row has no place (padding, before position 0, beyond the page table, a
 // page outside the pool).
-__device__ __forceinline__ long long kv_place(const KvBatch& kb, int t, int row_bytes) {
-  const int b = kv_find_sequence(kb, t);
+template <bool WARP>
+__device__ __forceinline__ long long kv_place(const KvBatch& kb, int t, int row_bytes, int lane) {
+  const int b = kv_find_sequence<WARP>(kb, t, lane);
   if (b < 0) return -1;
   const int end = __ldg(kb.offsets + b + 1);
   const int len = __ldg(kb.lengths + b);
@@ -181,7 +192,10 @@ __device__ __forceinline__ bool kv_io_work(const KvIoArgs& a, int lane, KvIoWork
   w->t0 = static_cast<int>(t0);
   w->n = min(a.tokens_per_warp, a.kb.tokens - w->t0);
   w->vec0 = static_cast<int>(id % a.parts) * KV_IO_PART + lane;
-  w->place = lane < w->n ? kv_place(a.kb, w->t0 + lane, ROW_BYTES) : -1;
+  if (a.tokens_per_warp == 1)
+    w->place = kv_place<true>(a.kb, w->t0, ROW_BYTES, lane);
+  else
+    w->place = lane < w->n ? kv_place<false>(a.kb, w->t0 + lane, ROW_BYTES, lane) : -1;
   return true;
 }
 
@@ -208,33 +222,49 @@ __device__ __forceinline__ __half2 kv_group_range(const uint32_t (&w)[4]) {
 }
 
 // Codes of 8 values: min(top, round_half_even((x - lo) / s)). The quotient is
-// first formed with the reciprocal: two roundings of 2^-24 each, so off by less than
-// 2^-14.9 below 260. Where that could decide between two codes (closer than 2^-14
-// to a half), the division itself decides. out[j] holds 0x4B400000 + code.
+// first formed with an approximate reciprocal (off by 2^-23) and a product (2^-24),
+// so it is off by less than 2^-14.3 below 260. Where that could decide between
+// two codes (closer than 2^-14 to a half), the division itself decides; so it does
+// for subnormal scales, the only ones whose quotients pass top + 1/2 (a scale is cut
+// by up to 2^-10 of itself otherwise). out[j] holds KV_CODE + code.
+constexpr uint32_t KV_CODE = 0x4B400000u;  // fp32 1.5 * 2^23: adding it rounds to an integer, half to even
 __device__ __forceinline__ void kv_quantise8(const uint32_t (&w)[4], float lo, float s, float top,
                                              uint32_t (&out)[8]) {
-  constexpr float ROUND = 12582912.0f;  // 1.5 * 2^23: adding it rounds to an integer, half to even
-  const float inv = s > 0.f ? __frcp_rn(s) : 0.f;
-  bool close = false;
-  float d[8];
+  const float round = __uint_as_float(KV_CODE);
+  float inv;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+  bool exact = s < 6.103515625e-5f;
+  if (exact) inv = 0.f;
+  float2 d[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const float2 f = __half22float2(as_half2(w[j]));
-    d[2 * j] = __fsub_rn(f.x, lo);
-    d[2 * j + 1] = __fsub_rn(f.y, lo);
+    d[j] = fadd2(__half22float2(as_half2(w[j])), make_float2(-lo, -lo));
+    const float2 q = ffma2(d[j], make_float2(inv, inv), make_float2(0.f, 0.f));
+    const float2 r = fadd2(q, make_float2(round, round));
+    const float2 n = fadd2(r, make_float2(-round, -round));
+    const float2 off = fadd2(q, make_float2(-n.x, -n.y));
+    exact = exact || fmaxf(fabsf(off.x), fabsf(off.y)) > 0.5f - 6.103515625e-5f;
+    out[2 * j] = __float_as_uint(r.x);
+    out[2 * j + 1] = __float_as_uint(r.y);
   }
+  if (exact) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float q = fminf(__fmul_rn(d[j], inv), top);
-    const float r = __fadd_rn(q, ROUND);
-    close = close || fabsf(__fsub_rn(q, __fsub_rn(r, ROUND))) > 0.5f - 6.103515625e-5f;
-    out[j] = __float_as_uint(r);
+    for (int j = 0; j < 8; ++j) {
+      const float x = (j & 1) ? d[j / 2].y : d[j / 2].x;
+      out[j] = s > 0.f ? __float_as_uint(__fadd_rn(fminf(__fdiv_rn(x, s), top), round)) : KV_CODE;
+    }
   }
-  if (close && s > 0.f) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      out[j] = __float_as_uint(__fadd_rn(fminf(__fdiv_rn(d[j], s), top), ROUND));
-  }
+}
+
+// x / top rounded to fp32 as a division would: a product with the rounded
+// reciprocal is off by less than a unit in the last place, its remainder is exact
+// in a fused multiply-add, and adding remainder * reciprocal rounds correctly
+// (Markstein, IBM J. Res. Dev. 34, 1990). x is 0 or at least 2^-24.
+template <int TOP>
+__device__ __forceinline__ float kv_divide_by_top(float x) {
+  constexpr float INV = 1.0f / TOP;
+  const float q = __fmul_rn(x, INV);
+  return __fmaf_rn(__fmaf_rn(-q, static_cast<float>(TOP), x), INV, q);
 }
 
 // Quantises K and V of the batch's rows. A warp takes 128 vectors of 8 elements of
@@ -242,14 +272,14 @@ __device__ __forceinline__ void kv_quantise8(const uint32_t (&w)[4], float lo, f
 // shuffles of one register. Bound by the bytes it moves: 512 in and 160 out per
 // token and head at D = 128 in 4 bits.
 template <int D, int BITS>
-__global__ void __launch_bounds__(KV_IO_WARPS * 32) kv_append_kernel(const KvIoArgs a) {
-  constexpr float TOP = static_cast<float>((1 << BITS) - 1);
+__global__ void __launch_bounds__(KV_IO_WARPS * 32, 8) kv_append_kernel(const KvIoArgs a) {
+  constexpr int TOP = (1 << BITS) - 1;
   using Row = KvRow<D, BITS>;
   const int lane = threadIdx.x & 31;
   const int half_vecs = a.kb.heads_kv * (D / 8);  // vectors of K; as many of V
   KvIoWork work;
   if (!kv_io_work<Row::BYTES>(a, lane, &work)) return;
-#pragma unroll 2
+#pragma unroll 1
   for (int i = 0; i < work.n; ++i) {
     const long long t = work.t0 + i;
     uint4 in[KV_IO_VECS];
@@ -291,26 +321,29 @@ __global__ void __launch_bounds__(KV_IO_WARPS * 32) kv_append_kernel(const KvIoA
       const __half2 range = kv_group_range(w);
       const __half zero = __low2half(range);
       const float lo = __half2float(zero), hi = -__half2float(__high2half(range));
-      const __half scale = __float2half_rz(__fdiv_rn(__fsub_rn(hi, lo), TOP));
+      const __half scale = __float2half_rz(kv_divide_by_top<TOP>(__fsub_rn(hi, lo)));
       uint32_t code[8];
       kv_quantise8(w, lo, __half2float(scale), TOP, code);
       if (v >= 2 * half_vecs) continue;
       int d;
       uint8_t* dst = page + kv_vector_row<D, BITS>(a.kb, v, half_vecs, &d);
-      // The constant part of the codes' bits falls away modulo 2^32.
+      // Codes are packed by multiplication and addition modulo 2^32, KV_CODE with
+      // them, and what that adds up to is taken off.
       if constexpr (BITS == 4) {
-        uint32_t packed = 0;
+        constexpr uint32_t TAKE = KV_CODE * 0x11111111u;
+        uint32_t packed = code[7];
 #pragma unroll
-        for (int j = 7; j >= 0; --j) packed = packed * 16u + (code[j] - 0x4B400000u);
-        *reinterpret_cast<uint32_t*>(dst + d / 2) = packed;
+        for (int j = 6; j >= 0; --j) packed = packed * 16u + code[j];
+        *reinterpret_cast<uint32_t*>(dst + d / 2) = packed - TAKE;
       } else {
-        uint32_t packed[2] = {0, 0};
+        constexpr uint32_t TAKE = KV_CODE * 0x01010101u;
+        uint32_t packed[2] = {code[3], code[7]};
 #pragma unroll
-        for (int j = 3; j >= 0; --j) {
-          packed[0] = packed[0] * 256u + (code[j] - 0x4B400000u);
-          packed[1] = packed[1] * 256u + (code[4 + j] - 0x4B400000u);
+        for (int j = 2; j >= 0; --j) {
+          packed[0] = packed[0] * 256u + code[j];
+          packed[1] = packed[1] * 256u + code[4 + j];
         }
-        *reinterpret_cast<uint2*>(dst + d) = make_uint2(packed[0], packed[1]);
+        *reinterpret_cast<uint2*>(dst + d) = make_uint2(packed[0] - TAKE, packed[1] - TAKE);
       }
       if ((lane & 3) == 0)
         *reinterpret_cast<__half2*>(dst + Row::CODES + d / KV_GROUP * 4) = __halves2half2(scale, zero);

@@ -77,6 +77,8 @@ class KVCachePlan:
         h = ctypes.c_void_p()
         _lib.check(self._L.mm4_kv_cache_plan_create(ctypes.byref(h), ctypes.byref(d)))
         self._h = h
+        import torch
+        self._f16, self._u8, self._device = torch.float16, torch.uint8, torch._C._cuda_getDevice
         self.pageBytes = int(self._L.mm4_kv_cache_page_bytes(h))
         self.cacheBytes = int(self._L.mm4_kv_cache_bytes(h))
 
@@ -92,30 +94,24 @@ class KVCachePlan:
         return torch.zeros(self.dims.pages, self.pageBytes, dtype=torch.uint8, device=device)
 
     def _cache(self, cache, batch):
-        import torch
-        if cache.dtype is not torch.uint8 or cache.numel() != self.cacheBytes or not cache.is_contiguous():
+        if cache.dtype is not self._u8 or cache.numel() != self.cacheBytes or not cache.is_contiguous():
             raise ValueError(f"cache must be a contiguous CUDA uint8 tensor of {self.cacheBytes} bytes")
         dev = batch.device
         if cache.get_device() != dev:
             raise ValueError("cache and batch must be on one device")
-        if dev != torch._C._cuda_getDevice():
+        if dev != self._device():
             raise ValueError(f"the tensors are on device {dev}, which is not the current CUDA device")
         return cache.data_ptr()
 
     def _rows(self, name, t, heads, batch):
-        import torch
-        shape = t.shape
-        if len(shape) != 3 or shape[0] != batch.tokens or shape[1] != heads or shape[2] != self.dims.K or \
-                t.dtype is not torch.float16 or t.get_device() != batch.device:
-            raise ValueError(f"{name} must be an fp16 tensor of shape {(batch.tokens, heads, self.dims.K)} on the "
-                             "batch's device")
-        stride = t.stride()
-        if stride[2] != 1 or (stride[1] != self.dims.K and heads > 1):
+        """(address, elements from row to row) of rows fp16 [tokens][heads][K]."""
+        K = self.dims.K
+        if t.shape != (batch.tokens, heads, K) or t.dtype is not self._f16 or t.get_device() != batch.device:
+            raise ValueError(f"{name} must be an fp16 tensor of shape {(batch.tokens, heads, K)} on the batch's device")
+        row, head, element = t.stride()
+        if element != 1 or (head != K and heads > 1):
             raise ValueError(f"the heads of each row of {name} must be contiguous")
-        width = heads * self.dims.K
-        if shape[0] <= 1:
-            return t.data_ptr(), width
-        return t.data_ptr(), stride[0]
+        return t.data_ptr(), row if batch.tokens > 1 else heads * K
 
     def append(self, K, V, cache, batch, stream=None) -> None:
         """Quantises the rows of K and V (fp16 [tokens][Hk][K]; rows may be strided, as slices of a fused
@@ -128,19 +124,19 @@ class KVCachePlan:
     def read(self, cache, batch, K=None, V=None, stream=None):
         """(K, V): the fp16 values [tokens][Hk][K] that an append of this batch left in the cache
         (mm4_kv_cache_read). Padding rows of given tensors are left as they were; of new ones they are
-        uninitialised."""
-        import torch
-        shape = (batch.tokens, self.dims.Hk, self.dims.K)
-        if K is None:
-            K = torch.empty(shape, dtype=torch.float16, device=cache.device)
-            _keep(K, stream)
-        if V is None:
-            V = torch.empty(shape, dtype=torch.float16, device=cache.device)
-            _keep(V, stream)
-        kp, ks = self._rows("K", K, self.dims.Hk, batch)
-        vp, vs = self._rows("V", V, self.dims.Hk, batch)
-        _lib.check(self._L.mm4_kv_cache_read(self._h, batch._ref, self._cache(cache, batch), kp, ks, vp, vs,
-                                             _lib.stream_handle(stream)))
+        uninitialised. Without K and V, the two are halves of one new tensor."""
+        Hk, D = self.dims.Hk, self.dims.K
+        cp = self._cache(cache, batch)
+        if K is None and V is None:
+            pair = cache.new_empty((2, batch.tokens, Hk, D), dtype=self._f16)
+            if stream is not None:
+                pair.record_stream(stream)
+            K, V = pair.unbind(0)
+        elif K is None or V is None:
+            raise ValueError("give both K and V, or neither")
+        kp, ks = self._rows("K", K, Hk, batch)
+        vp, vs = self._rows("V", V, Hk, batch)
+        _lib.check(self._L.mm4_kv_cache_read(self._h, batch._ref, cp, kp, ks, vp, vs, _lib.stream_handle(stream)))
         return K, V
 
     def attention_workspace_bytes(self, batch) -> int:
@@ -155,17 +151,19 @@ class KVCachePlan:
         (mm4_kv_cache_attention); append the call's tokens first. With `lse` (fp32 [tokens][Hq]) also writes each
         row's natural-log sum of exp(scale * S). A row that attends to nothing gets O = 0 and lse = -inf.
         `workspace`: a CUDA uint8 tensor; by default each call takes one from torch's allocator."""
-        import torch
-        Hq = self.dims.Hq
+        Hq, D = self.dims.Hq, self.dims.K
         qp, qs = self._rows("Q", Q, Hq, batch)
         cp = self._cache(cache, batch)
         if O is None:
-            O = torch.empty((batch.tokens, Hq, self.dims.K), dtype=torch.float16, device=Q.device)
-            _keep(O, stream)
-        op, os_ = self._rows("O", O, Hq, batch)
+            O = Q.new_empty((batch.tokens, Hq, D))
+            if stream is not None:
+                O.record_stream(stream)  # not reused before that stream is done with it
+            op, os_ = O.data_ptr(), Hq * D
+        else:
+            op, os_ = self._rows("O", O, Hq, batch)
         lp = None
         if lse is not None:
-            if tuple(lse.shape) != (batch.tokens, Hq) or lse.dtype != torch.float32 or not lse.is_contiguous() or \
+            if lse.shape != (batch.tokens, Hq) or str(lse.dtype) != "torch.float32" or not lse.is_contiguous() or \
                     lse.get_device() != batch.device:
                 raise ValueError(f"lse must be a contiguous CUDA fp32 tensor of shape {(batch.tokens, Hq)}")
             lp = lse.data_ptr()
@@ -173,8 +171,9 @@ class KVCachePlan:
         wp = None
         if nbytes:
             if workspace is None:
-                workspace = torch.empty(nbytes, dtype=torch.uint8, device=Q.device)
-                _keep(workspace, stream)
+                workspace = cache.new_empty(nbytes)
+                if stream is not None:
+                    workspace.record_stream(stream)
             elif workspace.get_device() != batch.device or not workspace.is_contiguous():
                 raise ValueError("workspace must be a contiguous tensor on the batch's device")
             else:
@@ -183,10 +182,3 @@ class KVCachePlan:
         _lib.check(self._L.mm4_kv_cache_attention(self._h, batch._ref, qp, qs, cp, op, os_, lp, wp, nbytes,
                                                   _lib.stream_handle(stream)))
         return O
-
-
-def _keep(t, stream) -> None:
-    """A tensor made here on torch's current stream and used on a stream of the caller's is not reused before
-    that stream is done with it."""
-    if stream is not None:
-        t.record_stream(stream)
