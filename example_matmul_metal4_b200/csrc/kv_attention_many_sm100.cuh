@@ -16,7 +16,8 @@
 //   warp 1        TMEM allocation; one lane issues S_i(g) = Q_i K(g)^T (M = 128,
 //                 N = 64) into slot g % 2 of row tile i.
 //   warp 2        one lane issues O_i += P_i(g) V(g) (P from TMEM).
-//   warp 3        finds the CTA's range.
+//   warp 3        finds the CTA's range (and warp 2, before its products, the unit
+//                 that the range leaves to others).
 //   warps 4-11    softmax, one row a thread: P = 2^(S scale log2 e - m), rescaling
 //                 O only when the maximum grew by more than 2^8; results out. A
 //                 thread also copies its row of the next unit's Q, as soon as it has
@@ -249,6 +250,15 @@ template <int D, int ROWS>
 __device__ __forceinline__ long long kvm_slot(long long slot) {
   return slot * KvPartial<D, ROWS>::FLOATS;
 }
+// Behind the partials, for each worker: the unit that it begins and leaves to
+// others, and the last of them (last = -1: none).
+struct KvmShared {
+  int b, rb, h, last;
+};
+template <int D, int ROWS>
+__device__ __forceinline__ KvmShared* kvm_shared(const KvAttnArgs& a) {
+  return reinterpret_cast<KvmShared*>(a.partials + kvm_slot<D, ROWS>(2ll * a.workers));
+}
 
 // As att_exp_store64, calling between() behind the first half.
 template <int EMU, typename F>
@@ -353,6 +363,22 @@ __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const
   if (warp == 1) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
+  }
+  if (warp == 2) {
+    // For the join: the unit that this CTA begins and leaves to others.
+    const long long total = kvm_total(a, ROWS, lane);
+    const long long active = min(static_cast<long long>(a.workers), total);
+    const int w = blockIdx.x;
+    KvmShared shared{0, 0, 0, -1};
+    if (w + 1 < active) {
+      long long begin;
+      int cost;
+      const KvmPlace f = kvm_find(a, ROWS, kv_range_begin(w + 1, total, active), lane, &begin, &cost);
+      // Behind the unit's first step, and the first border that is.
+      if (f.off > KVM_UNIT && begin + KVM_UNIT >= kv_range_begin(w, total, active) && f.b < kb.sequences)
+        shared = KvmShared{f.b, f.rb, f.h, static_cast<int>(kv_worker_of(begin + cost - 1, total, active))};
+    }
+    if (lane == 0) kvm_shared<D, ROWS>(a)[w] = shared;
   }
   if (warp == 3) {
     const long long total = kvm_total(a, ROWS, lane);
@@ -807,39 +833,18 @@ __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const
   }
 }
 
-// Joins the partials of units that several CTAs share. Block (w, c) looks at
-// the border between workers w and w + 1: if it lies in a unit that worker w
-// began, the block joins 32 rows of that unit. Lane = row; a warp takes D / 8
+// Joins the partials of units that several CTAs share: block (w, c) 32 rows of
+// the unit that worker w began and left to others. Lane = row; a warp takes D / 8
 // elements of them.
 template <int D, int ROWS>
 __global__ void __launch_bounds__(256) kv_attention_many_join_kernel(const __grid_constant__ KvAttnArgs a) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int G4 = D / 32;  // groups of 4 elements a warp
-  __shared__ KvmPlace place;
-  __shared__ int last_worker;
   const int w = blockIdx.x;
-  if (warp == 0) {
-    const long long total = kvm_total(a, ROWS, lane);
-    const long long active = min(static_cast<long long>(a.workers), total);
-    int last = -1;
-    KvmPlace f{};
-    if (w + 1 < active) {
-      long long begin;
-      int cost;
-      f = kvm_find(a, ROWS, kv_range_begin(w + 1, total, active), lane, &begin, &cost);
-      // Behind the unit's first step, and the first border that is.
-      if (f.off > KVM_UNIT && begin + KVM_UNIT >= kv_range_begin(w, total, active) && f.b < a.kb.sequences)
-        last = static_cast<int>(kv_worker_of(begin + cost - 1, total, active));
-    }
-    if (lane == 0) {
-      place = f;
-      last_worker = last;
-    }
-  }
-  __syncthreads();
   kv_wait_for_previous();  // in every block: what follows this kernel also follows the one before it
-  const KvmPlace p = place;
-  const int last = last_worker;
+  const int4 left = __ldcg(reinterpret_cast<const int4*>(kvm_shared<D, ROWS>(a) + w));
+  const KvmShared p{left.x, left.y, left.z, left.w};
+  const int last = p.last;
   if (last < 0) return;
   const KvSequence s = kvm_sequence(a, p.b);
   const int local = blockIdx.y * 32 + lane;

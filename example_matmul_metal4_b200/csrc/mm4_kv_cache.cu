@@ -147,7 +147,7 @@ Form attention_form(const mm4_kv_cache_plan* p, const mm4_kv_cache_batch* b) {
   Form f{};
   if (rows > kFewRows) {
     f.kind = Form::MANY;
-    f.workspace = sizeof(float) * 2 * kMaxCtas * 256 * (p->d.head_dim + 2);
+    f.workspace = sizeof(float) * 2 * kMaxCtas * 256 * (p->d.head_dim + 2) + sizeof(KvmShared) * kMaxCtas;
     f.name = "kv_attention_many";
     return f;
   }
