@@ -1,5 +1,5 @@
 // Attention over the key / value cache for many rows (prompts, chunks of them,
-// and tokens times query heads beyond 16 rows).
+// and tokens times query heads beyond 48 rows).
 //
 // Bound by the tensor cores and the exponentials, as attention over fp16 K and
 // V is (4 D FLOP and one exponential per row and key); what the cache adds is
@@ -18,14 +18,21 @@
 //   warp 2        one lane issues O_i += P_i(g) V(g) (P from TMEM).
 //   warp 3        finds the CTA's range (and warp 2, before its products, the unit
 //                 that the range leaves to others).
-//   warps 4-11    softmax, one row a thread: P = 2^(S scale log2 e - m), rescaling
-//                 O only when the maximum grew by more than 2^8; results out. A
-//                 thread also copies its row of the next unit's Q, as soon as it has
-//                 the last scores of the unit, so the copy overlaps the results.
+//   warps 4-11    softmax, one row a thread: P = 2^(S scale log2 e - m) with fp32 m
+//                 and sums, P rounded to fp16 for the product (2^-11 of itself,
+//                 like the result); O is rescaled only when the maximum grew by
+//                 more than 2^8. Results out; a warp also copies its rows of the
+//                 next unit's Q, as soon as it has the last scores of the unit.
 //   warps 12-15   codes to fp16: a lane takes 32 elements (one scale and zero).
 // TMEM: two 64-column S slots for each row tile, then O_i (D columns each). Steps
 // of 64 keys are counted across a CTA's units (g), which fixes slots and
 // mbarrier phases; S runs two steps ahead of the softmax.
+//
+// Four prompts of 4096 tokens, 16 heads of 128, causal, 4 bits, on one B200: 308 us,
+// 893 TFLOP/s (floor 163 us of measured peak). A step of 64 keys takes about
+// 2000 clocks, of which the products need 1280 (S of N = 64 is bound by the
+// 6 KB an instruction reads from shared memory); unpacking alone costs 11 %,
+// its 42 KB a step through shared memory among them.
 #pragma once
 
 #include "attention_sm100.cuh"
@@ -106,11 +113,11 @@ __device__ __forceinline__ long long kvm_warp_sum(long long x) {
   for (int s = 16; s > 0; s >>= 1) x += __shfl_xor_sync(0xffffffffu, x, s);
   return x;
 }
-__device__ __forceinline__ int kvm_lane_cost(const KvAttnArgs& a, int b, int rows) {  // lanes: sequences
+__device__ __forceinline__ long long kvm_lane_cost(const KvAttnArgs& a, int b, int rows) {  // lanes: sequences
   if (b >= a.kb.sequences) return 0;
   const KvSequence s = kvm_sequence(a, b);
   const int blocks = kvm_blocks(s, a.group, rows);
-  int sum = 0;
+  long long sum = 0;
   for (int rb = 0; rb < blocks; ++rb) sum += KVM_UNIT + kvm_steps(s, rb, a, rows);
   return sum;
 }
@@ -154,7 +161,7 @@ __device__ __forceinline__ KvmPlace kvm_find(const KvAttnArgs& a, int rows, long
     }
   } else {
     for (; p.b < a.kb.sequences; p.b += 32) {
-      const int t = kvm_lane_cost(a, p.b + lane, rows);
+      const long long t = kvm_lane_cost(a, p.b + lane, rows);
       long long inc = t;
 #pragma unroll
       for (int s = 1; s < 32; s <<= 1) {

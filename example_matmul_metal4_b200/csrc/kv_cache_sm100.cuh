@@ -269,8 +269,10 @@ __device__ __forceinline__ float kv_divide_by_top(float x) {
 
 // Quantises K and V of the batch's rows. A warp takes 128 vectors of 8 elements of
 // each of its tokens; the four lanes of a group of 32 find its range by two
-// shuffles of one register. Bound by the bytes it moves: 512 in and 160 out per
-// token and head at D = 128 in 4 bits.
+// shuffles of one register. Its floor are the bytes it moves: 512 in and 160 out
+// per token and head at D = 128 in 4 bits, 23 us for four prompts of up to 4096
+// tokens and 16 heads; it takes 60 us (184 instructions for 8 elements a lane, issue
+// slots 70 % busy).
 template <int D, int BITS>
 __global__ void __launch_bounds__(KV_IO_WARPS * 32, 8) kv_append_kernel(const KvIoArgs a) {
   constexpr int TOP = (1 << BITS) - 1;
@@ -352,6 +354,7 @@ __global__ void __launch_bounds__(KV_IO_WARPS * 32, 8) kv_append_kernel(const Kv
 }
 
 // Reads the rows of a batch back as fp16 values; the mapping of kv_append_kernel.
+// Bound by memory: 8 sequences of up to 8192 tokens, 306 MB, in 55 us (5.6 TB/s).
 template <int D, int BITS>
 __global__ void __launch_bounds__(KV_IO_WARPS * 32) kv_read_kernel(const KvIoArgs a) {
   using Row = KvRow<D, BITS>;

@@ -122,12 +122,20 @@ mm4_status launch_io(const mm4_kv_cache_plan* p, KvIoArgs& a, bool write, cudaSt
 // Which kernel attention over a batch runs, from its sizes alone (the lengths
 // lie on the device). Rows are the most that one key / value head has in one
 // sequence: max_new tokens times the query heads that share it.
-//   FEW    up to 8, 16 or 24 rows of a unit, and 4 units of 24 rows: a 32-key tile
-//          costs an SM about 250 clocks for each 24 rows.
-//   MANY   more than 96 rows: about 1050 clocks for up to 256 rows.
-//   TEAM   FEW of at most 16 rows, if no sequence can hold more than a few tiles a
-//          warp and there are no more units than SMs: whole units to a CTA, one
-//          launch.
+//   FEW    up to 8, 16 or 24 rows of a unit, and two units of 24: its time grows
+//          with the units. MANY for more: 256 rows cost little more than one.
+//          16 sequences of 4096 tokens, heads 32 / 8 of 128, 4 bits, one B200:
+//          rows      24     48     72     96    256
+//          FEW       42     72    100    128    327 us
+//          MANY      75     76     77     77     84 us
+//          (heads of 64, 8 bits: FEW 31, 50, 68, 86, 215, MANY 70, 73, 73, 75, 81).
+//   TEAM   FEW of at most 16 rows where no sequence can hold more than 2048 tokens
+//          and there are no more units than SMs: a whole unit to a CTA, one
+//          launch, no workspace. 8 rows, 8 heads of 128, TEAM against split ranges:
+//          tokens              64           1024          2048
+//          1 sequence      4.8,  7.6     9.0, 11.2    13.2, 11.8 us
+//          16 sequences    5.2, 10.8     9.4, 15.8    13.9, 19.7 us
+//          64 sequences   15.1, 13.1    32.6, 29.5    55.0, 46.3 us
 struct Form {
   enum Kind { FEW8, FEW16, FEW24, MANY } kind;
   bool team;
@@ -136,8 +144,8 @@ struct Form {
 };
 
 constexpr int kMaxCtas = 160;    // workspaces are sized for this many SMs
-constexpr int kFewRows = 96;     // the most rows that FEW takes
-constexpr int kTeamTokens = 32 * KVF_TK;  // the most tokens of a sequence for TEAM: 3 or 5 tiles a warp
+constexpr int kFewRows = 48;     // the most rows that FEW takes
+constexpr int kTeamTokens = 2048;         // the most tokens of a sequence for TEAM
 constexpr long long kTeamUnits = 148;     // and the most units (heads of sequences): one for each SM
 
 Form attention_form(const mm4_kv_cache_plan* p, const mm4_kv_cache_batch* b) {
@@ -211,10 +219,14 @@ mm4_status launch_many(KvAttnArgs& a, int sms, cudaStream_t st) {
   {
     // The kernel moves registers between warpgroups (setmaxnreg); that only
     // completes if the launch allocates enough of them.
-    static const int launch_regs = [&] {
+    static std::atomic<int> regs{0};
+    int launch_regs = regs.load();
+    if (launch_regs == 0) {
       cudaFuncAttributes fa;
-      return cudaFuncGetAttributes(&fa, kern) == cudaSuccess ? fa.numRegs : -1;
-    }();
+      cudaError_t e = cudaFuncGetAttributes(&fa, kern);
+      if (e != cudaSuccess) return cuda_fail(e, "cudaFuncGetAttributes(kv_attention_many_kernel)");
+      regs.store(launch_regs = fa.numRegs);
+    }
     if (launch_regs < Cfg::REGS_NEEDED)
       return fail(MM4_ERR_UNSUPPORTED, "attention kernel built with %d registers per thread, needs %d", launch_regs,
                   Cfg::REGS_NEEDED);

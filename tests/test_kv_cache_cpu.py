@@ -131,3 +131,55 @@ def test_restatement_rounds_scales_towards_zero_and_inverts():
         assert np.array_equal(back, ref.values(codes, scale, zero))
         err = np.abs(back.astype(np.float64) - x).reshape(50, 4, 32).max(-1)
         assert (err <= span / top / 2 + span * 2.0 ** -10 + 4 * 2.0 ** -11).all()
+
+
+def test_attention_form_by_sizes():
+    """The kernel is chosen from the batch's sizes: rows of a key / value head in one sequence (max_new times the
+    group of 4 here), the tokens a sequence can hold and the number of units."""
+    L = _lib.lib()
+    rc, h = _plan()
+    assert rc == 0
+
+    def form(**kw):
+        b = _batch(**kw)
+        return (L.mm4_kv_cache_attention_kernel_name(h, ctypes.byref(b)),
+                L.mm4_kv_cache_attention_workspace_size(h, ctypes.byref(b)))
+
+    assert form(max_new=2) == (b"kv_attention_few<8 rows, team>", 0)
+    assert form(max_new=3) == (b"kv_attention_few<16 rows, team>", 0)
+    assert form(max_new=2, pages_per_sequence=32) == (b"kv_attention_few<8 rows, team>", 0)
+    name, ws = form(max_new=2, pages_per_sequence=33)
+    assert name == b"kv_attention_few<8 rows, split>" and ws > 0
+    assert form(max_new=2, sequences=75)[0] == b"kv_attention_few<8 rows, split>"
+    for new in (5, 12):
+        name, ws = form(max_new=new)
+        assert name == b"kv_attention_few<24 rows, split>" and ws > 0
+    name, ws = form(max_new=13)
+    assert name == b"kv_attention_many" and ws >= 2 * 148 * 256 * (128 + 2) * 4
+    assert form(tokens=0)[1] == 0 and form(sequences=0)[1] == 0
+    # a workspace that is missing, too small or misaligned
+    b = _batch(max_new=13)
+    args = (FAKE, 1024, FAKE, FAKE, 1024, None)
+    assert L.mm4_kv_cache_attention(h, ctypes.byref(b), *args, None, ws, None) == _lib.MM4_ERR_WORKSPACE
+    assert L.mm4_kv_cache_attention(h, ctypes.byref(b), *args, FAKE, ws - 1, None) == _lib.MM4_ERR_WORKSPACE
+    assert L.mm4_kv_cache_attention(h, ctypes.byref(b), *args, FAKE + 8, ws, None) == INVALID
+    b = _batch(max_new=1 << 28, tokens=1 << 30)
+    assert L.mm4_kv_cache_attention(h, ctypes.byref(b), *args, FAKE, 1 << 40, None) == UNSUPPORTED
+    L.mm4_kv_cache_plan_destroy(h)
+
+
+def test_exact_division_by_the_code_range():
+    """x / 15 and x / 255 in fp32 by a product, its remainder and a correction (Markstein) equal the division, for
+    the differences of fp16 values that a group's range can be: all bit patterns of one sign against a few."""
+    f = np.float32
+    v = np.arange(0, 0x7C00, dtype=np.uint16).view(np.float16).astype(f)
+    for other in (0.0, 2.0 ** -24, 0.333, 1.0, 1000.5, 65504.0):
+        x = np.abs(v - f(np.float16(other))).astype(f)
+        x = np.concatenate([x, (v + f(np.float16(other))).astype(f)])
+        for top in (15, 255):
+            inv = f(1) / f(top)
+            q = (x * inv).astype(f)
+            # float64 holds -q * top + x and q + r * inv to well below half a unit of the fp32 result
+            r = (x.astype(np.float64) - q.astype(np.float64) * top).astype(f)
+            got = (q.astype(np.float64) + r.astype(np.float64) * np.float64(inv)).astype(f)
+            assert np.array_equal(got, (x / f(top)).astype(f)), (other, top)

@@ -282,7 +282,7 @@ def test_long_axis_is_split_and_joined(cuda, new, length):
     s.check(*s.attend())
 
 
-@pytest.mark.parametrize("new,maxNew", [(1, 1), (2, 2), (5, 5)])
+@pytest.mark.parametrize("new,maxNew", [(1, 1), (2, 2), (5, 5), (9, 12), (20, 24)])
 def test_many_sequences_on_shared_pages(cuda, new, maxNew):
     """600 sequences that share one prefix's pages: every worker's range crosses heads and sequences of more than
     32 pages each, and page-table reads start over at each of them."""
@@ -425,6 +425,110 @@ def test_captured_step_replays_with_new_lengths(cuda):
                 eO, _, tO, _ = ref.attention(Q[b:b + 1].cpu().numpy(), held[b][0], held[b][1], 1, True, plan.scale)
                 assert (np.abs(got[b:b + 1] - eO) <= tO).all(), (step, g, b)
     sync_check()
+
+
+FIRST_CALL_CAPTURED = """
+import torch
+from example_matmul_metal4_b200 import sync_check
+from example_matmul_metal4_b200.kv_cache import KVCacheBatch, KVCacheDimensions, KVCachePlan
+i32 = dict(dtype=torch.int32, device="cuda")
+for new in (1, 100):
+    plan = KVCachePlan(KVCacheDimensions(64, 64, 8, 2, 128))
+    cache = plan.allocate("cuda")
+    batch = KVCacheBatch(torch.arange(64, **i32).view(1, 64), torch.tensor([2500], **i32),
+                         torch.tensor([0, new], **i32), new, new)
+    K, V = (torch.randn(new, 2, 128, device="cuda").half() for _ in range(2))
+    Q = torch.randn(new, 8, 128, device="cuda").half()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        plan.append(K, V, cache, batch)
+        O = plan.attention(Q, cache, batch)
+        k, v = plan.read(cache, batch)
+    graph.replay()
+    graph.replay()
+    sync_check()
+    want = plan.attention(Q, cache, batch)
+    sync_check()
+    assert torch.equal(O, want) and torch.isfinite(O).all()
+    assert (k.float() - K.float()).abs().max() < 0.5
+print("captured")
+"""
+
+
+def test_first_calls_of_a_process_may_be_captured(cuda):
+    """The library's first calls on a device, made inside a stream capture in a fresh process."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL_CAPTURED], cwd=Path(__file__).resolve().parents[1],
+                       capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
+def test_wrapper_refusals(cuda):
+    """Shapes, types, devices and layouts that the wrapper turns away before any launch."""
+    import torch
+    s = Setup(cuda, [100, 60], [2, 2], 4, 2, D=64)
+    plan, cache, batch = s.plan, s.cache, s.batch
+    Q = torch.from_numpy(s.Q).to(cuda)
+    K = torch.zeros(4, 2, 64, dtype=torch.float16, device=cuda)
+    bad_q = [Q.float(), Q[:3], Q.cpu(), torch.zeros(4, 4, 128, dtype=torch.float16, device=cuda)[:, :, ::2],
+             torch.zeros(4, 64, 4, dtype=torch.float16, device=cuda).transpose(1, 2)]
+    for q in bad_q:
+        with pytest.raises(ValueError):
+            plan.attention(q, cache, batch)
+        with pytest.raises(ValueError):
+            plan.attention(Q, cache, batch, O=q)
+    for c in (cache.cpu(), cache[1:], cache.view(torch.int8), torch.cat([cache, cache], 1)[:, :plan.pageBytes]):
+        for call in (lambda: plan.attention(Q, c, batch), lambda: plan.append(K, K, c, batch),
+                     lambda: plan.read(c, batch)):
+            with pytest.raises(ValueError):
+                call()
+    with pytest.raises(ValueError):
+        plan.append(K[:, :1], K, cache, batch)
+    with pytest.raises(ValueError):
+        plan.read(cache, batch, K=K)
+    for lse in (torch.zeros(4, 4, device=cuda).half(), torch.zeros(4, 3, device=cuda), torch.zeros(4, 4),
+                torch.zeros(4, 8, device=cuda)[:, ::2]):
+        with pytest.raises(ValueError):
+            plan.attention(Q, cache, batch, lse=lse)
+    with pytest.raises(MM4Error):  # rows that are not 8 elements apart
+        plan.attention(torch.zeros(4, 260, dtype=torch.float16, device=cuda)[:, :256].view(4, 4, 64), cache, batch)
+    with pytest.raises(MM4Error):  # a base that is not 16-byte aligned
+        plan.attention(torch.zeros(4 * 256 + 4, dtype=torch.float16, device=cuda)[4:].view(4, 4, 64), cache, batch)
+    many = KVCacheBatch(batch.pageTable, batch.lengths, batch.offsets, 4, 40)
+    small = torch.empty(plan.attention_workspace_bytes(many) - 16, dtype=torch.uint8, device=cuda)
+    with pytest.raises(MM4Error):
+        plan.attention(Q, cache, many, workspace=small)
+    i32 = dict(dtype=torch.int32, device=cuda)
+    t, ln, off = torch.zeros(2, 3, **i32), torch.zeros(2, **i32), torch.zeros(3, **i32)
+    for args in ((t.long(), ln, off), (t[:1], ln, off), (t, ln[:1], off), (t, ln, off[:2]), (t.T, ln, off),
+                 (t.view(-1), ln, off), (t, ln, off.cpu())):
+        with pytest.raises(ValueError):
+            KVCacheBatch(*args, 4, 2)
+    with pytest.raises(ValueError):
+        KVCacheBatch(t, ln, off, -1, 1)
+    sync_check()
+
+
+def test_given_workspace_and_empty_batches(cuda):
+    """A workspace of the caller's with anything in it; batches without rows and without sequences do nothing."""
+    import torch
+    s = Setup(cuda, [3000], [20], 8, 2)
+    ws = torch.full((s.plan.attention_workspace_bytes(s.batch) + 64,), 0xFF, dtype=torch.uint8, device=cuda)
+    s.check(*s.attend(workspace=ws))
+    i32 = dict(dtype=torch.int32, device=cuda)
+    for seqs, tokens in ((0, 3), (2, 0), (0, 0)):
+        b = KVCacheBatch(torch.zeros(seqs, 4, **i32), torch.zeros(seqs, **i32), torch.zeros(seqs + 1, **i32), tokens, 1)
+        K = torch.ones(tokens, 2, 128, dtype=torch.float16, device=cuda)
+        O = torch.ones(tokens, 8, 128, dtype=torch.float16, device=cuda)
+        before = s.cache.clone()
+        s.plan.append(K, K, s.cache, b)
+        s.plan.read(s.cache, b, K=K, V=K.clone())
+        s.plan.attention(O.clone(), s.cache, b, O=O)
+        sync_check()
+        assert (K == 1).all() and (O == 1).all() and torch.equal(before, s.cache)
 
 
 def test_two_streams_at_once(cuda):
