@@ -78,7 +78,8 @@ class KVCachePlan:
         _lib.check(self._L.mm4_kv_cache_plan_create(ctypes.byref(h), ctypes.byref(d)))
         self._h = h
         import torch
-        self._f16, self._u8, self._device = torch.float16, torch.uint8, torch._C._cuda_getDevice
+        self._f16, self._u8, self._f32 = torch.float16, torch.uint8, torch.float32
+        self._empty_like, self._device = torch.empty_like, torch._C._cuda_getDevice
         self.pageBytes = int(self._L.mm4_kv_cache_page_bytes(h))
         self.cacheBytes = int(self._L.mm4_kv_cache_bytes(h))
 
@@ -124,18 +125,22 @@ class KVCachePlan:
     def read(self, cache, batch, K=None, V=None, stream=None):
         """(K, V): the fp16 values [tokens][Hk][K] that an append of this batch left in the cache
         (mm4_kv_cache_read). Padding rows of given tensors are left as they were; of new ones they are
-        uninitialised. Without K and V, the two are halves of one new tensor."""
+        uninitialised."""
         Hk, D = self.dims.Hk, self.dims.K
         cp = self._cache(cache, batch)
         if K is None and V is None:
-            pair = cache.new_empty((2, batch.tokens, Hk, D), dtype=self._f16)
-            if stream is not None:
-                pair.record_stream(stream)
-            K, V = pair.unbind(0)
+            K = cache.new_empty((batch.tokens, Hk, D), dtype=self._f16)
+            V = self._empty_like(K)
+            if stream is not None:  # not reused before that stream is done with them
+                K.record_stream(stream)
+                V.record_stream(stream)
+            kp, vp, ks = K.data_ptr(), V.data_ptr(), Hk * D
+            vs = ks
         elif K is None or V is None:
             raise ValueError("give both K and V, or neither")
-        kp, ks = self._rows("K", K, Hk, batch)
-        vp, vs = self._rows("V", V, Hk, batch)
+        else:
+            kp, ks = self._rows("K", K, Hk, batch)
+            vp, vs = self._rows("V", V, Hk, batch)
         _lib.check(self._L.mm4_kv_cache_read(self._h, batch._ref, cp, kp, ks, vp, vs, _lib.stream_handle(stream)))
         return K, V
 
@@ -155,7 +160,7 @@ class KVCachePlan:
         qp, qs = self._rows("Q", Q, Hq, batch)
         cp = self._cache(cache, batch)
         if O is None:
-            O = Q.new_empty((batch.tokens, Hq, D))
+            O = self._empty_like(Q) if Q.is_contiguous() else Q.new_empty((batch.tokens, Hq, D))
             if stream is not None:
                 O.record_stream(stream)  # not reused before that stream is done with it
             op, os_ = O.data_ptr(), Hq * D
@@ -163,7 +168,7 @@ class KVCachePlan:
             op, os_ = self._rows("O", O, Hq, batch)
         lp = None
         if lse is not None:
-            if lse.shape != (batch.tokens, Hq) or str(lse.dtype) != "torch.float32" or not lse.is_contiguous() or \
+            if lse.shape != (batch.tokens, Hq) or lse.dtype is not self._f32 or not lse.is_contiguous() or \
                     lse.get_device() != batch.device:
                 raise ValueError(f"lse must be a contiguous CUDA fp32 tensor of shape {(batch.tokens, Hq)}")
             lp = lse.data_ptr()
