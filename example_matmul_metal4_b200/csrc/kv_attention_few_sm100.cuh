@@ -41,10 +41,10 @@ struct KvFew {
   static constexpr int ROWS = 8 * NT;
   static constexpr int ROW_BYTES = KvRow<D, BITS>::BYTES;
   static constexpr int STAGE_BYTES = 2 * KVF_TK * ROW_BYTES;  // K rows of a tile, then V rows
-  // Warps that compute: 14 with 128 registers a thread, or 7 with more. What
-  // bounds the arithmetic is the SM's logic and fp16 instructions, not their
-  // number; fewer warps leave more of the ring to each.
-  static constexpr int WARPS = NT == 1 && STAGE_BYTES <= 5120 ? 14 : 7;
+  // Warps that compute: 15 with 128 registers a thread, or 7 with more (9 to 12
+  // warps get 168). 14 with three tiles each in flight: 99 us where 15 with two
+  // take 97.
+  static constexpr int WARPS = NT == 1 && STAGE_BYTES <= 5120 ? 15 : 7;
   static constexpr int THREADS = 32 * (WARPS + 1);
   static constexpr int PARTS = (WARPS + 1) / 2;               // of the join inside a CTA (TEAM)
   static constexpr int JOIN_BYTES = TEAM ? PARTS * KvPartial<D, ROWS>::FLOATS * 4 : 0;
@@ -734,8 +734,27 @@ __global__ void __launch_bounds__(256) kv_attention_join_kernel(const KvAttnArgs
   for (int i = 0; i < V; ++i) acc[i] = 0.f;
   if (row < rows) {
     auto slot = [&](int i) { return a.partials + (2 * (first + i) + (i == 0 ? 1 : 0)) * F; };
+    auto load = [&](int i, float (&v)[V]) {
+      const float* src = slot(i) + (row0 + row) * D + lane * V;
+      if constexpr (V == 4) {
+        const float4 x = __ldcg(reinterpret_cast<const float4*>(src));
+        v[0] = x.x;
+        v[1] = x.y;
+        v[2] = x.z;
+        v[3] = x.w;
+      } else {
+        const float2 x = __ldcg(reinterpret_cast<const float2*>(src));
+        v[0] = x.x;
+        v[1] = x.y;
+      }
+    };
     for (int i0 = c0; i0 < c1; i0 += 32) {
       const int n = min(32, c1 - i0);
+      // The first O rows are on their way while weights are formed.
+      float early[8][V];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < n) load(i0 + i, early[i]);
       float pm = KV_NO_MAX, pl = 0.f;
       if (lane < n) {
         const float2 ml = __ldcg(reinterpret_cast<const float2*>(slot(i0 + lane) + ROWS * D + 2 * (row0 + row)));
@@ -751,21 +770,20 @@ __global__ void __launch_bounds__(256) kv_attention_join_kernel(const KvAttnArgs
 #pragma unroll
       for (int i = 0; i < V; ++i) acc[i] *= f;
       ls += kv_warp_sum(w * pl);
-#pragma unroll 8
-      for (int i = 0; i < n; ++i) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
         const float wi = __shfl_sync(0xffffffffu, w, i);
-        const float* src = slot(i0 + i) + (row0 + row) * D + lane * V;
-        if constexpr (V == 4) {
-          const float4 v = __ldcg(reinterpret_cast<const float4*>(src));
-          acc[0] += wi * v.x;
-          acc[1] += wi * v.y;
-          acc[2] += wi * v.z;
-          acc[3] += wi * v.w;
-        } else {
-          const float2 v = __ldcg(reinterpret_cast<const float2*>(src));
-          acc[0] += wi * v.x;
-          acc[1] += wi * v.y;
-        }
+        if (i < n)
+#pragma unroll
+          for (int e = 0; e < V; ++e) acc[e] += wi * early[i][e];
+      }
+#pragma unroll 8
+      for (int i = 8; i < n; ++i) {
+        const float wi = __shfl_sync(0xffffffffu, w, i);
+        float v[V];
+        load(i0 + i, v);
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[e] += wi * v[e];
       }
     }
   }

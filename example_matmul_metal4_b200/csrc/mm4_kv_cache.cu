@@ -162,7 +162,7 @@ Form attention_form(const mm4_kv_cache_plan* p, const mm4_kv_cache_batch* b) {
   f.kind = rows <= 8 ? Form::FEW8 : rows <= 16 ? Form::FEW16 : Form::FEW24;
   f.team = rows <= 16 && room <= kTeamTokens && static_cast<long long>(b->sequences) * p->d.heads_kv <= kTeamUnits;
   const int nt = rows <= 8 ? 1 : rows <= 16 ? 2 : 3;
-  const int warps = nt == 1 ? 14 : 7;  // at most
+  const int warps = nt == 1 ? 15 : 7;  // at most
   if (!f.team) f.workspace = sizeof(float) * 2 * kMaxCtas * warps * 8 * nt * (p->d.head_dim + 2);
   static const char* const names[3][2] = {{"kv_attention_few<8 rows, split>", "kv_attention_few<8 rows, team>"},
                                           {"kv_attention_few<16 rows, split>", "kv_attention_few<16 rows, team>"},
@@ -196,7 +196,7 @@ mm4_status launch_few(KvAttnArgs& a, int sms, cudaStream_t st) {
   if (rc != MM4_OK) return rc;
   const long long units = static_cast<long long>(a.kb.sequences) * a.kb.heads_kv;
   const unsigned grid = static_cast<unsigned>(TEAM ? std::min<long long>(units, sms) : sms);
-  static_assert(Cfg::WARPS <= (NT == 1 ? 14 : 7), "attention_form sizes the workspace for this many");
+  static_assert(Cfg::WARPS <= (NT == 1 ? 15 : 7), "attention_form sizes the workspace for this many");
   a.workers = sms * Cfg::WARPS;
   kv_attention_few_kernel<D, BITS, NT, TEAM><<<grid, Cfg::THREADS, Cfg::SMEM_BYTES, st>>>(a);
   cudaError_t e = cudaGetLastError();
