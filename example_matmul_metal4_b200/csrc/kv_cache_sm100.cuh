@@ -271,64 +271,79 @@ __device__ __forceinline__ float kv_divide_by_top(float x) {
 // each of its tokens; the four lanes of a group of 32 find its range by two
 // shuffles of one register. Its floor are the bytes it moves: 512 in and 160 out
 // per token and head at D = 128 in 4 bits, 23 us for four prompts of up to 4096
-// tokens and 16 heads; it takes 60 us (184 instructions for 8 elements a lane, issue
-// slots 70 % busy).
+// tokens and 16 heads; it takes 51 us (142 instructions for 8 elements a lane, issue
+// slots 64 % busy).
 template <int D, int BITS>
-__global__ void __launch_bounds__(KV_IO_WARPS * 32, 8) kv_append_kernel(const KvIoArgs a) {
+__global__ void __launch_bounds__(KV_IO_WARPS * 32, 6) kv_append_kernel(const KvIoArgs a) {
   constexpr int TOP = (1 << BITS) - 1;
   using Row = KvRow<D, BITS>;
   const int lane = threadIdx.x & 31;
   const int half_vecs = a.kb.heads_kv * (D / 8);  // vectors of K; as many of V
   KvIoWork work;
   if (!kv_io_work<Row::BYTES>(a, lane, &work)) return;
+  // What does not change from token to token: where this lane's vectors come
+  // from, and where their codes and parameters go in a page (-1: no vector).
+  const __half* src[KV_IO_VECS];
+  int to[KV_IO_VECS], par[KV_IO_VECS];
+#pragma unroll
+  for (int k = 0; k < KV_IO_VECS; ++k) {
+    const int v = work.vec0 + 32 * k;
+    const bool is_v = v >= half_vecs;
+    const __half* rows = is_v ? a.in_v + (v - half_vecs) * 8 : a.in_k + v * 8;
+    src[k] = rows + work.t0 * (is_v ? a.v_stride : a.k_stride);
+    int d;
+    const int row = kv_vector_row<D, BITS>(a.kb, v, half_vecs, &d);
+    to[k] = v < 2 * half_vecs ? row + d * BITS / 8 : -1;
+    par[k] = row + Row::CODES + d / KV_GROUP * 4;
+  }
 #pragma unroll 1
   for (int i = 0; i < work.n; ++i) {
-    const long long t = work.t0 + i;
-    uint4 in[KV_IO_VECS];
+    uint32_t w[KV_IO_VECS][4];
+    uint32_t odd = 0;
 #pragma unroll
     for (int k = 0; k < KV_IO_VECS; ++k) {
-      const int v = work.vec0 + 32 * k;
-      in[k] = make_uint4(0u, 0u, 0u, 0u);
-      if (v >= 2 * half_vecs) continue;
-      const __half* src =
-          v < half_vecs ? a.in_k + t * a.k_stride + v * 8 : a.in_v + t * a.v_stride + (v - half_vecs) * 8;
-      in[k] = __ldg(reinterpret_cast<const uint4*>(src));
+      uint4 in = make_uint4(0u, 0u, 0u, 0u);
+      if (to[k] >= 0) in = __ldg(reinterpret_cast<const uint4*>(src[k]));
+      src[k] += work.vec0 + 32 * k >= half_vecs ? a.v_stride : a.k_stride;
+      w[k][0] = in.x;
+      w[k][1] = in.y;
+      w[k][2] = in.z;
+      w[k][3] = in.w;
     }
     const long long place = __shfl_sync(0xffffffffu, work.place, i);
     if (place < 0) continue;
     uint8_t* page = a.cache + place;
+    // NaN counts as 0 and infinities as the largest finite value: exponents of
+    // all ones carry into the sign bit here.
 #pragma unroll
-    for (int k = 0; k < KV_IO_VECS; ++k) {
-      const int v = work.vec0 + 32 * k;
-      uint32_t w[4] = {in[k].x, in[k].y, in[k].z, in[k].w};
-      // NaN counts as 0 and infinities as the largest finite value: exponents of
-      // all ones carry into the sign bit here.
-      uint32_t odd = 0;
+    for (int k = 0; k < KV_IO_VECS; ++k)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) odd |= (w[j] & 0x7FFF7FFFu) + 0x04000400u;
-      if ((odd & 0x80008000u) != 0) {
+      for (int j = 0; j < 4; ++j) odd |= (w[k][j] & 0x7FFF7FFFu) + 0x04000400u;
+    if ((odd & 0x80008000u) != 0) {
+#pragma unroll
+      for (int k = 0; k < KV_IO_VECS; ++k)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           uint32_t fixed = 0;
 #pragma unroll
           for (int h = 0; h < 32; h += 16) {
-            uint32_t x = (w[j] >> h) & 0xFFFFu;
-            if ((x & 0x7FFFu) > 0x7C00u) x = 0;                                  // NaN
-            if ((x & 0x7FFFu) == 0x7C00u) x = (x & 0x8000u) | 0x7BFFu;           // infinity
+            uint32_t x = (w[k][j] >> h) & 0xFFFFu;
+            if ((x & 0x7FFFu) > 0x7C00u) x = 0;                         // NaN
+            if ((x & 0x7FFFu) == 0x7C00u) x = (x & 0x8000u) | 0x7BFFu;  // infinity
             fixed |= x << h;
           }
-          w[j] = fixed;
+          w[k][j] = fixed;
         }
-      }
-      const __half2 range = kv_group_range(w);
+    }
+#pragma unroll
+    for (int k = 0; k < KV_IO_VECS; ++k) {
+      const __half2 range = kv_group_range(w[k]);
       const __half zero = __low2half(range);
       const float lo = __half2float(zero), hi = -__half2float(__high2half(range));
       const __half scale = __float2half_rz(kv_divide_by_top<TOP>(__fsub_rn(hi, lo)));
       uint32_t code[8];
-      kv_quantise8(w, lo, __half2float(scale), TOP, code);
-      if (v >= 2 * half_vecs) continue;
-      int d;
-      uint8_t* dst = page + kv_vector_row<D, BITS>(a.kb, v, half_vecs, &d);
+      kv_quantise8(w[k], lo, __half2float(scale), static_cast<float>(TOP), code);
+      if (to[k] < 0) continue;
       // Codes are packed by multiplication and addition modulo 2^32, KV_CODE with
       // them, and what that adds up to is taken off.
       if constexpr (BITS == 4) {
@@ -336,7 +351,7 @@ __global__ void __launch_bounds__(KV_IO_WARPS * 32, 8) kv_append_kernel(const Kv
         uint32_t packed = code[7];
 #pragma unroll
         for (int j = 6; j >= 0; --j) packed = packed * 16u + code[j];
-        *reinterpret_cast<uint32_t*>(dst + d / 2) = packed - TAKE;
+        *reinterpret_cast<uint32_t*>(page + to[k]) = packed - TAKE;
       } else {
         constexpr uint32_t TAKE = KV_CODE * 0x01010101u;
         uint32_t packed[2] = {code[3], code[7]};
@@ -345,10 +360,9 @@ __global__ void __launch_bounds__(KV_IO_WARPS * 32, 8) kv_append_kernel(const Kv
           packed[0] = packed[0] * 256u + code[j];
           packed[1] = packed[1] * 256u + code[4 + j];
         }
-        *reinterpret_cast<uint2*>(dst + d) = make_uint2(packed[0] - TAKE, packed[1] - TAKE);
+        *reinterpret_cast<uint2*>(page + to[k]) = make_uint2(packed[0] - TAKE, packed[1] - TAKE);
       }
-      if ((lane & 3) == 0)
-        *reinterpret_cast<__half2*>(dst + Row::CODES + d / KV_GROUP * 4) = __halves2half2(scale, zero);
+      if ((lane & 3) == 0) *reinterpret_cast<__half2*>(page + par[k]) = __halves2half2(scale, zero);
     }
   }
 }
