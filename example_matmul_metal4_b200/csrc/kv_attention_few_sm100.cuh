@@ -185,7 +185,7 @@ __global__ void __launch_bounds__(KvFew<D, BITS, NT, TEAM>::THREADS, 1) kv_atten
       s.n = warp;
     } else {
       constexpr int R = Cfg::ROWS;
-      const long long total = kv_total_tiles<KVF_TK, R>(kb, kb.sequences, a.group, lane) * kb.heads_kv;
+      const long long total = kv_total_tiles<KVF_TK, R>(kb, a.group, lane) * kb.heads_kv;
       const long long active = min(static_cast<long long>(a.workers), total);
       const long long w = static_cast<long long>(warp) * gridDim.x + blockIdx.x;
       if (w < active) {
@@ -711,13 +711,36 @@ __global__ void __launch_bounds__(256) kv_attention_join_kernel(const KvAttnArgs
   const int blocks = kv_blocks<ROWS>(kb, s, a.group), block = blockIdx.y / chunks;
   const int row0 = blockIdx.y % chunks * a.join_rows;  // in the unit
   const int rows = min(min(min(s.n, kb.max_new) * a.group - block * ROWS, ROWS) - row0, a.join_rows);
-  const long long total = kv_total_tiles<TK, ROWS>(kb, kb.sequences, a.group, lane) * kb.heads_kv;
+  // Tiles of all sequences and of those before this one, by the whole block.
+  __shared__ long long sums[2][8];
+  long long all = 0, ahead = 0;
+  for (int i = threadIdx.x; i < kb.sequences; i += 256) {
+    const int t = kv_sequence_tiles<TK, ROWS>(kb, i, a.group);
+    all += t;
+    if (i < b) ahead += t;
+  }
+#pragma unroll
+  for (int k = 16; k > 0; k >>= 1) {
+    all += __shfl_xor_sync(0xffffffffu, all, k);
+    ahead += __shfl_xor_sync(0xffffffffu, ahead, k);
+  }
+  if (lane == 0) {
+    sums[0][warp] = all;
+    sums[1][warp] = ahead;
+  }
+  __syncthreads();
+  all = ahead = 0;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    all += sums[0][k];
+    ahead += sums[1][k];
+  }
+  const long long total = all * kb.heads_kv;
   const long long active = min(static_cast<long long>(a.workers), total);
   const int tiles = kv_tiles<TK>(s);
   long long first = 0, last = 0;
   if (rows > 0) {
-    const long long x0 = kv_total_tiles<TK, ROWS>(kb, b, a.group, lane) * kb.heads_kv +
-                         (static_cast<long long>(h) * blocks + block) * tiles;
+    const long long x0 = ahead * kb.heads_kv + (static_cast<long long>(h) * blocks + block) * tiles;
     first = kv_worker_of(x0, total, active);
     last = kv_worker_of(x0 + tiles - 1, total, active);
   }

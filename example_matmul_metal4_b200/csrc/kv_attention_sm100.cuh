@@ -71,11 +71,11 @@ __device__ __forceinline__ int kv_sequence_tiles(const KvBatch& kb, int b, int g
   return kv_tiles<TK>(s) * kv_blocks<ROWS>(kb, s, group);
 }
 
-// Sum of kv_sequence_tiles over the first n sequences, by one warp.
+// Sum of kv_sequence_tiles over all sequences, by one warp.
 template <int TK, int ROWS>
-__device__ __forceinline__ long long kv_total_tiles(const KvBatch& kb, int n, int group, int lane) {
+__device__ __forceinline__ long long kv_total_tiles(const KvBatch& kb, int group, int lane) {
   long long sum = 0;
-  for (int b = lane; b < n; b += 32) sum += kv_sequence_tiles<TK, ROWS>(kb, b, group);
+  for (int b = lane; b < kb.sequences; b += 32) sum += kv_sequence_tiles<TK, ROWS>(kb, b, group);
 #pragma unroll
   for (int s = 16; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
   return sum;

@@ -380,11 +380,11 @@ typedef struct mm4_kv_cache_plan mm4_kv_cache_plan;
  *  max_new    most rows of one sequence (mm4_kv_cache_attention only).
  * A sequence may have no rows in a call, length 0, or more rows than its length:
  * rows that come to lie before position 0 are not written by append or read,
- * and attend to nothing. Page-table entries behind a sequence's length are not
- * read. What the kernels find wrong in these arrays - a page number outside the
- * pool, a length beyond the page table, more rows than max_new, offsets out
- * of order or beyond tokens - never leads to an access out of bounds: such
- * tokens are left out by append and read, the outputs of such sequences are
+ * and with causal = 1 attend to nothing. Page-table entries behind a sequence's
+ * length are not read. What the kernels find wrong in these arrays - a page
+ * number outside the pool, a length beyond the page table, more rows than max_new,
+ * offsets out of order or beyond tokens - never leads to an access out of bounds:
+ * such tokens are left out by append and read, the outputs of such sequences are
  * unspecified in attention, and mm4_check() reports MM4_ERR_INVALID. */
 typedef struct mm4_kv_cache_batch {
   int32_t sequences;
