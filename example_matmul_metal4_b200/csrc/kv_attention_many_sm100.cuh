@@ -649,6 +649,10 @@ __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const
         mbar_arrive(&p_full[2 * ti + sl]);
       }
       if (!ok) break;
+      // A row that has seen no key: ex2_poly2 gives 2^-125, not 0, for its masked
+      // scores. The sum of any other row is about 1 or more (its maximum counts 1); a NaN
+      // stays.
+      if (l < 0x1p-100f) l = 0.f;
       // The unit's last S_i is complete: Q_i takes the next unit's rows.
       more = kvm_next(a, ROWS, walk, sg);
       if (more) {

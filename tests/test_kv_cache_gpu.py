@@ -246,6 +246,17 @@ def test_rows_that_attend_to_nothing(cuda, new, maxNew):
             assert (got[1:1 + new - 5] == 0).all()
 
 
+@pytest.mark.parametrize("new,length", [(1, 0), (9, 5), (60, 30), (300, 40)])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_rows_that_attend_to_nothing_at_head_dim_64(cuda, bits, new, length):
+    """O = 0 and lse = -inf exactly, where part of the exponentials comes from a polynomial that never gives 0."""
+    s = Setup(cuda, [length, 700, length], [new, new, new], 4, 2, D=64, bits=bits, page=16)
+    O, lse = s.attend()
+    s.check(O, lse)
+    empty = new - min(new, length)
+    assert (O[:empty] == 0).all() and (lse[:empty] == -float("inf")).all()
+
+
 @pytest.mark.parametrize("new", [1, 12, 70])
 def test_large_scores(cuda, new):
     """Keys that grow along the sequence and a large scale, so the running maximum moves far and often."""
