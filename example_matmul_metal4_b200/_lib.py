@@ -191,6 +191,23 @@ def stream_handle(stream=None) -> int | None:
     return stream.cuda_stream or None
 
 
+def new_on_stream(stream, make, returned: bool = True):
+    """make() (a new CUDA tensor, or a tuple of them) for kernels that run on the torch stream `stream` (None: the
+    current one). The blocks come from that stream's pool: one of the current stream's pool may have been freed with
+    work of the current stream on it still pending, which a kernel on `stream` would not wait for. What is `returned` to
+    the caller is not reused before the current stream, on which they go on, is done with it."""
+    if stream is None:
+        return make()
+    import torch
+    with torch.cuda.stream(stream):
+        made = make()
+    if returned:
+        here = torch.cuda.current_stream()
+        for t in made if isinstance(made, tuple) else (made,):
+            t.record_stream(here)
+    return made
+
+
 def sync_check(stream=None) -> None:
     """Synchronises the stream and raises MM4Error if a kernel recorded an error."""
     check(lib().mm4_check(stream_handle(stream)))

@@ -65,7 +65,11 @@ class KVCacheBatch:
 
 class KVCachePlan:
     """Cache geometry and attention options. `causal`: a token attends to itself and what lies before it (else to
-    all its sequence has cached); `scale` as in AttentionPlan. Immutable; may be used from several streams."""
+    all its sequence has cached); `scale` as in AttentionPlan. Immutable; may be used from several streams.
+
+    `stream` of a call is a torch stream of the tensors' device (None: the current one). Its kernels follow what that
+    stream holds already; inputs that another stream writes need a wait of the caller's, as do outputs read elsewhere.
+    Tensors that a call allocates come from the memory of that stream."""
 
     def __init__(self, dims: KVCacheDimensions, causal: bool = True, scale: float | None = None):
         self._L = _lib.lib()
@@ -94,7 +98,7 @@ class KVCachePlan:
         import torch
         return torch.zeros(self.dims.pages, self.pageBytes, dtype=torch.uint8, device=device)
 
-    def _cache(self, cache, batch):
+    def _cache(self, cache, batch, stream):
         if cache.dtype is not self._u8 or cache.numel() != self.cacheBytes or not cache.is_contiguous():
             raise ValueError(f"cache must be a contiguous CUDA uint8 tensor of {self.cacheBytes} bytes")
         dev = batch.device
@@ -102,6 +106,8 @@ class KVCachePlan:
             raise ValueError("cache and batch must be on one device")
         if dev != self._device():
             raise ValueError(f"the tensors are on device {dev}, which is not the current CUDA device")
+        if stream is not None and stream.device_index != dev:
+            raise ValueError(f"the stream belongs to device {stream.device_index}, the tensors are on device {dev}")
         return cache.data_ptr()
 
     def _rows(self, name, t, heads, batch):
@@ -119,7 +125,7 @@ class KVCachePlan:
         projection are) into the cache (mm4_kv_cache_append)."""
         kp, ks = self._rows("K", K, self.dims.Hk, batch)
         vp, vs = self._rows("V", V, self.dims.Hk, batch)
-        _lib.check(self._L.mm4_kv_cache_append(self._h, batch._ref, kp, ks, vp, vs, self._cache(cache, batch),
+        _lib.check(self._L.mm4_kv_cache_append(self._h, batch._ref, kp, ks, vp, vs, self._cache(cache, batch, stream),
                                                _lib.stream_handle(stream)))
 
     def read(self, cache, batch, K=None, V=None, stream=None):
@@ -127,13 +133,14 @@ class KVCachePlan:
         (mm4_kv_cache_read). Padding rows of given tensors are left as they were; of new ones they are
         uninitialised."""
         Hk, D = self.dims.Hk, self.dims.K
-        cp = self._cache(cache, batch)
+        cp = self._cache(cache, batch, stream)
         if K is None and V is None:
-            K = cache.new_empty((batch.tokens, Hk, D), dtype=self._f16)
-            V = self._empty_like(K)
-            if stream is not None:  # not reused before that stream is done with them
-                K.record_stream(stream)
-                V.record_stream(stream)
+            if stream is None:
+                K = cache.new_empty((batch.tokens, Hk, D), dtype=self._f16)
+                V = self._empty_like(K)
+            else:
+                K, V = _lib.new_on_stream(stream, lambda: tuple(
+                    cache.new_empty((batch.tokens, Hk, D), dtype=self._f16) for _ in range(2)))
             kp, vp, ks = K.data_ptr(), V.data_ptr(), Hk * D
             vs = ks
         elif K is None or V is None:
@@ -158,11 +165,12 @@ class KVCachePlan:
         `workspace`: a CUDA uint8 tensor; by default each call takes one from torch's allocator."""
         Hq, D = self.dims.Hq, self.dims.K
         qp, qs = self._rows("Q", Q, Hq, batch)
-        cp = self._cache(cache, batch)
+        cp = self._cache(cache, batch, stream)
         if O is None:
-            O = self._empty_like(Q) if Q.is_contiguous() else Q.new_empty((batch.tokens, Hq, D))
-            if stream is not None:
-                O.record_stream(stream)  # not reused before that stream is done with it
+            if stream is None and Q.is_contiguous():
+                O = self._empty_like(Q)
+            else:
+                O = _lib.new_on_stream(stream, lambda: Q.new_empty((batch.tokens, Hq, D)))
             op, os_ = O.data_ptr(), Hq * D
         else:
             op, os_ = self._rows("O", O, Hq, batch)
@@ -176,9 +184,8 @@ class KVCachePlan:
         wp = None
         if nbytes:
             if workspace is None:
-                workspace = cache.new_empty(nbytes)
-                if stream is not None:
-                    workspace.record_stream(stream)
+                workspace = cache.new_empty(nbytes) if stream is None else \
+                    _lib.new_on_stream(stream, lambda: cache.new_empty(nbytes), returned=False)
             elif workspace.get_device() != batch.device or not workspace.is_contiguous():
                 raise ValueError("workspace must be a contiguous tensor on the batch's device")
             else:

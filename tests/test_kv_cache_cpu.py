@@ -183,3 +183,122 @@ def test_exact_division_by_the_code_range():
             r = (x.astype(np.float64) - q.astype(np.float64) * top).astype(f)
             got = (q.astype(np.float64) + r.astype(np.float64) * np.float64(inv)).astype(f)
             assert np.array_equal(got, (x / f(top)).astype(f)), (other, top)
+
+
+# ----------------------------------------------------------------------------------------------------------
+# the wrapper with stand-ins for tensors, streams and the library
+# ----------------------------------------------------------------------------------------------------------
+
+class FakeTensor:
+    """What the wrapper asks of a CUDA tensor. `pool` is the stream whose memory it was allocated from."""
+
+    def __init__(self, shape, dtype, env, pool=None):
+        import math
+        self.shape, self.dtype, self.env, self.pool, self.recorded = tuple(shape), dtype, env, pool, []
+        self.n, self.is_cuda = math.prod(self.shape), True
+
+    def _new(self, shape, dtype):
+        t = FakeTensor([shape] if isinstance(shape, int) else shape, dtype, self.env, self.env.current)
+        self.env.made.append(t)
+        return t
+
+    def new_empty(self, shape, dtype=None):
+        return self._new(shape, dtype or self.dtype)
+
+    def stride(self):
+        strides, n = [], 1
+        for d in reversed(self.shape):
+            strides.append(n)
+            n *= d
+        return tuple(reversed(strides))
+
+    def numel(self):
+        return self.n
+
+    def dim(self):
+        return len(self.shape)
+
+    def is_contiguous(self):
+        return True
+
+    def get_device(self):
+        return 0
+
+    def data_ptr(self):
+        return FAKE
+
+    def record_stream(self, stream):
+        self.recorded.append(stream)
+
+
+class FakeStream:
+    def __init__(self, device_index=0):
+        self.device_index, self.cuda_stream = device_index, 0x1234
+
+
+class FakeEnv:
+    """The wrapper on device 0 with torch's current stream and the library's entry points replaced."""
+
+    def __init__(self, monkeypatch, max_new=40):
+        import contextlib
+
+        import torch
+        from example_matmul_metal4_b200.kv_cache import KVCacheBatch, KVCacheDimensions, KVCachePlan
+        self.made, self.calls, self.main = [], [], FakeStream()
+        self.current = self.main
+
+        @contextlib.contextmanager
+        def on(stream):
+            kept, self.current = self.current, stream
+            yield
+            self.current = kept
+
+        monkeypatch.setattr(torch.cuda, "stream", on)
+        monkeypatch.setattr(torch.cuda, "current_stream", lambda *a: self.current)
+        monkeypatch.setattr(_lib, "stream_handle", lambda stream=None: None)
+        i32 = torch.int32
+        self.plan = KVCachePlan(KVCacheDimensions(7, 64, 8, 2, 128))
+        self.batch = KVCacheBatch(FakeTensor((3, 4), i32, self), FakeTensor((3,), i32, self),
+                                  FakeTensor((4,), i32, self), 5, max_new)
+        real, env = self.plan._L, self
+
+        class Library:
+            def __getattr__(self, name):
+                if name in ("mm4_kv_cache_append", "mm4_kv_cache_read", "mm4_kv_cache_attention"):
+                    return lambda *a: env.calls.append((name, a)) or 0
+                return getattr(real, name)
+
+        self.plan._L, self.plan._device = Library(), lambda: 0
+        self.plan._empty_like = lambda t: t._new(t.shape, t.dtype)
+        self.cache = FakeTensor((7, self.plan.pageBytes), torch.uint8, self)
+        self.Q = FakeTensor((5, 8, 128), torch.float16, self)
+        self.K = FakeTensor((5, 2, 128), torch.float16, self)
+
+
+def test_tensors_that_a_call_makes_come_from_the_memory_of_its_stream(monkeypatch):
+    """A block of the current stream's pool may still be written by pending work of that stream, which a kernel on
+    another stream does not wait for. What is returned is kept from reuse until the caller's stream is done with it."""
+    env = FakeEnv(monkeypatch)
+    side = FakeStream()
+    for stream in (None, side):
+        env.made.clear()
+        O = env.plan.attention(env.Q, env.cache, env.batch, stream=stream)
+        K, V = env.plan.read(env.cache, env.batch, stream=stream)
+        assert len(env.made) == 4 and env.current is env.main  # O, workspace, K, V
+        for t in env.made:
+            assert t.pool is (env.main if stream is None else side)
+        for t in (O, K, V):
+            assert t.recorded == ([] if stream is None else [env.main])
+        assert O.shape == (5, 8, 128) and K.shape == V.shape == (5, 2, 128)
+    assert len(env.calls) == 4
+
+
+def test_a_stream_of_another_device_is_refused(monkeypatch):
+    env = FakeEnv(monkeypatch)
+    for call in (lambda s: env.plan.append(env.K, env.K, env.cache, env.batch, stream=s),
+                 lambda s: env.plan.read(env.cache, env.batch, stream=s),
+                 lambda s: env.plan.attention(env.Q, env.cache, env.batch, stream=s)):
+        with pytest.raises(ValueError, match="device 1"):
+            call(FakeStream(1))
+        call(FakeStream(0))
+    assert len(env.calls) == 3

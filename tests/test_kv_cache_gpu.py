@@ -560,6 +560,32 @@ def test_two_streams_at_once(cuda):
         assert torch.equal(x, wa) and torch.equal(y, wb)
 
 
+@pytest.mark.parametrize("new", [1, 40])
+def test_memory_freed_on_the_current_stream_with_work_pending(cuda, new):
+    """Blocks of the sizes of O, the workspace, K and V are freed on the current stream while it still has to write
+    them; calls on another stream must not be given them."""
+    import torch
+    s = Setup(cuda, [3000], [new], 8, 2)
+    Q = torch.from_numpy(s.Q).to(cuda)
+    want = s.plan.attention(Q, s.cache, s.batch)
+    K, V = s.plan.read(s.cache, s.batch)
+    nbytes = s.plan.attention_workspace_bytes(s.batch)
+    assert nbytes > 0
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(3):
+        held = [torch.empty_like(t) for t in (want, K, V) for _ in range(3)]
+        held += [torch.empty(nbytes, dtype=torch.uint8, device=cuda) for _ in range(3)]
+        torch.cuda._sleep(20_000_000)  # about 10 ms
+        for t in held:
+            t.fill_(77)
+        del held, t
+        O = s.plan.attention(Q, s.cache, s.batch, stream=side)
+        k, v = s.plan.read(s.cache, s.batch, stream=side)
+        torch.cuda.synchronize()
+        assert torch.equal(O, want) and torch.equal(k, K) and torch.equal(v, V)
+
+
 def test_cache_offsets_past_32_bits(cuda):
     """A pool of over 5 GB whose used pages lie at its end."""
     import torch
