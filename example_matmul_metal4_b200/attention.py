@@ -93,7 +93,8 @@ class AttentionPlan:
         d = self.dims
         self._check(Q=Q, K=K, V=V)
         if O is None:
-            O = torch.empty(self.shape(d.R, d.Hq), dtype=torch.float16, device=Q.device)
+            O = _lib.new_on_stream(stream, lambda: torch.empty(self.shape(d.R, d.Hq), dtype=torch.float16,
+                                                               device=Q.device))
         if lse is not None:
             if tuple(lse.shape) != self.lse_shape() or lse.dtype != torch.float32 or not lse.is_contiguous():
                 raise ValueError(f"lse must be a contiguous fp32 tensor of shape {self.lse_shape()}")
@@ -159,11 +160,11 @@ class AttentionPlan:
         self._check(Q=Q, K=K, V=V, O=O, dO=dO)
         if tuple(lse.shape) != self.lse_shape() or lse.dtype != torch.float32 or not lse.is_contiguous():
             raise ValueError(f"lse must be a contiguous fp32 tensor of shape {self.lse_shape()}")
-        dQ = torch.empty_like(Q) if dQ is None else dQ
-        dK = torch.empty_like(K) if dK is None else dK
-        dV = torch.empty_like(V) if dV is None else dV
+        dQ, dK, dV = (_lib.new_on_stream(stream, lambda: torch.empty_like(t)) if g is None else g
+                      for t, g in ((Q, dQ), (K, dK), (V, dV)))
         if workspace is None:
-            workspace = torch.empty(self.backward_workspace_bytes(), dtype=torch.uint8, device=Q.device)
+            workspace = _lib.new_on_stream(stream, lambda: torch.empty(
+                self.backward_workspace_bytes(), dtype=torch.uint8, device=Q.device), returned=False)
         _lib.check(self._L.mm4_attention_bwd(self._h, Q.data_ptr(), K.data_ptr(), V.data_ptr(), O.data_ptr(),
                                              dO.data_ptr(), lse.data_ptr(), dQ.data_ptr(), dK.data_ptr(),
                                              dV.data_ptr(), workspace.data_ptr(), workspace.numel(),

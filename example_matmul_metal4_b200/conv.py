@@ -178,7 +178,7 @@ class ConvPlan:
         if self.bias and (bias is None or bias.numel() != self.dims.outputChannels):
             raise ValueError("bias of Cout elements is required")
         if y is None:
-            y = torch.empty(self.out_shape, dtype=torch.float16, device=x.device)
+            y = _lib.new_on_stream(stream, lambda: torch.empty(self.out_shape, dtype=torch.float16, device=x.device))
         _lib.check(self._L.mm4_conv_run(self._h, x.data_ptr(), w.data_ptr(),
                                         bias.data_ptr() if self.bias else None, y.data_ptr(),
                                         _lib.stream_handle(stream), int(duplicatedCount)))
@@ -217,7 +217,7 @@ def permute_weights(src, from_layout: int, to_layout: int, dims5, stream=None, d
     import torch
     L = _lib.lib()
     if dst is None:
-        dst = torch.empty_like(src)
+        dst = _lib.new_on_stream(stream, lambda: torch.empty_like(src))
     elif dst.numel() != src.numel() or dst.dtype != src.dtype:
         raise ValueError("dst must match src in size and dtype")
     arr = (ctypes.c_int32 * 5)(*dims5)

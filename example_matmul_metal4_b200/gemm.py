@@ -95,7 +95,7 @@ class GemmPlan:
         if self.bias:
             _check_tensor(bias, (d.N,), "bias")
         if C is None:
-            C = torch.empty((d.M, d.N), dtype=torch.float16, device=A.device)
+            C = _lib.new_on_stream(stream, lambda: torch.empty((d.M, d.N), dtype=torch.float16, device=A.device))
         ws = workspace if workspace is not None else self.workspace(A.device)
         _lib.check(self._L.mm4_gemm_run(self._h, A.data_ptr(), B.data_ptr(), bias.data_ptr() if self.bias else None,
                                         C.data_ptr(), ws.data_ptr() if ws is not None else None,
@@ -134,7 +134,7 @@ class GemmPlan:
         _check_tensor(A, self.a_shape(), "A")
         _check_tensor(B, self.b_shape(), "B")
         if C32 is None:
-            C32 = torch.empty((d.M, d.N), dtype=torch.float32, device=A.device)
+            C32 = _lib.new_on_stream(stream, lambda: torch.empty((d.M, d.N), dtype=torch.float32, device=A.device))
         ws = workspace if workspace is not None else self.workspace(A.device)
         _lib.check(self._L.mm4_gemm_partial_run(self._h, A.data_ptr(), B.data_ptr(), C32.data_ptr(),
                                                 ws.data_ptr() if ws is not None else None,
@@ -147,7 +147,7 @@ def splitk_finalize(C32, bias, C=None, stream=None):
     import torch
     M, N = C32.shape
     if C is None:
-        C = torch.empty((M, N), dtype=torch.float16, device=C32.device)
+        C = _lib.new_on_stream(stream, lambda: torch.empty((M, N), dtype=torch.float16, device=C32.device))
     L = _lib.lib()
     _lib.check(L.mm4_splitk_finalize(M, N, C32.data_ptr(), bias.data_ptr() if bias is not None else None,
                                      C.data_ptr(), _lib.stream_handle(stream)))

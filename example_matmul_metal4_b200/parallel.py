@@ -229,7 +229,8 @@ class Comm:
         if plan.bias:
             _check_tensor(bias, (plan.dims.N,), "bias")
         if self.rank == 0 and C is None:
-            C = torch.empty((plan.dims.M, plan.dims.N), dtype=torch.float16, device=A.device)
+            C = self._lib.new_on_stream(stream, lambda: torch.empty((plan.dims.M, plan.dims.N), dtype=torch.float16,
+                                                                    device=A.device))
         self._lib.check(self._L.mm4_gemm_splitk_run_distributed(
             plan._h, self._h, A.data_ptr(), B.data_ptr(), bias.data_ptr() if plan.bias else None,
             C.data_ptr() if C is not None else None, self._lib.stream_handle(stream), int(duplicatedCount)))
