@@ -73,9 +73,11 @@ __device__ __forceinline__ KvSequence kv_sequence(const KvBatch& kb, int b) {
 }
 
 // The sequence whose rows hold row t: a search of the ascending offsets, then a
-// check, so offsets that are out of order find nothing rather than something
-// wrong. -1 for padding rows. Lanes with tokens of their own search binary; a
-// warp with one token searches 32-way, two steps for up to 1024 sequences.
+// check, so where offsets are out of order a row finds a sequence whose own
+// offsets hold it, or none. -1 for padding rows, and for sequences whose offsets
+// leave the rows: kv_sequence gives them no rows either. Lanes with tokens of their
+// own search binary; a warp with one token searches 32-way, two steps for up to
+// 1024 sequences.
 template <bool WARP>
 __device__ __forceinline__ int kv_find_sequence(const KvBatch& kb, int t, int lane) {
   int lo = 0, n = kb.sequences;
@@ -95,13 +97,13 @@ __device__ __forceinline__ int kv_find_sequence(const KvBatch& kb, int t, int la
     }
   }
   const int first = __ldg(kb.offsets + lo), end = __ldg(kb.offsets + lo + 1);
-  if (end < first) kv_note(KV_DATA_OFFSETS);
-  return first <= t && t < end ? lo : -1;
+  return first >= 0 && first <= t && t < end && end <= kb.tokens ? lo : -1;
 }
 
 // Where the K row of token t lies for head 0, as an offset into the cache; -1 if
-// the row has no place (padding, before position 0, beyond the page table, a
-// page outside the pool).
+// the row has no place (padding, a sequence with a wrong length, before position
+// 0, a page outside the pool). Wrong offsets and lengths are reported by
+// kv_check_batch.
 template <bool WARP>
 __device__ __forceinline__ long long kv_place(const KvBatch& kb, int t, int row_bytes, int lane) {
   const int b = kv_find_sequence<WARP>(kb, t, lane);
@@ -110,8 +112,7 @@ __device__ __forceinline__ long long kv_place(const KvBatch& kb, int t, int row_
   const int len = __ldg(kb.lengths + b);
   const long long pos = static_cast<long long>(len) - (end - t);
   const int room = kb.pages_per_seq << kb.page_shift;
-  if (len < 0 || len > room) kv_note(KV_DATA_LENGTH);
-  if (pos < 0 || pos >= room) return -1;
+  if (pos < 0 || len > room) return -1;  // pos < 0 for a negative length too
   const int p = static_cast<int>(pos);
   const int page = __ldg(kb.table + static_cast<long long>(b) * kb.pages_per_seq + (p >> kb.page_shift));
   if (page < 0 || page >= kb.pages) {
@@ -119,6 +120,14 @@ __device__ __forceinline__ long long kv_place(const KvBatch& kb, int t, int row_
     return -1;
   }
   return page * kb.page_bytes + static_cast<long long>(p & ((1 << kb.page_shift) - 1)) * row_bytes;
+}
+
+// Reports what is wrong in the lengths and offsets of a batch, whether a row's
+// search meets it or not: threads `first`, `first + step`, ... of a call take a
+// sequence each. Offsets are in order if every sequence's are, and the last ends
+// in the rows.
+__device__ __forceinline__ void kv_check_batch(const KvBatch& kb, int first, int step) {
+  for (long long b = first; b < kb.sequences; b += step) kv_sequence(kb, static_cast<int>(b));
 }
 
 // ---------------------------------------------------------------------------
@@ -174,6 +183,7 @@ struct KvIoArgs {
   __half* out_v;
   long long k_stride, v_stride;
   uint8_t* cache;
+  int blocks;           // that move rows; those behind them check the batch
   int parts;            // warps that share a token
   int tokens_per_warp;  // 1 .. 32: looked up by a lane each, so that their places cost one latency
 };
@@ -186,6 +196,11 @@ struct KvIoWork {
 };
 template <int ROW_BYTES>
 __device__ __forceinline__ bool kv_io_work(const KvIoArgs& a, int lane, KvIoWork* w) {
+  if (blockIdx.x >= a.blocks) {
+    kv_check_batch(a.kb, static_cast<int>((blockIdx.x - a.blocks) * blockDim.x + threadIdx.x),
+                   static_cast<int>((gridDim.x - a.blocks) * blockDim.x));
+    return false;
+  }
   const long long id = static_cast<long long>(blockIdx.x) * KV_IO_WARPS + (threadIdx.x >> 5);
   const long long t0 = id / a.parts * a.tokens_per_warp;
   if (t0 >= a.kb.tokens) return false;

@@ -107,12 +107,16 @@ mm4_status launch_io(const mm4_kv_cache_plan* p, KvIoArgs& a, bool write, cudaSt
   a.tokens_per_warp = static_cast<int>(std::max(1ll, std::min(8ll, warps / (64ll * info.sm_count))));
   const long long groups = (a.kb.tokens + a.tokens_per_warp - 1) / a.tokens_per_warp;
   const long long blocks = (groups * a.parts + KV_IO_WARPS - 1) / KV_IO_WARPS;
-  if (blocks > 0x7fffffffLL) return fail(MM4_ERR_UNSUPPORTED, "too many tokens for one launch");
+  // Blocks of their own check the batch, beside the others and at no cost to them.
+  const int checks = std::min(info.sm_count, (a.kb.sequences - 1) / (KV_IO_WARPS * 32) + 1);
+  if (blocks + checks > 0x7fffffffLL) return fail(MM4_ERR_UNSUPPORTED, "too many tokens for one launch");
+  a.blocks = static_cast<int>(blocks);
+  const unsigned grid = static_cast<unsigned>(blocks + checks);
   return by_row(p->d, [&](auto, auto D, auto B) -> mm4_status {
     if (write)
-      kv_append_kernel<D.value, B.value><<<static_cast<unsigned>(blocks), KV_IO_WARPS * 32, 0, st>>>(a);
+      kv_append_kernel<D.value, B.value><<<grid, KV_IO_WARPS * 32, 0, st>>>(a);
     else
-      kv_read_kernel<D.value, B.value><<<static_cast<unsigned>(blocks), KV_IO_WARPS * 32, 0, st>>>(a);
+      kv_read_kernel<D.value, B.value><<<grid, KV_IO_WARPS * 32, 0, st>>>(a);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return cuda_fail(e, write ? "kv_append_kernel launch" : "kv_read_kernel launch");
     return MM4_OK;

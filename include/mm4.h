@@ -374,8 +374,8 @@ typedef struct mm4_kv_cache_plan mm4_kv_cache_plan;
  *  offsets    [sequences + 1], ascending: rows offsets[b] .. offsets[b+1]-1 of
  *             K, V, Q and O are the LAST tokens of sequence b, so the last of
  *             them has position lengths[b] - 1. Rows outside every sequence
- *             (below offsets[0], from offsets[sequences] on) are padding: not
- *             read, and left as they were in outputs.
+ *             (below offsets[0], from offsets[sequences] on) are padding: what
+ *             they hold is not used, and they are left as they were in outputs.
  *  tokens     rows of K, V, Q and O.
  *  max_new    most rows of one sequence (mm4_kv_cache_attention only).
  * A sequence may have no rows in a call, length 0, or more rows than its length:
@@ -383,9 +383,12 @@ typedef struct mm4_kv_cache_plan mm4_kv_cache_plan;
  * and with causal = 1 attend to nothing. Page-table entries behind a sequence's
  * length are not read. What the kernels find wrong in these arrays - a page
  * number outside the pool, a length beyond the page table, more rows than max_new,
- * offsets out of order or beyond tokens - never leads to an access out of bounds:
- * such tokens are left out by append and read, the outputs of such sequences are
- * unspecified in attention, and mm4_check() reports MM4_ERR_INVALID. */
+ * offsets out of order or beyond tokens - never leads to an access out of bounds,
+ * and mm4_check() reports MM4_ERR_INVALID. Append and read leave out the rows of
+ * sequences whose own offsets or length are wrong, and rows whose page is (a row
+ * that the offsets of several sequences hold, as only offsets out of order can, goes
+ * to one of them); max_new does not concern them. The outputs of such sequences are
+ * unspecified in attention. */
 typedef struct mm4_kv_cache_batch {
   int32_t sequences;
   int32_t tokens;

@@ -642,6 +642,66 @@ def test_a_page_outside_the_pool_is_reported_and_touches_no_other_sequence(cuda,
     sync_check()
 
 
+@pytest.mark.parametrize("n", [1, 40, 7000])
+@pytest.mark.parametrize("what", ["end beyond the rows", "start before the rows", "out of order", "negative length",
+                                  "length beyond the table"])
+def test_append_and_read_leave_out_wrong_sequences_and_report_them(cuda, what, n):
+    """Three sequences of n rows each, one of them wrong: the others are written and read exactly, and no other byte
+    changes. 21,000 rows take the form in which a warp has several tokens."""
+    import torch
+    Hk, D, page, bits = 2, 64, 64, 4
+    lengths, offsets, wrong = [2 * n + 9, 2 * n + 30, 2 * n + 3], [0, n, 2 * n, 3 * n], []
+    room = (max(lengths) + page - 1) // page
+    table = np.random.default_rng(n).permutation(3 * room + 1)[:3 * room].reshape(3, room).astype(np.int32)
+    told = list(lengths)
+    if what == "end beyond the rows":
+        offsets[3], wrong = 3 * n + 1, [2]
+    elif what == "start before the rows":
+        offsets[0], wrong = -1, [0]
+    elif what == "out of order":
+        offsets[1], offsets[2], wrong = 2 * n, n, [1]   # rows n .. 2 n - 1 are in sequences 0 and 2
+    elif what == "negative length":
+        told[1], wrong = -5, [1]
+    else:
+        told[1], wrong = room * page + 1, [1]
+    plan = KVCachePlan(KVCacheDimensions(3 * room + 1, page, Hk, Hk, D, bits))
+    K, V = data.normal((3 * n, Hk, D), 1.0, n, 0), data.normal((3 * n, Hk, D), 1.0, n, 1)
+    packed = [ref.pack(x, bits) for x in (K, V)]
+    values = [ref.unpack(x, D, bits) for x in packed]
+    host = np.full((3 * room + 1, Hk, 2, page, ref.row_bytes(D, bits)), 0xA5, dtype=np.uint8)
+    cache = torch.from_numpy(host.reshape(len(host), -1).copy()).to(cuda)
+    batch = KVCacheBatch(torch.from_numpy(table).to(cuda), torch.tensor(told, dtype=torch.int32, device=cuda),
+                         torch.tensor(offsets, dtype=torch.int32, device=cuda), 3 * n, n)
+    plan.append(torch.from_numpy(K).to(cuda), torch.from_numpy(V).to(cuda), cache, batch)
+    text = "length" if "length" in what else "offsets"
+    _reported(text)
+    free = np.zeros(host.shape[:1] + host.shape[3:4], dtype=bool)    # places of rows that two sequences hold
+    read = np.zeros(3 * n, dtype=bool)
+    either = np.zeros(3 * n, dtype=bool)
+    if what == "out of order":
+        either[n:2 * n] = True
+    for b in range(3):
+        if b in wrong:
+            continue
+        t = np.arange(max(0, offsets[b]), offsets[b + 1])
+        pos = lengths[b] - (offsets[b + 1] - t)
+        to, row = table[b, pos // page], pos % page
+        for kv in (0, 1):
+            host[to, :, kv, row] = packed[kv][t]
+        free[to[either[t]], row[either[t]]] = True
+        read[t] = True
+    got = cache.cpu().numpy().reshape(host.shape)
+    same = (got == host).all(axis=(1, 2, 4))
+    assert same[~free].all() and (same | (got == 0xA5).all(axis=(1, 2, 4))).all()
+    oK, oV = (torch.full((3 * n, Hk, D), -3.0, dtype=torch.float16, device=cuda) for _ in range(2))
+    plan.read(torch.from_numpy(host.reshape(len(host), -1)).to(cuda), batch, K=oK, V=oV)
+    _reported(text)
+    for out, want in ((oK, values[0]), (oV, values[1])):
+        out = out.cpu().numpy()
+        assert np.array_equal(out[read & ~either], want[read & ~either])
+        assert (out[~read] == -3.0).all()
+
+
 @pytest.mark.parametrize("new", [1, 100])
 def test_wrong_lengths_offsets_and_row_counts_are_reported(cuda, new):
     import torch
