@@ -272,6 +272,55 @@ def test_scores_far_below_zero(cuda, new):
     s.check(*s.attend())
 
 
+def _exact_scores(s, S, sequence=0):
+    """(O, lse, tol_O, tol_lse) in float64 of the rows of one sequence whose scores before scaling, S [n][Hq][len], are
+    exact in fp32. Beside what kv_cache_ref.attention derives, with ds = 0: the exponent y = (s - max) scale log2 e has
+    two roundings of its own and two of the factor, 2^-22 |y| in all, which shift p by as much (ln 2 < 1)."""
+    n, Hq, ln = S.shape
+    V = s.V[sequence].astype(np.float64).repeat(Hq // s.Hk, 1)                       # [len][Hq][D]
+    scale = float(np.float32(s.plan.scale))
+    if s.causal:
+        S = np.where(np.arange(ln)[None, None] > (ln - n + np.arange(n))[:, None, None], -np.inf, S)
+    m = S.max(-1, keepdims=True)
+    y = (S - m) * scale / np.log(2)
+    p = np.exp2(y)
+    total = p.sum(-1)
+    off = np.where(p > 0, p * np.abs(np.maximum(y, -2000)) * 2.0 ** -22, 0)
+    mean = lambda w, v: np.einsum("nhl,lhd->nhd", w, v) / total[..., None]            # noqa: E731
+    O, a = mean(p, V), mean(p, np.abs(V))
+    rest = 2.0 ** -11 + 2.0 ** -19 + (ln / 16 + 64) * 2.0 ** -23
+    tol = a * rest + mean(off, np.abs(V)) + np.abs(O) * (off.sum(-1) / total)[..., None] \
+        + np.abs(V).sum(0) * 2.0 ** -25 / total[..., None] + 2.0 ** -11 * np.abs(O) + 2.0 ** -25
+    lse = m[..., 0] * scale + np.log(total)
+    tol_lse = off.sum(-1) / total + 2.0 ** -20 + (ln / 16 + 64) * 2.0 ** -23 + 2.0 ** -22 * np.abs(lse) \
+        + 2.0 ** -22 * np.abs(m[..., 0]) * scale
+    return O, lse, tol, tol_lse
+
+
+def _check_exact(s, S):
+    O, lse = s.attend()
+    eO, eL, tO, tL = _exact_scores(s, S)
+    dO, dL = np.abs(O.double().cpu().numpy() - eO), np.abs(lse.double().cpu().numpy() - eL)
+    assert (dO <= tO).all(), (np.nanmax(dO / tO), np.isnan(dO).sum())
+    assert (dL <= tL).all(), (np.nanmax(dL / tL), np.isnan(dL).sum())
+
+
+@pytest.mark.parametrize("D,bits", [(64, 8), (64, 4), (128, 4)])
+@pytest.mark.parametrize("new,name", [(1, "few<8"), (10, "few<24"), (70, "many")])
+@pytest.mark.parametrize("key", [64 * 3 + i for i in range(8)] + [0, 38, 63, 230])
+def test_rows_that_one_key_dominates(cuda, key, new, name, D, bits):
+    """One key has nearly all of a row's weight, at every position of a group of 8: lse is that key's score, and O its
+    value, to fp32 and fp16 precision wherever the key lies."""
+    c = np.zeros(300, np.float32)
+    c[key] = 16
+    s = Setup(cuda, [300], [new], 4, 2, D=D, bits=bits, scale=0.125, causal=False,
+              k_map=lambda k: np.ones_like(k) * c[:, None, None])
+    assert name in s.plan.attention_kernel_name(s.batch)
+    s.Q = np.zeros((new, 4, D), np.float16)
+    s.Q[:, :, D - 1] = np.resize(np.float16([10, 12, 16]), (new, 4))
+    _check_exact(s, s.Q[:, :, D - 1].astype(np.float64)[..., None] * c)
+
+
 @pytest.mark.parametrize("new", [1, 100])
 def test_strided_queries_and_outputs(cuda, new):
     import torch
