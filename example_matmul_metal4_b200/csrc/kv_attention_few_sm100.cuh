@@ -20,9 +20,9 @@
 //    permute per two words.
 //  - P is rounded to fp16 for its product (2^-11 of itself, like the result);
 //    sums, maxima and O stay fp32.
-//  - The running maximum is raised only when a score exceeds it by 2^8 (log2
-//    domain), which one vote per tile decides; the stale maximum cancels in
-//    O / l.
+//  - The running maximum is raised only when a score exceeds it by 8 in the log2
+//    domain (P up to 2^8), which one vote per tile decides; the stale maximum
+//    cancels in O / l.
 //
 // 64 sequences of up to 8192 tokens, heads 32 / 8 of 128, 4 bits, on one B200: 97 us,
 // 4.5 TB/s (floor 68 us; copying the tiles without computing takes 73 us).
@@ -354,13 +354,13 @@ __global__ void __launch_bounds__(KvFew<D, BITS, NT, TEAM>::THREADS, 1) kv_atten
   Place at = place_of(warp);
   uint32_t q[NT][D / 16][2];
   float acc[NT][MT][4];
-  float m[NT][2], l[NT][2];  // running maximum (log2 domain) and sum of rows 2 c, 2 c + 1
+  float m[NT][2], l[NT][2];  // running maximum (a score) and sum of rows 2 c, 2 c + 1
   float raise[NT][2];        // the score above which the maximum is raised
   int limit[NT][2];
   int clear = 0;             // keys before this one are masked in no row
   int st = 0, phase = 0;     // the ring's next tile and its parity
   bool ok = true;
-  const float sl2 = a.scale_log2, inv_sl2 = 1.0f / sl2;
+  const float sl2 = a.scale_log2, margin = 8.0f / sl2;
   const uint32_t k1024 = __shfl_sync(0xffffffffu, a.k1024, 0);
 
   // Rows of the unit at p: at most ROWS, and none behind max_new tokens.
@@ -484,10 +484,10 @@ __global__ void __launch_bounds__(KvFew<D, BITS, NT, TEAM>::THREADS, 1) kv_atten
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-          const float m_new = fmaxf(m[nt][e], x * sl2);
-          const float f = kv_ex2(m[nt][e] - m_new);
+          const float m_new = fmaxf(m[nt][e], x);
+          const float f = kv_ex2((m[nt][e] - m_new) * sl2);
           m[nt][e] = m_new;
-          raise[nt][e] = (m_new + 8.0f) * inv_sl2;
+          raise[nt][e] = __fadd_rd(m_new, margin);  // down, so that no P passes 2^8 where scores lie far apart
           l[nt][e] *= f;
 #pragma unroll
           for (int t = 0; t < MT; ++t) {
@@ -505,7 +505,7 @@ __global__ void __launch_bounds__(KvFew<D, BITS, NT, TEAM>::THREADS, 1) kv_atten
         float p4[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          p4[e] = kv_ex2(fmaf(s[hf][nt][e], sl2, -m[nt][e & 1]));
+          p4[e] = kv_ex2((s[hf][nt][e] - m[nt][e & 1]) * sl2);
           l[nt][e & 1] += p4[e];
         }
         pt[hf][nt][0] = kv_transpose(pack_half2(p4[0], p4[1]));
@@ -624,7 +624,7 @@ __global__ void __launch_bounds__(KvFew<D, BITS, NT, TEAM>::THREADS, 1) kv_atten
                                       pack_half2(acc[nt][t + 1][e] * inv, acc[nt][t + 1][e + 2] * inv),
                                       pack_half2(acc[nt][t + 2][e] * inv, acc[nt][t + 2][e + 2] * inv),
                                       pack_half2(acc[nt][t + 3][e] * inv, acc[nt][t + 3][e + 2] * inv));
-            if (lse != nullptr && g == 0) *lse = (m[nt][e] + log2f(l[nt][e])) * 0.6931471805599453f;
+            if (lse != nullptr && g == 0) *lse = kv_lse(m[nt][e], l[nt][e], sl2);
           }
       } else {
         store_partial(slots + (n0 == 0 ? KvPartial<D, Cfg::ROWS>::FLOATS : 0), rows);
@@ -654,7 +654,7 @@ __global__ void __launch_bounds__(KvFew<D, BITS, NT, TEAM>::THREADS, 1) kv_atten
               const int row = nt * 8 + 2 * c + e;
               if (row >= rows) continue;
               const float m2 = other[Cfg::ROWS * D + 2 * row], l2 = other[Cfg::ROWS * D + 2 * row + 1];
-              const float mm = fmaxf(m[nt][e], m2), f1 = kv_ex2(m[nt][e] - mm), f2 = kv_ex2(m2 - mm);
+              const float mm = fmaxf(m[nt][e], m2), f1 = kv_ex2((m[nt][e] - mm) * sl2), f2 = kv_ex2((m2 - mm) * sl2);
               m[nt][e] = mm;
               l[nt][e] = l[nt][e] * f1 + l2 * f2;
 #pragma unroll
@@ -675,7 +675,7 @@ __global__ void __launch_bounds__(KvFew<D, BITS, NT, TEAM>::THREADS, 1) kv_atten
           float ls = 0.f, x = 0.f, y = 0.f;
 #pragma unroll
           for (int k = 0; k < Cfg::PARTS; ++k) {
-            const float f = kv_ex2(join[k * F + Cfg::ROWS * D + 2 * row] - mm);
+            const float f = kv_ex2((join[k * F + Cfg::ROWS * D + 2 * row] - mm) * sl2);
             ls += f * join[k * F + Cfg::ROWS * D + 2 * row + 1];
             x += f * join[k * F + row * D + d];
             y += f * join[k * F + row * D + d + 1];
@@ -685,7 +685,7 @@ __global__ void __launch_bounds__(KvFew<D, BITS, NT, TEAM>::THREADS, 1) kv_atten
           output_row(at, row, &o, &lse);
           const float inv = ls > 0.f ? 1.0f / ls : 0.f;
           *reinterpret_cast<__half2*>(o + d) = __floats2half2_rn(x * inv, y * inv);
-          if (lse != nullptr && d == 0) *lse = (mm + log2f(ls)) * 0.6931471805599453f;
+          if (lse != nullptr && d == 0) *lse = kv_lse(mm, ls, sl2);
         }
         named_barrier(1, W * 32);  // the parts are free for the next unit
       }
@@ -752,6 +752,7 @@ __global__ void __launch_bounds__(256) kv_attention_join_kernel(const KvAttnArgs
   const int count = static_cast<int>(last - first + 1);
   const int c0 = static_cast<int>(static_cast<long long>(mine) * count / parts),
             c1 = static_cast<int>(static_cast<long long>(mine + 1) * count / parts);
+  const float sl2 = a.scale_log2;
   float mm = KV_NO_MAX, ls = 0.f, acc[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) acc[i] = 0.f;
@@ -787,7 +788,7 @@ __global__ void __launch_bounds__(256) kv_attention_join_kernel(const KvAttnArgs
       float top = pm;
 #pragma unroll
       for (int k = 16; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
-      const float m_new = fmaxf(mm, top), f = kv_ex2(mm - m_new), w = kv_ex2(pm - m_new);
+      const float m_new = fmaxf(mm, top), f = kv_ex2((mm - m_new) * sl2), w = kv_ex2((pm - m_new) * sl2);
       mm = m_new;
       ls *= f;
 #pragma unroll
@@ -823,7 +824,7 @@ __global__ void __launch_bounds__(256) kv_attention_join_kernel(const KvAttnArgs
     if (mine == 0 && row < rows) {
       for (int k = 1; k < parts; ++k) {
         const float* o = part[k * per + row];
-        const float m2 = o[D], m_new = fmaxf(mm, m2), f1 = kv_ex2(mm - m_new), f2 = kv_ex2(m2 - m_new);
+        const float m2 = o[D], m_new = fmaxf(mm, m2), f1 = kv_ex2((mm - m_new) * sl2), f2 = kv_ex2((m2 - m_new) * sl2);
         mm = m_new;
         ls = ls * f1 + o[D + 1] * f2;
 #pragma unroll
@@ -842,7 +843,7 @@ __global__ void __launch_bounds__(256) kv_attention_join_kernel(const KvAttnArgs
                                                 pack_half2(acc[2] * inv, acc[3] * inv));
     else
       *reinterpret_cast<uint32_t*>(o) = pack_half2(acc[0] * inv, acc[1] * inv);
-    if (a.lse != nullptr && lane == 0) a.lse[tok * a.heads_q + head] = (mm + log2f(ls)) * 0.6931471805599453f;
+    if (a.lse != nullptr && lane == 0) a.lse[tok * a.heads_q + head] = kv_lse(mm, ls, sl2);
   }
 }
 

@@ -18,11 +18,12 @@
 //   warp 2        one lane issues O_i += P_i(g) V(g) (P from TMEM).
 //   warp 3        finds the CTA's range (and warp 2, before its products, the unit
 //                 that the range leaves to others).
-//   warps 4-11    softmax, one row a thread: P = 2^(S scale log2 e - m) with fp32 m
-//                 and sums, P rounded to fp16 for the product (2^-11 of itself,
-//                 like the result); O is rescaled only when the maximum grew by
-//                 more than 2^8. Results out; a warp also copies its rows of the
-//                 next unit's Q, as soon as it has the last scores of the unit.
+//   warps 4-11    softmax, one row a thread: P = 2^((S - max) scale log2 e) with fp32
+//                 maxima and sums, P rounded to fp16 for the product (2^-11 of
+//                 itself, like the result); O is rescaled only when the maximum
+//                 grew by more than 8 in the log2 domain. Results out; a warp also
+//                 copies its rows of the next unit's Q, as soon as it has the last
+//                 scores of the unit.
 //   warps 12-15   codes to fp16: a lane takes 32 elements (one scale and zero).
 // TMEM: two 64-column S slots for each row tile, then O_i (D columns each). Steps
 // of 64 keys are counted across a CTA's units (g), which fixes slots and
@@ -60,7 +61,8 @@ struct KvMany {
   static constexpr int OUT_ROW = 64 + 16;              // a row of 32 results, on banks of its own
   static constexpr int OUT_BYTES = 32 * OUT_ROW;       // a softmax warp's results on their way out
   static constexpr int OUT_OFFSET = QT * Q_BYTES + (KS + VS) * TILE_BYTES + RS * RAW_BYTES;
-  static constexpr int BAR_OFFSET = OUT_OFFSET + 4 * QT * OUT_BYTES;
+  static constexpr int MAX_OFFSET = OUT_OFFSET + 4 * QT * OUT_BYTES;  // each row's largest score
+  static constexpr int BAR_OFFSET = MAX_OFFSET + ROWS * 4;
   static constexpr int SMEM_BYTES = BAR_OFFSET + 512 + 1024;
   // Registers: 128 threads each of warps 0-3, the softmax warps and the
   // unpacking warps; the sum must not exceed what the block is launched with.
@@ -299,6 +301,39 @@ __device__ __forceinline__ float kvm_exp_store64(const float (&x)[64], float sl2
   return sum.x + sum.y;
 }
 
+// P = 2^((s - top) sl2) of a row's 64 scores, read again from the TMEM columns at tP,
+// of which the first `valid` count. kvm_exp_store64 subtracts m = fl(top sl2) in place
+// of the product, so its P are off by the rounding: a factor that a row's P share, but
+// one that passes fp16's range for scores that fp16 inputs reach (2^474). From |m| =
+// 2^20 on, where it passes 2^(1/16), m is a NaN, which takes the row's warp to this
+// function. Subtracting top from every score instead costs 5 % (prompts, head_dim 128);
+// this way, with no instruction and no register on the common path, nothing.
+__device__ __forceinline__ float kvm_exp_store64_far(float sl2, float top, int valid, uint32_t tP) {
+  float sum = 0.f;
+#pragma unroll 1
+  for (int half = 0; half < 2; ++half) {
+    uint32_t v[32], pk[16];
+    __syncwarp();
+    tmem_ld_32x32b_x32(tP + half * 32, v);
+    tmem_ld_wait();
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+      const int key = half * 32 + i;
+      const float p0 = key < valid ? ex2_approx((__uint_as_float(v[i]) - top) * sl2) : 0.f;
+      const float p1 = key + 1 < valid ? ex2_approx((__uint_as_float(v[i + 1]) - top) * sl2) : 0.f;
+      sum += p0 + p1;
+      pk[i / 2] = pack_half2(p0, p1);
+    }
+    tmem_st_32x32b_x16(tP + half * 16, pk);
+  }
+  return sum;
+}
+
+// log2 of the factor by which kvm_exp_store64's P are too small.
+__device__ __forceinline__ float kvm_rest(float top, float sl2, bool far) {
+  return far || top == KV_NO_MAX ? 0.f : fmaf(-top, sl2, top * sl2);
+}
+
 template <int D, int BITS>
 __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const __grid_constant__ KvAttnArgs a) {
   using Cfg = KvMany<D, BITS>;
@@ -522,6 +557,9 @@ __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const
     const uint32_t tS = tmem_base + ti * 128 + lane_off;
     const uint32_t tO = tmem_base + 256 + ti * D + lane_off;
     const float sl2 = a.scale_log2;
+    // This row's running maximum, a score (possibly stale by 8 in the log2 domain).
+    // Needed where it is raised, for large ones and for partials, so it takes no register.
+    auto top = [&] { return reinterpret_cast<volatile float*>(smem + Cfg::MAX_OFFSET) + (threadIdx.x - 128); };
     bool ok = true;
     int g = 0;
     // This thread's row of a segment, and its copy of it into Q_i.
@@ -575,8 +613,9 @@ __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const
       } const cur{sg.n0, sg.n1, sg.steps};
       RowOf next{};
       const int limit = me.limit;
-      float m = KV_NO_MAX;  // running max, log2 domain (possibly stale by < 8)
+      float m = KV_NO_MAX;  // its product with sl2, NaN from 2^20 on
       float l = 0.f;
+      *top() = KV_NO_MAX;
       for (int n = cur.n0; n < cur.n1; ++n, ++g) {
         const int sl = g & 1;
         const uint32_t tSl = tS + sl * KVM_TK;
@@ -605,14 +644,21 @@ __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const
             if ((hi & (1u << i)) == 0) x[32 + i] = -INFINITY;
           }
         }
-        const float mx = att_row_max64(x) * sl2;
-        const bool grow = mx > m + 8.0f;
-        if (__any_sync(0xffffffffu, grow)) {
-          const float m_new = grow ? mx : m;
-          const float factor = grow ? ex2_approx(m - m_new) : 1.0f;
+        const float raw = att_row_max64(x);
+        const float mx = raw * sl2;
+        if (__any_sync(0xffffffffu, !(mx <= m + 8.0f))) {
+          const bool was = __any_sync(0xffffffffu, isnan(m));
+          const float old = *top();
+          float y = kvm_rest(old, sl2, was);
+          if (was ? raw > old : mx > m + 8.0f) {
+            m = fabsf(mx) < 0x1p20f ? mx : NAN;
+            *top() = raw;
+            y += (old - raw) * sl2;
+          }
+          const bool far = __any_sync(0xffffffffu, isnan(m));
+          const float factor = ex2_approx(y - kvm_rest(*top(), sl2, far));
           l *= factor;
-          m = m_new;
-          if (n > cur.n0) {
+          if (n > cur.n0 && __any_sync(0xffffffffu, factor != 1.0f)) {
             // Rescale this warp's O rows once the previous step's P V (the only
             // MMA that may still write them) is done.
             ok = __all_sync(0xffffffffu,
@@ -629,6 +675,19 @@ __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const
               tmem_st_32x32b_x16(tO + c * 16, v);
             }
             tmem_st_wait();
+          }
+          if (far) {
+            // The turns are taken as below.
+            if (ti == 1 || g > 0)
+              ok = mbar_wait(&turn[(1 - ti) * 4 + q], (ti == 1 ? g : g - 1) & 1, wd, SITE_KVM_SOFTMAX);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            l += kvm_exp_store64_far(sl2, *top(), valid, tSl);
+            if (lane == 0) mbar_arrive(&turn[ti * 4 + q]);
+            tmem_st_wait();
+            tc_fence_before();
+            mbar_arrive(&p_full[2 * ti + sl]);
+            continue;
           }
         }
         // The two row tiles' warps of an SM quarter take turns at the
@@ -699,11 +758,15 @@ __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const
                   *reinterpret_cast<const uint4*>(stage + rr * Cfg::OUT_ROW + (lane & 3) * 16);
           }
         }
-        if (me.have && a.lse != nullptr)
-          a.lse[static_cast<long long>(me.tok) * a.heads_q + me.head] = (m + log2f(l)) * 0.6931471805599453f;
+        if (a.lse != nullptr) {
+          const float fix = ex2_approx(kvm_rest(*top(), sl2, __any_sync(0xffffffffu, isnan(m))));
+          if (me.have) a.lse[static_cast<long long>(me.tok) * a.heads_q + me.head] = kv_lse(*top(), l * fix, sl2);
+        }
       } else {
         float* part = a.partials + kvm_slot<D, ROWS>(2ll * blockIdx.x + (cur.n0 == 0 ? 1 : 0));
         float4* dst = reinterpret_cast<float4*>(part) + ti * 128 + r;
+        // Partials of a row then differ by their maxima alone.
+        const float fix = ex2_approx(kvm_rest(*top(), sl2, __any_sync(0xffffffffu, isnan(m))));
 #pragma unroll 1
         for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];
@@ -714,8 +777,10 @@ __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const
 #pragma unroll
             for (int i = 0; i < 32; i += 4)
               dst[(c * 8 + i / 4) * ROWS] = make_float4(
-                  __uint_as_float(o[(i & ~7) + column(i & 7)]), __uint_as_float(o[(i & ~7) + column((i & 7) + 1)]),
-                  __uint_as_float(o[(i & ~7) + column((i & 7) + 2)]), __uint_as_float(o[(i & ~7) + column((i & 7) + 3)]));
+                  __uint_as_float(o[(i & ~7) + column(i & 7)]) * fix,
+                  __uint_as_float(o[(i & ~7) + column((i & 7) + 1)]) * fix,
+                  __uint_as_float(o[(i & ~7) + column((i & 7) + 2)]) * fix,
+                  __uint_as_float(o[(i & ~7) + column((i & 7) + 3)]) * fix);
           }
         }
         __syncwarp();
@@ -723,8 +788,8 @@ __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const
         mbar_arrive(&o_empty[ti]);
         if (more) q_in_place();
         if (me.have) {
-          part[ROWS * D + ti * 128 + r] = m;
-          part[ROWS * D + ROWS + ti * 128 + r] = l;
+          part[ROWS * D + ti * 128 + r] = *top();
+          part[ROWS * D + ROWS + ti * 128 + r] = l * fix;
         }
       }
       me = next;
@@ -863,7 +928,7 @@ __global__ void __launch_bounds__(256) kv_attention_many_join_kernel(const __gri
   for (int k = w; k <= last; ++k) {
     const float* part = a.partials + kvm_slot<D, ROWS>(2ll * k + (k == w ? 1 : 0));
     const float pm = __ldcg(part + ROWS * D + local), pl = __ldcg(part + ROWS * D + ROWS + local);
-    const float m_new = fmaxf(m, pm), f = kv_ex2(m - m_new), fp = kv_ex2(pm - m_new);
+    const float m_new = fmaxf(m, pm), f = kv_ex2((m - m_new) * a.scale_log2), fp = kv_ex2((pm - m_new) * a.scale_log2);
     m = m_new;
     l = l * f + pl * fp;
 #pragma unroll
@@ -883,7 +948,7 @@ __global__ void __launch_bounds__(256) kv_attention_many_join_kernel(const __gri
   for (int i = 0; i < G4; ++i)
     *reinterpret_cast<uint2*>(out + 4 * i) = make_uint2(pack_half2(acc[i][0] * inv, acc[i][1] * inv),
                                                         pack_half2(acc[i][2] * inv, acc[i][3] * inv));
-  if (a.lse != nullptr && warp == 0) a.lse[token * a.heads_q + head] = (m + log2f(l)) * 0.6931471805599453f;
+  if (a.lse != nullptr && warp == 0) a.lse[token * a.heads_q + head] = kv_lse(m, l, a.scale_log2);
 }
 
 }  // namespace mm4

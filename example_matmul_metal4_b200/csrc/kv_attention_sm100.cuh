@@ -46,13 +46,17 @@ __device__ __forceinline__ long long kv_worker_of(long long x, long long T, long
 
 // Partials of worker w: slot 2 w is a segment that began in another worker's
 // range, slot 2 w + 1 one that begins a unit here and goes on elsewhere.
-// Each holds ROWS x D floats, then (m, l) of ROWS rows; m in the log2 domain.
+// Each holds ROWS x D floats, then (m, l) of ROWS rows; m is a score.
 template <int D, int ROWS>
 struct KvPartial {
   static constexpr int FLOATS = ROWS * (D + 2);
 };
 
-constexpr float KV_NO_MAX = -1e30f;  // running maximum of a row that has seen no key
+// Exponentials are 2^((s - m) scale log2 e) with m, the running maximum, a score
+// like s: the maximum gives exactly 1 however large it is. (2^(s scale log2 e - m)
+// with m in the log2 domain would be off by m's rounding, which passes 2^16 for
+// scores that fp16 inputs reach.)
+constexpr float KV_NO_MAX = -1e30f;  // of a row that has seen no key: below all scores (2^39) of fp16 rows
 
 // Tiles of TK keys of a sequence (at least one: a row block with no key still
 // takes a tile, which writes its zeros), and its row blocks of ROWS rows (none if
@@ -115,6 +119,11 @@ __device__ __forceinline__ float kv_ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Natural-log sum of exp(scale * S) from the maximum and the sum.
+__device__ __forceinline__ float kv_lse(float m, float l, float scale_log2) {
+  return fmaf(m, scale_log2, log2f(l)) * 0.6931471805599453f;
 }
 
 // Lets the next kernel of the stream start its blocks, and waits in it until

@@ -321,6 +321,38 @@ def test_rows_that_one_key_dominates(cuda, key, new, name, D, bits):
     _check_exact(s, s.Q[:, :, D - 1].astype(np.float64)[..., None] * c)
 
 
+@pytest.mark.parametrize("D,bits", [(128, 4), (64, 8), (64, 4), (128, 8)])
+@pytest.mark.parametrize("new,length", [(1, 200), (1, 3000), (6, 150), (6, 2500), (12, 300), (70, 500), (200, 9000)])
+@pytest.mark.parametrize("scale", [None, 4.0, 1e-3])
+def test_scores_at_the_ends_of_fp16(cuda, scale, new, length, D, bits):
+    """Q and K up to 65504 of either sign: scores of 2^32 and beyond, whose maximum still has to count exactly 1. K is
+    constant in each row, so cached exactly, and Q has one element, so every score is one exact product."""
+    rng = np.random.default_rng(new)
+    c = rng.choice(np.float32([65504, 65472, 65504, 40000, 60000, 1.5, -3, -65504]), length)
+    s = Setup(cuda, [length], [new], 4, 2, D=D, bits=bits, scale=scale, k_map=lambda k: np.ones_like(k) * c[:, None, None])
+    q = np.resize(np.float16([65504, -65504, 1024, 1, -4096, 2.0 ** -10, 0, 65472, -65504]), (new, 4))
+    s.Q = np.zeros((new, 4, D), np.float16)
+    s.Q[:, :, 5] = q
+    _check_exact(s, q.astype(np.float64)[..., None] * c.astype(np.float64))
+
+
+@pytest.mark.parametrize("D,bits", [(128, 4), (64, 8)])
+@pytest.mark.parametrize("e", [24, 27, 30])
+@pytest.mark.parametrize("new,length", [(1, 900), (1, 5000), (12, 700), (70, 1500)])
+def test_maximum_rises_by_single_steps_of_fp32(cuda, new, length, e, D, bits):
+    """Scores 2^e plus 0, 1, 2, ... units in the last place, 5.3 in the log2 domain each: the margin by which the
+    running maximum may be stale is close to what fp32 resolves, and P must not leave fp16."""
+    unit = 2.0 ** (e - 23)
+    for order in (np.arange(length), np.random.default_rng(e).permutation(length)):
+        j = order % 2000
+        s = Setup(cuda, [length], [new], 2, 2, D=D, bits=bits, scale=5.3 * np.log(2) / unit,
+                  k_map=lambda k: np.where(np.arange(k.shape[-1]) < 32, 32768.0, 32.0 * j[:, None, None] + 0 * k))
+        s.Q = np.zeros((new, 2, D), np.float16)
+        s.Q[:, :, 3] = 2.0 ** (e - 15)      # times 2^15: 2^e
+        s.Q[:, :, 40] = unit / 32           # times 32 j: j units
+        _check_exact(s, np.broadcast_to(2.0 ** e + unit * j, (new, 2, length)).astype(np.float64))
+
+
 @pytest.mark.parametrize("new", [1, 100])
 def test_strided_queries_and_outputs(cuda, new):
     import torch
