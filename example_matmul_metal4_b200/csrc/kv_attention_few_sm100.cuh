@@ -18,10 +18,10 @@
 //    operand registers by logic instructions and one fp16 fused multiply-add a
 //    pair; no shuffles. For V the pairs are two keys of one element: one byte
 //    permute per two words.
-//  - P is rounded to fp16 for its product (2^-11 of itself, like the result);
-//    sums, maxima and O stay fp32.
+//  - P is rounded to fp16 for its product (2^-11 of itself, like the result, or
+//    2^-32 of the row's largest); sums, maxima and O stay fp32.
 //  - The running maximum is raised only when a score exceeds it by 8 in the log2
-//    domain (P up to 2^8), which one vote per tile decides; the stale maximum
+//    domain (P up to 2^15), which one vote per tile decides; the stale maximum
 //    cancels in O / l.
 //
 // 64 sequences of up to 8192 tokens, heads 32 / 8 of 128, 4 bits, on one B200: 97 us,
@@ -487,7 +487,7 @@ __global__ void __launch_bounds__(KvFew<D, BITS, NT, TEAM>::THREADS, 1) kv_atten
           const float m_new = fmaxf(m[nt][e], x);
           const float f = kv_ex2((m[nt][e] - m_new) * sl2);
           m[nt][e] = m_new;
-          raise[nt][e] = __fadd_rd(m_new, margin);  // down, so that no P passes 2^8 where scores lie far apart
+          raise[nt][e] = __fadd_rd(m_new, margin);  // down, so that no P passes 2^15 where scores lie far apart
           l[nt][e] *= f;
 #pragma unroll
           for (int t = 0; t < MT; ++t) {
@@ -505,7 +505,7 @@ __global__ void __launch_bounds__(KvFew<D, BITS, NT, TEAM>::THREADS, 1) kv_atten
         float p4[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          p4[e] = kv_ex2((s[hf][nt][e] - m[nt][e & 1]) * sl2);
+          p4[e] = kv_ex2(fmaf(s[hf][nt][e] - m[nt][e & 1], sl2, KV_LOG2_P));
           l[nt][e & 1] += p4[e];
         }
         pt[hf][nt][0] = kv_transpose(pack_half2(p4[0], p4[1]));

@@ -20,10 +20,10 @@
 //                 that the range leaves to others).
 //   warps 4-11    softmax, one row a thread: P = 2^((S - max) scale log2 e) with fp32
 //                 maxima and sums, P rounded to fp16 for the product (2^-11 of
-//                 itself, like the result); O is rescaled only when the maximum
-//                 grew by more than 8 in the log2 domain. Results out; a warp also
-//                 copies its rows of the next unit's Q, as soon as it has the last
-//                 scores of the unit.
+//                 itself, like the result, or 2^-32 of the row's largest); O is
+//                 rescaled only when the maximum grew by more than 8 in the log2
+//                 domain. Results out; a warp also copies its rows of the next
+//                 unit's Q, as soon as it has the last scores of the unit.
 //   warps 12-15   codes to fp16: a lane takes 32 elements (one scale and zero).
 // TMEM: two 64-column S slots for each row tile, then O_i (D columns each). Steps
 // of 64 keys are counted across a CTA's units (g), which fixes slots and
@@ -301,13 +301,14 @@ __device__ __forceinline__ float kvm_exp_store64(const float (&x)[64], float sl2
   return sum.x + sum.y;
 }
 
-// P = 2^((s - top) sl2) of a row's 64 scores, read again from the TMEM columns at tP,
-// of which the first `valid` count. kvm_exp_store64 subtracts m = fl(top sl2) in place
-// of the product, so its P are off by the rounding: a factor that a row's P share, but
-// one that passes fp16's range for scores that fp16 inputs reach (2^474). From |m| =
-// 2^20 on, where it passes 2^(1/16), m is a NaN, which takes the row's warp to this
-// function. Subtracting top from every score instead costs 5 % (prompts, head_dim 128);
-// this way, with no instruction and no register on the common path, nothing.
+// P = 2^((s - top) sl2 + KV_LOG2_P) of a row's 64 scores, read again from the TMEM
+// columns at tP, of which the first `valid` count. kvm_exp_store64 subtracts m =
+// fl(top sl2 - KV_LOG2_P) from the product, so its P are off by the rounding: a factor
+// that a row's P share, but one that passes fp16's range for scores that fp16 inputs
+// reach (2^474). From 2^20 on, where it passes 2^(1/16), m is a NaN, which takes the
+// row's warp to this function. Subtracting top from every score instead costs 5 %
+// (prompts, head_dim 128); this way, with no instruction and no register on the common
+// path, nothing.
 __device__ __forceinline__ float kvm_exp_store64_far(float sl2, float top, int valid, uint32_t tP) {
   float sum = 0.f;
 #pragma unroll 1
@@ -319,8 +320,8 @@ __device__ __forceinline__ float kvm_exp_store64_far(float sl2, float top, int v
 #pragma unroll
     for (int i = 0; i < 32; i += 2) {
       const int key = half * 32 + i;
-      const float p0 = key < valid ? ex2_approx((__uint_as_float(v[i]) - top) * sl2) : 0.f;
-      const float p1 = key + 1 < valid ? ex2_approx((__uint_as_float(v[i + 1]) - top) * sl2) : 0.f;
+      const float p0 = key < valid ? ex2_approx(fmaf(__uint_as_float(v[i]) - top, sl2, KV_LOG2_P)) : 0.f;
+      const float p1 = key + 1 < valid ? ex2_approx(fmaf(__uint_as_float(v[i + 1]) - top, sl2, KV_LOG2_P)) : 0.f;
       sum += p0 + p1;
       pk[i / 2] = pack_half2(p0, p1);
     }
@@ -331,7 +332,7 @@ __device__ __forceinline__ float kvm_exp_store64_far(float sl2, float top, int v
 
 // log2 of the factor by which kvm_exp_store64's P are too small.
 __device__ __forceinline__ float kvm_rest(float top, float sl2, bool far) {
-  return far || top == KV_NO_MAX ? 0.f : fmaf(-top, sl2, top * sl2);
+  return far || top == KV_NO_MAX ? 0.f : fmaf(-top, sl2, fmaf(top, sl2, -KV_LOG2_P)) + KV_LOG2_P;
 }
 
 template <int D, int BITS>
@@ -613,7 +614,7 @@ __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const
       } const cur{sg.n0, sg.n1, sg.steps};
       RowOf next{};
       const int limit = me.limit;
-      float m = KV_NO_MAX;  // its product with sl2, NaN from 2^20 on
+      float m = KV_NO_MAX;  // its product with sl2, less KV_LOG2_P; NaN for large ones
       float l = 0.f;
       *top() = KV_NO_MAX;
       for (int n = cur.n0; n < cur.n1; ++n, ++g) {
@@ -646,12 +647,12 @@ __global__ void __launch_bounds__(KVM_THREADS, 1) kv_attention_many_kernel(const
         }
         const float raw = att_row_max64(x);
         const float mx = raw * sl2;
-        if (__any_sync(0xffffffffu, !(mx <= m + 8.0f))) {
+        if (__any_sync(0xffffffffu, !(mx <= m + (8.0f + KV_LOG2_P)))) {
           const bool was = __any_sync(0xffffffffu, isnan(m));
           const float old = *top();
           float y = kvm_rest(old, sl2, was);
-          if (was ? raw > old : mx > m + 8.0f) {
-            m = fabsf(mx) < 0x1p20f ? mx : NAN;
+          if (was ? raw > old : mx > m + (8.0f + KV_LOG2_P)) {
+            m = fabsf(mx) < 0x1p20f ? fmaf(raw, sl2, -KV_LOG2_P) : NAN;
             *top() = raw;
             y += (old - raw) * sl2;
           }

@@ -56,6 +56,12 @@ struct KvPartial {
 // like s: the maximum gives exactly 1 however large it is. (2^(s scale log2 e - m)
 // with m in the log2 domain would be off by m's rounding, which passes 2^16 for
 // scores that fp16 inputs reach.)
+//
+// P is 2^7 times that: at most 2^15, as maxima may be stale by 8 in the log2 domain.
+// fp16 has steps of 2^-24 at the least, so P is off by 2^-32 of a row's largest and
+// not by 2^-25, which would drop the many small P of a long cache from O that l
+// counts: 2^17 keys of 2^-25.5 each are 0.3 % of a row.
+constexpr float KV_LOG2_P = 7.0f;
 constexpr float KV_NO_MAX = -1e30f;  // of a row that has seen no key: below all scores (2^39) of fp16 rows
 
 // Tiles of TK keys of a sequence (at least one: a row block with no key still
@@ -121,9 +127,9 @@ __device__ __forceinline__ float kv_ex2(float x) {
   return y;
 }
 
-// Natural-log sum of exp(scale * S) from the maximum and the sum.
+// Natural-log sum of exp(scale * S) from the maximum and the sum of P.
 __device__ __forceinline__ float kv_lse(float m, float l, float scale_log2) {
-  return fmaf(m, scale_log2, log2f(l)) * 0.6931471805599453f;
+  return fmaf(m, scale_log2, log2f(l) - KV_LOG2_P) * 0.6931471805599453f;
 }
 
 // Lets the next kernel of the stream start its blocks, and waits in it until

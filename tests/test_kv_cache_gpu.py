@@ -274,8 +274,9 @@ def test_scores_far_below_zero(cuda, new):
 
 def _exact_scores(s, S, sequence=0):
     """(O, lse, tol_O, tol_lse) in float64 of the rows of one sequence whose scores before scaling, S [n][Hq][len], are
-    exact in fp32. Beside what kv_cache_ref.attention derives, with ds = 0: the exponent y = (s - max) scale log2 e has
-    two roundings of its own and two of the factor, 2^-22 |y| in all, which shift p by as much (ln 2 < 1)."""
+    exact in fp32. What kv_cache_ref.attention derives, with ds = 0, and: the exponent y = (s - max) scale log2 e has two
+    roundings of its own and two of the factor, 2^-22 |y| in all, which shift p by as much (ln 2 < 1); a small P is off
+    by 2^-32 of the row's largest, as P is 2^7 p and fp16's steps are 2^-24."""
     n, Hq, ln = S.shape
     V = s.V[sequence].astype(np.float64).repeat(Hq // s.Hk, 1)                       # [len][Hq][D]
     scale = float(np.float32(s.plan.scale))
@@ -290,7 +291,7 @@ def _exact_scores(s, S, sequence=0):
     O, a = mean(p, V), mean(p, np.abs(V))
     rest = 2.0 ** -11 + 2.0 ** -19 + (ln / 16 + 64) * 2.0 ** -23
     tol = a * rest + mean(off, np.abs(V)) + np.abs(O) * (off.sum(-1) / total)[..., None] \
-        + np.abs(V).sum(0) * 2.0 ** -25 / total[..., None] + 2.0 ** -11 * np.abs(O) + 2.0 ** -25
+        + np.abs(V).sum(0) * 2.0 ** -32 / total[..., None] + 2.0 ** -11 * np.abs(O) + 2.0 ** -25
     lse = m[..., 0] * scale + np.log(total)
     tol_lse = off.sum(-1) / total + 2.0 ** -20 + (ln / 16 + 64) * 2.0 ** -23 + 2.0 ** -22 * np.abs(lse) \
         + 2.0 ** -22 * np.abs(m[..., 0]) * scale
@@ -319,6 +320,28 @@ def test_rows_that_one_key_dominates(cuda, key, new, name, D, bits):
     s.Q = np.zeros((new, 4, D), np.float16)
     s.Q[:, :, D - 1] = np.resize(np.float16([10, 12, 16]), (new, 4))
     _check_exact(s, s.Q[:, :, D - 1].astype(np.float64)[..., None] * c)
+
+
+@pytest.mark.parametrize("D,bits", [(128, 4), (64, 8)])
+@pytest.mark.parametrize("new,length,Hq,Hk", [(1, 1900, 4, 2), (1, 20000, 4, 2), (6, 1500, 4, 2), (12, 400, 300, 150),
+                                              (60, 300, 150, 150), (70, 2000, 4, 2)])
+@pytest.mark.parametrize("below", [18.3, 25.4, 28.5])
+def test_many_small_probabilities_add_up(cuda, below, new, length, Hq, Hk, D, bits):
+    """One key with nearly all of a row's weight and values of 0, and thousands of keys 2^-18 to 2^-28 of it: O comes
+    from those alone. Their share must not be lost to fp16."""
+    import torch
+    s = Setup(cuda, [length], [new], Hq, Hk, D=D, bits=bits, scale=np.log(2) / 64, causal=False)
+    c, v = np.zeros(length, np.float32), np.ones(length, np.float32)
+    c[length // 3], v[length // 3] = 64 * below, 0
+    K, V = (torch.from_numpy(np.broadcast_to(x.astype(np.float16)[:, None, None], (length, Hk, D)).copy()).to(cuda)
+            for x in (c, v))
+    whole = KVCacheBatch(s.batch.pageTable, s.batch.lengths, torch.tensor([0, length], dtype=torch.int32, device=cuda),
+                         length, length)
+    s.plan.append(K, V, s.cache, whole)
+    s.V = [V.cpu().numpy()]
+    s.Q = np.zeros((new, Hq, D), np.float16)
+    s.Q[:, :, 7] = 1
+    _check_exact(s, np.broadcast_to(c.astype(np.float16).astype(np.float64), (new, Hq, length)))
 
 
 @pytest.mark.parametrize("D,bits", [(128, 4), (64, 8), (64, 4), (128, 8)])
