@@ -41,7 +41,8 @@ class KVCacheBatch:
     [sequences] and `offsets` [sequences + 1] are contiguous CUDA int32 tensors; rows offsets[b] .. offsets[b+1]-1
     of K, V, Q and O are the last tokens of sequence b, whose length counts them. `tokens` is the number of rows,
     `maxNew` the most rows of one sequence. The tensors' contents are read when the kernels run, so they may be
-    updated in place between calls and between replays of a captured call."""
+    updated in place between calls and between replays of a captured call. The attributes are fixed: calls use the
+    addresses and sizes of the tensors that the batch was made of."""
 
     def __init__(self, pageTable, lengths, offsets, tokens: int, maxNew: int):
         import torch
@@ -60,7 +61,12 @@ class KVCacheBatch:
         self.sequences, self.tokens, self.maxNew, self.device = sequences, int(tokens), int(maxNew), dev
         self.desc = _lib.KVCacheBatchDesc(sequences, self.tokens, self.maxNew, pageTable.shape[1],
                                           pageTable.data_ptr(), lengths.data_ptr(), offsets.data_ptr())
-        self._ref = ctypes.addressof(self.desc)
+        self._ref = ctypes.addressof(self.desc)  # last: from here on attributes are fixed
+
+    def __setattr__(self, name, value):
+        if "_ref" in self.__dict__:
+            raise AttributeError(f"{name} of a KVCacheBatch is fixed: update the tensors in place or make another batch")
+        object.__setattr__(self, name, value)
 
 
 class KVCachePlan:

@@ -302,3 +302,16 @@ def test_a_stream_of_another_device_is_refused(monkeypatch):
             call(FakeStream(1))
         call(FakeStream(0))
     assert len(env.calls) == 3
+
+
+def test_attributes_of_a_batch_are_fixed(monkeypatch):
+    """Another tensor in place of a batch's would leave the old address in the descriptor and drop its memory."""
+    import torch
+    env = FakeEnv(monkeypatch)
+    for name in ("pageTable", "lengths", "offsets", "tokens", "maxNew", "sequences", "device", "desc"):
+        kept = getattr(env.batch, name)
+        with pytest.raises(AttributeError, match="fixed"):
+            setattr(env.batch, name, FakeTensor((3,), torch.int32, env))
+        assert getattr(env.batch, name) is kept
+    env.plan.append(env.K, env.K, env.cache, env.batch)
+    assert len(env.calls) == 1
