@@ -36,6 +36,13 @@ class KVCacheDimensions:
     bits: int = 4
 
 
+def _fits(bits: int, **sizes):
+    """Refuses sizes that the descriptors' integers, of `bits` bits beside the sign, would cut."""
+    for name, n in sizes.items():
+        if not -(1 << bits) <= n < 1 << bits:
+            raise ValueError(f"{name} {n} is out of range")
+
+
 class KVCacheBatch:
     """The sequences of one call (mm4_kv_cache_batch). `pageTable` [sequences][pages per sequence], `lengths`
     [sequences] and `offsets` [sequences + 1] are contiguous CUDA int32 tensors; rows offsets[b] .. offsets[b+1]-1
@@ -57,6 +64,7 @@ class KVCacheBatch:
             raise ValueError(f"{sequences} lengths need {sequences} page-table rows and {sequences + 1} offsets")
         if tokens < 0 or maxNew < 0:
             raise ValueError("tokens and maxNew must not be negative")
+        _fits(31, tokens=tokens, maxNew=maxNew, sequences=sequences, pagesPerSequence=pageTable.shape[1])
         self.pageTable, self.lengths, self.offsets = pageTable, lengths, offsets
         self.sequences, self.tokens, self.maxNew, self.device = sequences, int(tokens), int(maxNew), dev
         self.desc = _lib.KVCacheBatchDesc(sequences, self.tokens, self.maxNew, pageTable.shape[1],
@@ -79,6 +87,8 @@ class KVCachePlan:
 
     def __init__(self, dims: KVCacheDimensions, causal: bool = True, scale: float | None = None):
         self._L = _lib.lib()
+        _fits(63, pages=dims.pages)
+        _fits(31, pageSize=dims.pageSize, Hq=dims.Hq, Hk=dims.Hk, K=dims.K, bits=dims.bits)
         self.dims = dims
         self.causal = bool(causal)
         self.scale = scale if scale is not None else 1.0 / math.sqrt(dims.K) if dims.K > 0 else 0.0

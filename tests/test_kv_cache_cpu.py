@@ -315,3 +315,19 @@ def test_attributes_of_a_batch_are_fixed(monkeypatch):
         assert getattr(env.batch, name) is kept
     env.plan.append(env.K, env.K, env.cache, env.batch)
     assert len(env.calls) == 1
+
+
+def test_sizes_beyond_the_descriptors_are_refused(monkeypatch):
+    """Sizes that would arrive as others, cut to 32 (pages: 64) bits."""
+    import torch
+    from example_matmul_metal4_b200.kv_cache import KVCacheBatch, KVCacheDimensions, KVCachePlan
+    good = dict(pages=4, pageSize=64, Hq=8, Hk=2, K=128, bits=4)
+    KVCachePlan(KVCacheDimensions(**good))
+    for name, value in good.items():
+        with pytest.raises(ValueError, match=name):
+            KVCachePlan(KVCacheDimensions(**{**good, name: value + (1 << (64 if name == "pages" else 32))}))
+    env = FakeEnv(monkeypatch)
+    tensors = (FakeTensor((3, 4), torch.int32, env), FakeTensor((3,), torch.int32, env), FakeTensor((4,), torch.int32, env))
+    for sizes in ((5 + (1 << 32), 2), (5, 2 + (1 << 32)), (5, 1 << 31)):
+        with pytest.raises(ValueError, match="out of range"):
+            KVCacheBatch(*tensors, *sizes)
