@@ -36,10 +36,10 @@ class KVCacheDimensions:
     bits: int = 4
 
 
-def _fits(bits: int, **sizes):
-    """Refuses sizes that the descriptors' integers, of `bits` bits beside the sign, would cut."""
+def _fits(width: int, **sizes):
+    """Refuses sizes that the descriptors' integers, of `width` bits beside the sign, would cut."""
     for name, n in sizes.items():
-        if not -(1 << bits) <= n < 1 << bits:
+        if not -(1 << width) <= n < 1 << width:
             raise ValueError(f"{name} {n} is out of range")
 
 
