@@ -79,7 +79,7 @@ class KVCacheBatch:
 
 class KVCachePlan:
     """Cache geometry and attention options. `causal`: a token attends to itself and what lies before it (else to
-    all its sequence has cached); `scale` as in AttentionPlan. Immutable; may be used from several streams.
+    all its sequence has cached); `scale` None, 0 or less: 1 / sqrt(K). Immutable; may be used from several streams.
 
     `stream` of a call is a torch stream of the tensors' device (None: the current one). Its kernels follow what that
     stream holds already; inputs that another stream writes need a wait of the caller's, as do outputs read elsewhere.
@@ -91,12 +91,12 @@ class KVCachePlan:
         _fits(31, pageSize=dims.pageSize, Hq=dims.Hq, Hk=dims.Hk, K=dims.K, bits=dims.bits)
         self.dims = dims
         self.causal = bool(causal)
-        self.scale = scale if scale is not None else 1.0 / math.sqrt(dims.K) if dims.K > 0 else 0.0
         d = _lib.KVCacheDesc(dims.pages, dims.pageSize, dims.Hq, dims.Hk, dims.K, dims.bits, int(self.causal),
-                             float(self.scale))
+                             0.0 if scale is None else float(scale))
         h = ctypes.c_void_p()
         _lib.check(self._L.mm4_kv_cache_plan_create(ctypes.byref(h), ctypes.byref(d)))
         self._h = h
+        self.scale = float(scale) if d.scale > 0 else 1.0 / math.sqrt(dims.K)  # what the kernels use, as in mm4.h
         import torch
         self._f16, self._u8, self._f32 = torch.float16, torch.uint8, torch.float32
         self._empty_like, self._device = torch.empty_like, torch._C._cuda_getDevice

@@ -331,3 +331,14 @@ def test_sizes_beyond_the_descriptors_are_refused(monkeypatch):
     for sizes in ((5 + (1 << 32), 2), (5, 2 + (1 << 32)), (5, 1 << 31)):
         with pytest.raises(ValueError, match="out of range"):
             KVCacheBatch(*tensors, *sizes)
+
+
+@pytest.mark.parametrize("scale,used", [(None, 1 / 128 ** 0.5), (0, 1 / 128 ** 0.5), (-2.0, 1 / 128 ** 0.5), (1e-60, 1 / 128 ** 0.5),
+                                        (0.25, 0.25), (1, 1.0)])
+def test_scale_of_a_plan_is_the_one_that_its_kernels_use(scale, used):
+    """A scale of 0 or less (in fp32) selects 1 / sqrt(head_dim)."""
+    from example_matmul_metal4_b200.kv_cache import KVCacheDimensions, KVCachePlan
+    assert KVCachePlan(KVCacheDimensions(4, 64, 8, 2, 128), scale=scale).scale == used
+    for bad in (float("nan"), float("inf"), 1e300):
+        with pytest.raises(_lib.MM4Error):
+            KVCachePlan(KVCacheDimensions(4, 64, 8, 2, 128), scale=bad)
