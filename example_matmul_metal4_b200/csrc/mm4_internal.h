@@ -65,9 +65,10 @@ mm4_status launch_debug_wait(int* word, uint64_t timeout_ns, cudaStream_t stream
 mm4_status noalloc_take_status(int dev, int* code);
 
 // Reads and clears the status words of the key / value cache kernels on device
-// `dev` (both 0 when none ever ran there); the caller has synchronised the
-// stream. `wait` is a run-out wait, `data` what the kernels found wrong in a
-// batch's arrays. Defined in mm4_kv_cache.cu.
+// `dev` (left as they are when none ever ran there); the caller has synchronised
+// the stream. `wait` is a run-out wait, `data` what the kernels found wrong in a
+// batch's arrays: left for the next call where `wait` reports something, or
+// `data` is null. Defined in mm4_kv_cache.cu.
 mm4_status kv_cache_take_status(int dev, int* wait, int* data);
 // What a data site of the key / value cache kernels stands for.
 const char* kv_cache_site_text(int site);

@@ -248,12 +248,12 @@ mm4_status launch_many(KvAttnArgs& a, int sms, cudaStream_t st) {
 namespace mm4 {
 
 mm4_status kv_cache_take_status(int dev, int* wait, int* data) {
-  *wait = *data = 0;
   if (dev < 0 || dev >= kMaxDevices || !g_used[dev].load()) return MM4_OK;
   const int zero = 0;
   MM4_CUDA_TRY(cudaMemcpyFromSymbol(wait, g_kv_wait, sizeof(int)));
-  MM4_CUDA_TRY(cudaMemcpyFromSymbol(data, g_kv_data, sizeof(int)));
   if (*wait != 0) MM4_CUDA_TRY(cudaMemcpyToSymbol(g_kv_wait, &zero, sizeof(int)));
+  if (*wait != 0 || !data) return MM4_OK;
+  MM4_CUDA_TRY(cudaMemcpyFromSymbol(data, g_kv_data, sizeof(int)));
   if (*data != 0) MM4_CUDA_TRY(cudaMemcpyToSymbol(g_kv_data, &zero, sizeof(int)));
   return MM4_OK;
 }

@@ -280,10 +280,10 @@ mm4_status mm4_check(mm4_stream_t stream) {
   if (rc != MM4_OK) return rc;
   if (v == 0) v = nv;
   int kv_wait = 0, kv_data = 0;
-  rc = kv_cache_take_status(dev, &kv_wait, &kv_data);
+  rc = kv_cache_take_status(dev, &kv_wait, v == 0 ? &kv_data : nullptr);
   if (rc != MM4_OK) return rc;
   if (v == 0) v = kv_wait;
-  if (v == 0 && kv_data != 0)
+  if (kv_data != 0)
     return fail(kv_data & 0xff, "key / value cache batch: %s", kv_cache_site_text(kv_data >> 8));
   if (v != 0) {
     const int code = v & 0xff;

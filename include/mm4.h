@@ -58,8 +58,8 @@ MM4_API int mm4_device_supported(void);
  * two of the mm4_kv_cache_* calls.
  * Returns MM4_ERR_TIMEOUT when a kernel recorded a run-out wait (the
  * message names the wait site), MM4_ERR_INVALID when an mm4_kv_cache_* kernel
- * found a wrong page number, length or offset in its batch, MM4_ERR_CUDA on a
- * CUDA error, else MM4_OK.
+ * found a wrong page number, length or offset in its batch (reported by the next
+ * call if there was a run-out wait too), MM4_ERR_CUDA on a CUDA error, else MM4_OK.
  * It allocates no device memory. */
 MM4_API mm4_status mm4_check(mm4_stream_t stream);
 

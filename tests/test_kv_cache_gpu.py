@@ -806,6 +806,20 @@ def test_append_and_read_leave_out_wrong_sequences_and_report_them(cuda, what, n
         assert (out[~read] == -3.0).all()
 
 
+def test_a_wrong_batch_is_reported_behind_a_run_out_wait(cuda):
+    """A check reports one thing; what it does not report stays for the next."""
+    from example_matmul_metal4_b200._lib import MM4_ERR_TIMEOUT, check, lib, stream_handle
+    import torch
+    s = Setup(cuda, [200], [1], 4, 2)
+    s.batch.pageTable[0, 1] = -1
+    s.plan.attention(torch.from_numpy(s.Q).to(cuda), s.cache, s.batch)
+    check(lib().mm4_debug_wait_timeout(1_000_000, stream_handle()))  # a wait that runs out after 1 ms
+    with pytest.raises(MM4Error) as e:
+        sync_check()
+    assert e.value.status == MM4_ERR_TIMEOUT
+    _reported("page number")
+
+
 @pytest.mark.parametrize("new", [1, 100])
 def test_wrong_lengths_offsets_and_row_counts_are_reported(cuda, new):
     import torch
