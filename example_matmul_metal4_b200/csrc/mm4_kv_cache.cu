@@ -377,6 +377,8 @@ mm4_status mm4_kv_cache_attention(const mm4_kv_cache_plan* p, const mm4_kv_cache
       return fail(MM4_ERR_WORKSPACE, "attention over this batch needs a %zu-byte workspace", form.workspace);
     if (!aligned16(workspace)) return fail(MM4_ERR_INVALID, "workspace must be 16-byte aligned");
   }
+  // Workers read the Q of a unit when others have written their rows of O.
+  if (O == Q) return fail(MM4_ERR_INVALID, "O must not be Q");
   DeviceInfo info;
   if ((rc = use_device(&info)) != MM4_OK) return rc;
   KvAttnArgs a{};

@@ -342,3 +342,14 @@ def test_scale_of_a_plan_is_the_one_that_its_kernels_use(scale, used):
     for bad in (float("nan"), float("inf"), 1e300):
         with pytest.raises(_lib.MM4Error):
             KVCachePlan(KVCacheDimensions(4, 64, 8, 2, 128), scale=bad)
+
+
+@pytest.mark.parametrize("max_new", [2, 13])
+def test_attention_in_place_of_its_queries_is_refused(max_new):
+    L = _lib.lib()
+    rc, h = _plan()
+    assert rc == 0
+    assert L.mm4_kv_cache_attention(h, ctypes.byref(_batch(max_new=max_new)), FAKE, 1024, FAKE, FAKE, 1024, None, FAKE,
+                                    1 << 40, None) == INVALID
+    assert b"must not be Q" in L.mm4_last_error()
+    L.mm4_kv_cache_plan_destroy(h)
