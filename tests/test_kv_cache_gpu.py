@@ -134,6 +134,66 @@ def test_append_writes_the_defined_bytes_and_nothing_else(cuda, D, Hk, page, bit
     assert (out[used:] == -3.0).all() and (out[:, 2 * Hk * D:] == -3.0).all()
 
 
+@pytest.mark.parametrize("tokens,Hk,D,bits,per_warp", [(9501, 5, 128, 4, 2), (9600, 5, 128, 8, 2), (30001, 1, 128, 8, 3),
+                                                       (47403, 3, 64, 8, 5), (76003, 3, 64, 4, 8)])
+def test_append_and_read_of_several_tokens_a_warp(cuda, tokens, Hk, D, bits, per_warp):
+    """Calls large enough for a warp to take several tokens, which cross sequences of every length, empty ones and
+    rows before position 0 among them; padding at both ends, a last warp with fewer tokens, strides of their own for K
+    and V. Every byte of the cache and every row is compared."""
+    import torch
+    sms = torch.cuda.get_device_properties(cuda).multi_processor_count
+    parts = (2 * Hk * D // 8 + 127) // 128
+    assert max(1, min(8, tokens * parts // (64 * sms))) == per_warp
+    rng = np.random.default_rng(tokens)
+    page, first, last = 32, 5, tokens - 3
+    cut = np.unique(np.concatenate([[first, last], first + 1 + rng.integers(0, last - first - 1, 300),
+                                    first + np.arange(1, 40)]))
+    new = np.diff(cut)
+    new = np.insert(new, [0, 17, 17, len(new)], 0)                    # sequences without rows
+    offsets = (first + np.concatenate([[0], np.cumsum(new)])).astype(np.int32)
+    assert offsets[-1] == last
+    lengths = (new + rng.integers(0, 50, len(new))).astype(np.int32)
+    lengths[::9] = np.maximum(0, new[::9] - 4)                        # rows before position 0
+    used = (lengths + page - 1) // page
+    pages, table = int(used.sum()) + 2, np.full((len(new), int(used.max())), 2 ** 30, np.int32)
+    order, at = rng.permutation(pages), 0
+    for b, n in enumerate(used):
+        table[b, :n] = order[at:at + n]
+        at += n
+    K, V = data.normal((tokens, Hk, D), 1.0, tokens, 0), data.normal((tokens, Hk, D), 2.0, tokens, 1)
+    packed = [ref.pack(x, bits) for x in (K, V)]
+    values = [ref.unpack(x, D, bits) for x in packed]
+    t = np.arange(first, last)
+    b = np.searchsorted(offsets, t, side="right") - 1
+    pos = lengths[b] - (offsets[b + 1] - t)
+    placed = pos >= 0
+    t, b, pos = t[placed], b[placed], pos[placed]
+    host = np.full((pages, Hk, 2, page, ref.row_bytes(D, bits)), 0xA5, dtype=np.uint8)
+    cache = torch.from_numpy(host.reshape(pages, -1).copy()).to(cuda)
+    for kv in (0, 1):
+        host[table[b, pos // page], :, kv, pos % page] = packed[kv][t]
+    width = Hk * D
+    strided = [torch.full((tokens, width + extra), -3.0, dtype=torch.float16, device=cuda) for extra in (8, 24)]
+    k, v = (x[:, :width].unflatten(1, (Hk, D)) for x in strided)
+    k.copy_(torch.from_numpy(K))
+    v.copy_(torch.from_numpy(V))
+    i32 = dict(dtype=torch.int32, device=cuda)
+    batch = KVCacheBatch(torch.from_numpy(table).to(cuda), torch.tensor(lengths, **i32), torch.tensor(offsets, **i32),
+                         tokens, int(new.max()))
+    plan = KVCachePlan(KVCacheDimensions(pages, page, Hk, Hk, D, bits))
+    plan.append(k, v, cache, batch)
+    sync_check()
+    assert np.array_equal(cache.cpu().numpy().reshape(host.shape), host)
+    for x in strided:
+        x.fill_(-3.0)
+    plan.read(cache, batch, K=k, V=v)
+    sync_check()
+    for kv, x in enumerate(strided):
+        want = np.full(x.shape, -3.0, np.float16)
+        want[t, :width] = values[kv][t].reshape(len(t), width)
+        assert np.array_equal(x.cpu().numpy(), want)
+
+
 @pytest.mark.parametrize("bits", [4, 8])
 def test_groups_at_the_edges_of_fp16(cuda, bits):
     """Constant groups, zeros of both signs, NaN and infinities, the widest range, subnormals, a range of one
@@ -418,6 +478,60 @@ def test_many_sequences_on_shared_pages(cuda, new, maxNew):
         r = slice(b * new, (b + 1) * new)
         eO, _, tO, _ = ref.attention(Q[r], base.K[0][:lengths[b]], base.V[0][:lengths[b]], new, True, base.plan.scale)
         assert (np.abs(got[r] - eO) <= tO).all(), b
+
+
+@pytest.mark.parametrize("D", [128, 64])
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("new,name", [(1, "few<8 rows, split>"), (2, "few<8 rows, split>"), (3, "few<16 rows, split>"),
+                                      (4, "few<16 rows, split>"), (5, "few<24 rows, split>"), (11, "few<24 rows, split>"),
+                                      (13, "many")])
+def test_each_kernel_over_long_caches(cuda, new, name, bits, D):
+    """More tokens than a unit of its own CTA takes: every row count, width and head_dim on ranges that are split, with
+    lengths around the borders of tiles and pages, and a sequence of no row."""
+    lengths, rows = [5003, 2049, 64, 31, 2500], [new, max(1, new - 1), new, 1, 0]
+    s = Setup(cuda, lengths, rows, 8, 2, D=D, bits=bits, page=16, maxNew=new)
+    assert name in s.plan.attention_kernel_name(s.batch)
+    s.check(*s.attend())
+
+
+def _check_rows(s, O, lse, b, rows):
+    """Single rows of a causal sequence, each as the last token of what it sees."""
+    for i in rows:
+        r, seen = int(s.offsets[b]) + i, s.lengths[b] - s.new[b] + i + 1
+        eO, eL, tO, tL = ref.attention(s.Q[r:r + 1], s.K[b][:seen], s.V[b][:seen], 1, True, s.plan.scale)
+        assert (np.abs(O[r:r + 1].double().cpu().numpy() - eO) <= tO).all(), (b, i)
+        assert (np.abs(lse[r:r + 1].double().cpu().numpy() - eL) <= tL).all(), (b, i)
+
+
+@pytest.mark.parametrize("D,bits", [(128, 4), (64, 8)])
+@pytest.mark.parametrize("sequences", [40, 70, 150])
+def test_many_rows_of_many_sequences(cuda, sequences, D, bits):
+    """More sequences than a warp has lanes, of up to 30 tokens with 4 heads each, some with none."""
+    rng = np.random.default_rng(sequences)
+    rows = rng.integers(1, 31, sequences)
+    rows[[3, 33, sequences - 1]], rows[5] = 0, 30
+    lengths = rows + rng.integers(0, 200, sequences)
+    s = Setup(cuda, [int(x) for x in lengths], [int(x) for x in rows], 8, 2, D=D, bits=bits, page=32, maxNew=30)
+    assert "many" in s.plan.attention_kernel_name(s.batch)
+    s.check(*s.attend())
+
+
+@pytest.mark.parametrize("D,bits", [(128, 4), (64, 8)])
+@pytest.mark.parametrize("others", [0, 2, 45])
+def test_more_row_blocks_than_a_warp_has_lanes(cuda, others, D, bits):
+    """A prompt of 4200 tokens with 2 heads a key / value head: 33 blocks of 256 rows, alone, between fewer sequences
+    than blocks and between more of them."""
+    rng = np.random.default_rng(others)
+    small = [int(x) for x in rng.integers(1, 60, others)]
+    new = small[:others // 2] + [4200] + small[others // 2:]
+    lengths = [n + int(rng.integers(0, 40)) for n in new]
+    s = Setup(cuda, lengths, new, 4, 2, D=D, bits=bits)
+    assert "many" in s.plan.attention_kernel_name(s.batch)
+    O, lse = s.attend()
+    big = others // 2
+    s.check(O, lse, sequences=[b for b in range(others + 1) if b != big])
+    _check_rows(s, O, lse, big, [0, 1, 63, 127, 128, 255, 256, 1000, 2047, 4096, 4150, 4199] +
+                [int(x) for x in rng.integers(0, 4200, 30)])
 
 
 @pytest.mark.parametrize("new", [1, 5, 200])
