@@ -23,6 +23,7 @@ struct mm4_kv_cache_plan {
 namespace {
 
 constexpr int kMaxDevices = 64;
+constexpr float LOG2E = 1.4426950408889634f;
 // Set once a kernel that can write the status words was launched on a device;
 // before that mm4_check has nothing to read there.
 std::atomic<bool> g_used[kMaxDevices];
@@ -287,6 +288,7 @@ mm4_status mm4_kv_cache_plan_create(mm4_kv_cache_plan** out, const mm4_kv_cache_
   if (d->head_dim != 128 && d->head_dim != 64)
     return fail(MM4_ERR_UNSUPPORTED, "head_dim %d: this build implements head_dim 128 and 64", d->head_dim);
   if (std::isnan(d->scale) || std::isinf(d->scale)) return fail(MM4_ERR_INVALID, "scale must be finite");
+  if (d->scale > 0.f && std::isinf(d->scale * LOG2E)) return fail(MM4_ERR_UNSUPPORTED, "scale %g: at most 2^127", d->scale);
   if (d->heads_q > 4096) return fail(MM4_ERR_UNSUPPORTED, "heads_q %d: at most 4096", d->heads_q);
   if (d->pages > 0x7fffffffLL) return fail(MM4_ERR_UNSUPPORTED, "more than 2^31 - 1 pages");
   mm4_kv_cache_plan* p = new (std::nothrow) mm4_kv_cache_plan();
@@ -392,7 +394,7 @@ mm4_status mm4_kv_cache_attention(const mm4_kv_cache_plan* p, const mm4_kv_cache
   a.heads_q = p->d.heads_q;
   a.group = p->d.heads_q / p->d.heads_kv;
   a.causal = p->d.causal;
-  a.scale_log2 = p->scale * 1.4426950408889634f;
+  a.scale_log2 = p->scale * LOG2E;
   a.partials = static_cast<float*>(workspace);
   a.k1024 = KV_1024;
   a.timeout_ns = wait_timeout_ns();

@@ -353,3 +353,10 @@ def test_attention_in_place_of_its_queries_is_refused(max_new):
                                     1 << 40, None) == INVALID
     assert b"must not be Q" in L.mm4_last_error()
     L.mm4_kv_cache_plan_destroy(h)
+
+
+def test_scale_whose_product_with_log2_e_is_infinite_is_refused():
+    for scale, want in ((2.0 ** 127, 0), (2.3e38, 0), (2.4e38, UNSUPPORTED), (3.4e38, UNSUPPORTED), (-3.4e38, 0)):
+        rc, h = _plan(scale=scale)
+        assert rc == want, scale
+        _lib.lib().mm4_kv_cache_plan_destroy(h)
