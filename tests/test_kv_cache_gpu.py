@@ -420,6 +420,43 @@ def test_scores_at_the_ends_of_fp16(cuda, scale, new, length, D, bits):
 
 
 @pytest.mark.parametrize("D,bits", [(128, 4), (64, 8)])
+@pytest.mark.parametrize("new,length", [(1, 300), (3, 4000), (12, 300), (70, 500)])
+@pytest.mark.parametrize("e", [126, 60, 20, -20, -60, -126])
+def test_scales_at_the_ends_of_fp32(cuda, e, new, length, D, bits):
+    """A row that sees one key only, rows with equal largest scores and rows of zeros, at scales of 2^126 to 2^-126; lse
+    where fp32 holds it."""
+    c = np.resize(np.float32([2, -3, 0.5, 2, 1.5, 0]), length)
+    s = Setup(cuda, [length], [new], 4, 2, D=D, bits=bits, scale=2.0 ** e, k_map=lambda k: np.ones_like(k) * c[:, None, None])
+    q = np.resize(np.float16([1, -1, 0, 2.0 ** -10, 300]), (new, 4))
+    s.Q = np.zeros((new, 4, D), np.float16)
+    s.Q[:, :, 9] = q
+    O, lse = s.attend()
+    eO, eL, tO, tL = _exact_scores(s, q.astype(np.float64)[..., None] * c.astype(np.float64))
+    assert (np.abs(O.double().cpu().numpy() - eO) <= tO).all()
+    got, held = lse.double().cpu().numpy(), np.abs(eL) < 1e38
+    assert held.any() and (np.abs(got - eL) <= tL)[held].all()
+
+
+@pytest.mark.parametrize("D,bits", [(128, 4), (64, 8)])
+@pytest.mark.parametrize("new,length", [(1, 300), (1, 3000), (3, 4000), (12, 700), (70, 500)])
+def test_rows_of_nan_and_infinities_stay_alone(cuda, new, length, D, bits):
+    """A NaN or an infinity in a row of Q makes that row's results NaN, as in the formula. The other rows stay within
+    their tolerance (not bit for bit: the many-row kernel takes the exponents of a large row's warp another way)."""
+    s = Setup(cuda, [length, 77], [new, new], 8, 2, D=D, bits=bits, k_map=lambda k: np.abs(k) + 0.5)
+    bad = [(0, 1, np.nan), (new - 1, 2, np.inf), (new, 7, np.nan), (2 * new - 1, 4, np.inf)]
+    want = [ref.attention(s.Q[b * new:(b + 1) * new], s.K[b], s.V[b], new, True, s.plan.scale) for b in (0, 1)]
+    eO, eL, tO, tL = (np.concatenate(x) for x in zip(*want))
+    for r, h, x in bad:
+        s.Q[r, h, D // 2] = x
+    O, lse = (t.double().cpu().numpy() for t in s.attend())
+    other = np.ones(lse.shape, bool)
+    for r, h, _ in bad:
+        assert np.isnan(O[r, h]).all() and np.isnan(lse[r, h]), (r, h)
+        other[r, h] = False
+    assert (np.abs(lse - eL) <= tL)[other].all() and (np.abs(O - eO) <= tO)[other].all()
+
+
+@pytest.mark.parametrize("D,bits", [(128, 4), (64, 8)])
 @pytest.mark.parametrize("e", [24, 27, 30])
 @pytest.mark.parametrize("new,length", [(1, 900), (1, 5000), (12, 700), (70, 1500)])
 def test_maximum_rises_by_single_steps_of_fp32(cuda, new, length, e, D, bits):
