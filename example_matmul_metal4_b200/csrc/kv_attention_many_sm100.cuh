@@ -29,11 +29,11 @@
 // of 64 keys are counted across a CTA's units (g), which fixes slots and
 // mbarrier phases; S runs two steps ahead of the softmax.
 //
-// Four prompts of 4096 tokens, 16 heads of 128, causal, 4 bits, on one B200: 301 us,
-// 914 TFLOP/s (floor 163 us of measured peak). A step of 64 keys takes about
-// 2000 clocks, of which the products need 1280 (S of N = 64 is bound by the
-// 6 KB an instruction reads from shared memory); unpacking alone costs 11 %,
-// its 42 KB a step through shared memory among them.
+// Four prompts of 4096 tokens, 16 heads of 128, causal, 4 bits, on one B200: 297 us,
+// 926 TFLOP/s (floor 163 us of measured peak); 344 us in long runs, under the power
+// cap. A step of 64 keys takes about 2000 clocks, of which the products need 1280
+// (S of N = 64 is bound by the 6 KB an instruction reads from shared memory);
+// unpacking alone costs 11 %, its 42 KB a step through shared memory among them.
 #pragma once
 
 #include "attention_sm100.cuh"

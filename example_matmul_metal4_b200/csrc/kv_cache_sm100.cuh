@@ -150,7 +150,9 @@ __device__ __forceinline__ __half2 kv_bits_1024(uint32_t x, uint32_t mask, uint3
 }
 
 // The codes of a word whose 16-bit halves hold four 4-bit codes each: out[j] =
-// (code j of the low half, code j of the high half) as exact integers.
+// (code j of the low half, code j of the high half) as exact integers. Codes under the
+// exponent of 1024, which is then taken off, are a published way to halves (Kim et al.,
+// "Who Says Elephants Can't Run", 2022).
 __device__ __forceinline__ void kv_codes4(uint32_t w, __half2 (&out)[4], uint32_t k1024) {
   const __half2 m1024 = __float2half2_rn(-1024.0f), m64 = __float2half2_rn(-64.0f),
                 sixteenth = __float2half2_rn(0.0625f);
@@ -285,9 +287,10 @@ __device__ __forceinline__ float kv_divide_by_top(float x) {
 // Quantises K and V of the batch's rows. A warp takes 128 vectors of 8 elements of
 // each of its tokens; the four lanes of a group of 32 find its range by two
 // shuffles of one register. Its floor are the bytes it moves: 512 in and 160 out
-// per token and head at D = 128 in 4 bits, 23 us for four prompts of up to 4096
-// tokens and 16 heads; it takes 51 us (142 instructions for 8 elements a lane, issue
-// slots 64 % busy).
+// per token and head at D = 128 in 4 bits, 25 us for four prompts of up to 4096
+// tokens and 16 heads; it takes 50 us, and as much in 8 bits (30 us of bytes). No unit
+// is full (issue slots 64 %, logic 45 %): 142 instructions for 8 elements a lane, and a
+// token's loads wait for the codes of the one before it.
 template <int D, int BITS>
 __global__ void __launch_bounds__(KV_IO_WARPS * 32, 6) kv_append_kernel(const KvIoArgs a) {
   constexpr int TOP = (1 << BITS) - 1;
@@ -383,7 +386,8 @@ __global__ void __launch_bounds__(KV_IO_WARPS * 32, 6) kv_append_kernel(const Kv
 }
 
 // Reads the rows of a batch back as fp16 values; the mapping of kv_append_kernel.
-// Bound by memory: 8 sequences of up to 8192 tokens, 306 MB, in 55 us (5.6 TB/s).
+// Bound by memory: 8 sequences of up to 8192 tokens and 8 heads of 128 in 4 bits, 306 MB,
+// in 59 us (5.2 TB/s), in 8 bits, 364 MB, in 72 us (5.1).
 template <int D, int BITS>
 __global__ void __launch_bounds__(KV_IO_WARPS * 32) kv_read_kernel(const KvIoArgs a) {
   using Row = KvRow<D, BITS>;

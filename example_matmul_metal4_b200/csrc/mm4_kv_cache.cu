@@ -134,13 +134,32 @@ mm4_status launch_io(const mm4_kv_cache_plan* p, KvIoArgs& a, bool write, cudaSt
 //          FEW       42     72    100    128    327 us
 //          MANY      75     76     77     77     84 us
 //          (heads of 64, 8 bits: FEW 31, 50, 68, 86, 215, MANY 70, 73, 73, 75, 81).
+//          The most rows of any sequence decide for all: 63 single tokens over up to
+//          8192 take 102 us, a chunk of 1000 on 4000 takes 79, both in one call 365.
 //   TEAM   FEW of at most 16 rows where no sequence can hold more than 2048 tokens
-//          and there are no more units than SMs: a whole unit to a CTA, one
-//          launch, no workspace. 8 rows, 8 heads of 128, TEAM against split ranges:
-//          tokens              64           1024          2048
-//          1 sequence      4.8,  7.6     9.0, 11.2    13.2, 11.8 us
-//          16 sequences    5.2, 10.8     9.4, 15.8    13.9, 19.7 us
-//          64 sequences   15.1, 13.1    32.6, 29.5    55.0, 46.3 us
+//          and there are no more units than the 148 SMs of a B200 (the workspace is
+//          asked for without a device): a whole unit to a CTA, one launch, no
+//          workspace. 8 heads, TEAM against split ranges, us:
+//                                    64 tokens     512          1024         2048
+//          128, 4 bits, 8 rows
+//             1 sequence             6.2,  7.5   8.1,  8.3   9.9,  9.5  14.1,  9.9
+//             4                      6.4,  8.0   8.3, 10.0  10.2, 10.7  14.0, 13.0
+//             18                     6.6, 12.5   8.6, 16.1  10.6, 19.2  14.4, 23.1
+//             64                    20.8, 13.4  27.8, 21.7  37.6, 30.1
+//          128, 4 bits, 16 rows
+//             1 sequence             6.9,  8.3   9.7, 10.0  12.5, 10.3  19.0, 11.1
+//             18                     7.5, 13.1   9.9, 18.4  13.0, 20.5  20.0, 26.4
+//             64                    23.0, 18.7  33.7, 28.6  45.4, 39.5
+//          128, 8 bits, 8 rows
+//             1 sequence             5.2,  7.5   7.7,  7.8  10.1,  8.1  15.8,  8.5
+//             18                     5.4, 12.2   8.3, 15.8  10.6, 18.3  16.7, 23.1
+//             64                    15.6, 13.1  25.7, 21.9  39.3, 37.2
+//          64, 8 bits, 8 rows (4 bits alike)
+//             1 sequence             4.6,  7.3   6.5,  8.5   8.1, 10.5  11.9, 10.8
+//             18                     4.8, 10.3   6.6, 12.8   8.5, 14.6  12.2, 18.2
+//             64                    14.0, 11.8  19.4, 18.7  25.7, 25.6
+//          The room of a table is known here, the lengths in it are not: one or a few
+//          sequences that nearly fill 2048 tokens are the ones that lose.
 struct Form {
   enum Kind { FEW8, FEW16, FEW24, MANY } kind;
   bool team;

@@ -425,8 +425,11 @@ MM4_API mm4_status mm4_kv_cache_read(const mm4_kv_cache_plan* plan, const mm4_kv
  * rows q_stride / o_stride elements apart (multiples of 8, at least
  * heads_q * head_dim; 16-byte aligned bases). lse, if not NULL, receives fp32
  * [tokens][heads_q] natural-log sums of exp(scale * S). A row that attends to
- * nothing gets O = 0 and lse = -infinity. fp32 softmax statistics and sums. O and
- * lse must not overlap Q or each other. One launch or two.
+ * nothing gets O = 0 and lse = -infinity. Scores, softmax statistics and sums are
+ * fp32; the probabilities are rounded to fp16 for their product with V (2^-11 of
+ * themselves, or 2^-32 of the row's largest). O and lse must not overlap Q or each
+ * other. One launch or two. The kernel is chosen by max_new for the whole call: rows
+ * of one token beside a long chunk are slower in its call than in one of their own.
  * workspace: mm4_kv_cache_attention_workspace_size() bytes, 16-byte aligned, any
  * contents; calls that may overlap on the GPU need one each. */
 MM4_API size_t mm4_kv_cache_attention_workspace_size(const mm4_kv_cache_plan* plan, const mm4_kv_cache_batch* batch);
