@@ -68,14 +68,16 @@ class GemmPlan:
     def handle(self) -> ctypes.c_void_p:
         return self._h
 
-    def workspace(self, device):
-        """A zero-filled workspace for this plan on `device` (kernels leave it zeroed)."""
+    def workspace(self, device, stream=None):
+        """A zero-filled workspace for this plan on `device` (kernels leave it zeroed), filled in the order of `stream`
+        where this call makes it. Runs that share it follow one another."""
         import torch
         if self.workspace_bytes == 0:
             return None
         key = str(device)
         if key not in self._ws:
-            self._ws[key] = torch.zeros(self.workspace_bytes, dtype=torch.uint8, device=device)
+            self._ws[key] = _lib.new_on_stream(stream, lambda: torch.zeros(self.workspace_bytes, dtype=torch.uint8,
+                                                                           device=device))
         return self._ws[key]
 
     def a_shape(self):
@@ -96,7 +98,7 @@ class GemmPlan:
             _check_tensor(bias, (d.N,), "bias")
         if C is None:
             C = _lib.new_on_stream(stream, lambda: torch.empty((d.M, d.N), dtype=torch.float16, device=A.device))
-        ws = workspace if workspace is not None else self.workspace(A.device)
+        ws = workspace if workspace is not None else self.workspace(A.device, stream)
         _lib.check(self._L.mm4_gemm_run(self._h, A.data_ptr(), B.data_ptr(), bias.data_ptr() if self.bias else None,
                                         C.data_ptr(), ws.data_ptr() if ws is not None else None,
                                         ws.numel() if ws is not None else 0, _lib.stream_handle(stream),
@@ -119,7 +121,7 @@ class GemmPlan:
         for name, h, shape in (("A", A, self.a_shape()), ("B", B, self.b_shape()), ("C", C, (d.M, d.N))):
             if h.is_cuda or h.dtype != torch.float16 or not h.is_contiguous() or tuple(h.shape) != tuple(shape):
                 raise ValueError(f"{name} must be a contiguous CPU fp16 tensor of shape {tuple(shape)}")
-        ws = workspace if workspace is not None else self.workspace(dA.device)
+        ws = workspace if workspace is not None else self.workspace(dA.device, stream)
         _lib.check(self._L.mm4_gemm_run_host(
             self._h, A.data_ptr(), B.data_ptr(), bias.data_ptr() if self.bias else None, C.data_ptr(),
             dA.data_ptr(), dB.data_ptr(), db.data_ptr() if self.bias else None, dC.data_ptr(),
@@ -135,7 +137,7 @@ class GemmPlan:
         _check_tensor(B, self.b_shape(), "B")
         if C32 is None:
             C32 = _lib.new_on_stream(stream, lambda: torch.empty((d.M, d.N), dtype=torch.float32, device=A.device))
-        ws = workspace if workspace is not None else self.workspace(A.device)
+        ws = workspace if workspace is not None else self.workspace(A.device, stream)
         _lib.check(self._L.mm4_gemm_partial_run(self._h, A.data_ptr(), B.data_ptr(), C32.data_ptr(),
                                                 ws.data_ptr() if ws is not None else None,
                                                 ws.numel() if ws is not None else 0, _lib.stream_handle(stream)))

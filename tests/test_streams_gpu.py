@@ -2,9 +2,10 @@
 current stream still writes."""
 import pytest
 
+from example_matmul_metal4_b200 import sync_check
 from example_matmul_metal4_b200.attention import AttentionDimensions, AttentionPlan
 from example_matmul_metal4_b200.conv import WEIGHTS_HWIO, WEIGHTS_OHWI, Conv2DDimensions, ConvPlan, permute_weights
-from example_matmul_metal4_b200.gemm import GEMMDimensions, GemmPlan, splitk_finalize
+from example_matmul_metal4_b200.gemm import BuildOptions, GEMMDimensions, GemmPlan, splitk_finalize
 
 pytestmark = pytest.mark.gpu
 
@@ -58,3 +59,27 @@ def test_memory_freed_on_the_current_stream_with_work_pending(cuda, name):
         torch.cuda.synchronize()
         for g, w in zip(got if isinstance(got, tuple) else (got,), want):
             assert torch.equal(g, w)
+
+
+def test_split_k_workspace_is_zeroed_before_its_first_run_on_another_stream(cuda):
+    """The zero fill of a plan's workspace must not wait behind work of the current stream that the run's stream does
+    not wait for. Small integers: fp32 sums are exact in any order."""
+    import torch
+    A = torch.randint(-2, 3, (256, 8192), device=cuda).half()
+    B = torch.randint(-2, 3, (512, 8192), device=cuda).half()
+    want = (A.float() @ B.float().T).half()
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(3):
+        plan = GemmPlan(GEMMDimensions(256, 512, 8192), bias=False, buildOptions=BuildOptions(splitK=8))
+        assert plan.workspace_bytes > 0
+        held = [torch.full((plan.workspace_bytes,), 77, dtype=torch.uint8, device=cuda) for _ in range(3)]
+        with torch.cuda.stream(side):
+            held += [torch.full((plan.workspace_bytes,), 77, dtype=torch.uint8, device=cuda) for _ in range(3)]
+        torch.cuda.synchronize()
+        del held
+        torch.cuda._sleep(20_000_000)  # about 10 ms
+        C = plan.run(A, B, stream=side)
+        torch.cuda.synchronize()
+        assert torch.equal(C, want)
+    sync_check()
